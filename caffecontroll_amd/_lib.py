@@ -9,6 +9,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libcct_hip.so")
 
 ROW_MAJOR, COL_MAJOR, NO_TRANS, TRANS = 101, 102, 111, 112
+F32, BF16 = 0, 1
 
 
 class CctHipError(RuntimeError):
@@ -55,6 +56,24 @@ class LrnBackwardArgs(C.Structure):
                 ("alpha_over_size", C.c_float), ("beta", C.c_float),
                 ("norm_window", C.c_int), ("local_size", C.c_int),
                 ("denoms", C.c_void_p), ("input_data", C.c_void_p), ("output_data", C.c_void_p)]
+
+
+class EmbeddingArgs(C.Structure):
+    """cct_embedding_args."""
+    _fields_ = [(n, C.c_int) for n in ("tokens", "width", "vocab", "dtype")] + \
+               [("scale", C.c_float), ("padding_id", C.c_int), ("table_stride", C.c_size_t), ("out_stride", C.c_size_t)]
+
+
+class VocabLossArgs(C.Structure):
+    """cct_vocab_loss_args."""
+    _fields_ = [(n, C.c_int) for n in ("tokens", "width", "vocab", "dtype", "ignore_label", "piece")] + \
+               [("x_stride", C.c_size_t), ("w_stride", C.c_size_t)]
+
+
+class DistillLossArgs(C.Structure):
+    """cct_distill_loss_args."""
+    _fields_ = [(n, C.c_int) for n in ("tokens", "vocab", "top", "dtype")] + \
+               [("temperature", C.c_float), ("logits_stride", C.c_size_t), ("top_stride", C.c_size_t)]
 
 
 _P, _I, _F, _Z, _U = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint
@@ -153,6 +172,17 @@ PROTOTYPES = {
     "cct_hip_softmax_loss_forward": [_P, _P, _P, _P, _I, _I],
     "cct_hip_softmax_loss_backward": [_P, _P, _P, _I, _I, _I],
     "cct_hip_softmax_loss_forward_backward": [_P, _P, _P, _P, _P, _I, _I, _I],
+    "cct_hip_embedding_forward": [_P, _P, _P, C.POINTER(EmbeddingArgs)],
+    "cct_hip_embedding_workspace_bytes": [C.POINTER(EmbeddingArgs)],
+    "cct_hip_embedding_backward": [_P, _P, _P, C.POINTER(EmbeddingArgs), _I, _P, _Z],
+    "cct_hip_vocab_loss_workspace_bytes": [C.POINTER(VocabLossArgs), _I],
+    "cct_hip_vocab_loss_forward": [_P, _P, _P, _P, _P, _P, C.POINTER(VocabLossArgs), _P, _Z],
+    "cct_hip_vocab_loss_backward": [_P] * 9 + [C.POINTER(VocabLossArgs), _P, _Z],
+    "cct_hip_vocab_loss_forward_backward": [_P] * 10 + [C.POINTER(VocabLossArgs), _P, _Z],
+    "cct_hip_distill_loss_workspace_bytes": [C.POINTER(DistillLossArgs)],
+    "cct_hip_distill_loss_forward": [_P] * 5 + [C.POINTER(DistillLossArgs), _P, _Z],
+    "cct_hip_distill_loss_backward": [_P] * 6 + [C.POINTER(DistillLossArgs), _P, _Z],
+    "cct_hip_distill_loss_forward_backward": [_P] * 7 + [C.POINTER(DistillLossArgs), _P, _Z],
     "cct_hip_timer_create": [C.POINTER(_P)],
     "cct_hip_timer_destroy": [_P],
     "cct_hip_timer_start": [_P],
@@ -162,6 +192,8 @@ PROTOTYPES = {
 _RESTYPE = {"cct_hip_last_error": C.c_char_p, "cct_hip_last_kernel": C.c_char_p, "cct_hip_conv_direct_slab_floats": C.c_size_t,
             "cct_hip_conv_direct_slab_floats_grouped": C.c_size_t,
             "cct_hip_conv_strided_slab_floats": C.c_size_t,
+            "cct_hip_embedding_workspace_bytes": C.c_size_t, "cct_hip_vocab_loss_workspace_bytes": C.c_size_t,
+            "cct_hip_distill_loss_workspace_bytes": C.c_size_t,
             "cct_hip_conv_strided_backward_data_slab_floats": C.c_size_t}
 
 _lib = None

@@ -1,0 +1,331 @@
+// Distillation loss from a teacher's top logits, on stored scores.
+//
+//   q = softmax(top_logits / T) over a token's list,  p = softmax(logits / T) over the vocabulary
+//   lse = log sum exp(logits / T),  loss = T^2 sum_k q_k (log q_k - logits[id_k] / T + lse)
+//   dlogits_v = loss_grad * T * (p_v - sum of q_k over id_k == v)
+//
+// Exponentials are v_exp_f32 of (difference * log2 e / T).  Bound by HBM: the scores are
+// read once for the loss; the list costs a few hundred bytes a token.
+#include "narrow.h"
+
+namespace cct {
+
+constexpr int DST_THREADS = 256;
+constexpr int DST_WAVES = DST_THREADS / 64;
+constexpr int DST_TOP_MAX = 1024;
+
+struct DistillShape {
+  int tokens, vocab, top;
+  float temperature, inv_t, scale2;  // T, 1 / T, log2(e) / T
+  size_t logits_stride, top_stride;
+  int splits, chunk;  // a row is cut into `splits` ranges of `chunk` elements
+};
+
+__device__ __forceinline__ SoftStat wave_join(SoftStat a, float scale2) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) a = shfl_xor_join(a, m, scale2);
+  return a;
+}
+
+// A vector of values on top of a running maximum and sum.
+template <int V>
+__device__ __forceinline__ void add_values(SoftStat &st, const float (&z)[V], float scale2) {
+  float m = st.m;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = fmaxf(m, z[i]);
+  const float base = m == neg_inf() ? 0.0f : m;  // nothing but -inf so far: 2^(-inf) = 0 without -inf - -inf
+  float s = st.s * (st.m == m ? 1.0f : exp2_fast((st.m - base) * scale2));
+#pragma unroll
+  for (int i = 0; i < V; ++i) s += exp2_fast((z[i] - base) * scale2);
+  st.m = m;
+  st.s = s;
+}
+
+// Maximum and sum of one range of one token's scores.
+template <class T>
+__global__ __launch_bounds__(DST_THREADS) void distill_stats_kernel(SoftStat *__restrict__ part,
+                                                                    const T *__restrict__ logits, DistillShape s) {
+  constexpr int V = Num<T>::V;
+  __shared__ SoftStat sh[DST_WAVES];
+  const int t = blockIdx.x / s.splits, cut = blockIdx.x % s.splits;
+  const T *row = logits + (size_t)t * s.logits_stride;
+  const int end = min(s.vocab, (cut + 1) * s.chunk);
+  SoftStat st{neg_inf(), 0.0f};
+  for (int col = cut * s.chunk + threadIdx.x * V; col < end; col += DST_THREADS * V) {
+    float z[V];
+    load_vec<T>(z, row, col, s.vocab);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = col + i < end ? z[i] : neg_inf();
+    add_values<V>(st, z, s.scale2);
+  }
+  st = wave_join(st, s.scale2);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < DST_WAVES; ++w) st = join(st, sh[w], s.scale2);
+    part[blockIdx.x] = st;
+  }
+}
+
+// softmax(logits / T) of one score; the difference is formed before log2 e is applied
+__device__ __forceinline__ float probability(float score, float lse, const DistillShape &s) {
+  return exp2_fast(__builtin_fmaf(score, s.inv_t, -lse) * kLog2e);
+}
+
+// The teacher's distribution of one token, by one wavefront: lane l holds entries l, l + 64, ...
+struct Teacher {
+  float m, s;   // maximum and sum over the valid entries
+  bool bad;     // an entry names a row outside the vocabulary
+};
+__device__ __forceinline__ Teacher teacher_stats(const int *__restrict__ ids, const float *__restrict__ top, int n,
+                                                 int vocab, float scale2, int lane) {
+  SoftStat st{neg_inf(), 0.0f};
+  bool bad = false;
+  for (int k = lane; k < n; k += 64) {
+    const int id = ids[k];
+    bad |= id >= vocab;
+    float z[1] = {id >= 0 ? top[k] : neg_inf()};
+    add_values<1>(st, z, scale2);
+  }
+  st = wave_join(st, scale2);
+  return Teacher{st.m, st.s, __any(bad) != 0};
+}
+
+// q of one entry; 0 where it has no weight
+__device__ __forceinline__ float teacher_weight(const Teacher &te, int id, float top, float scale2) {
+  if (id < 0 || te.m == neg_inf()) return 0.0f;
+  return exp2_fast((top - te.m) * scale2) / te.s;
+}
+
+// Joins a token's ranges and computes its loss: one wavefront per token.
+template <class T>
+__device__ __forceinline__ void distill_loss_wave(float *__restrict__ loss, float *__restrict__ lse, SoftStat st,
+                                                  const T *__restrict__ row, const int *__restrict__ ids,
+                                                  const float *__restrict__ top, const DistillShape &s, int t, int lane) {
+  const float l = log_sum(st, s.inv_t);
+  const Teacher te = teacher_stats(ids, top, s.top, s.vocab, s.scale2, lane);
+  const float logs = __builtin_log2f(te.s) * kLn2;
+  float sum = 0.0f;
+  for (int k = lane; k < s.top; k += 64) {
+    const int id = ids[k];
+    const float q = teacher_weight(te, id, top[k], s.scale2);
+    if (q != 0.0f && id < s.vocab) {
+      const float logp = __builtin_fmaf((float)row[id], s.inv_t, -l);
+      sum += q * (((top[k] - te.m) * s.inv_t - logs) - logp);
+    }
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  if (lane == 0) {
+    lse[t] = l;
+    loss[t] = te.bad ? __builtin_nanf("") : s.temperature * s.temperature * sum;
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(DST_THREADS) void distill_loss_kernel(float *__restrict__ loss, float *__restrict__ lse,
+                                                                   const SoftStat *__restrict__ part,
+                                                                   const T *__restrict__ logits,
+                                                                   const int *__restrict__ ids,
+                                                                   const float *__restrict__ top, DistillShape s) {
+  const int t = blockIdx.x * DST_WAVES + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= s.tokens) return;
+  SoftStat st{neg_inf(), 0.0f};
+  for (int i = lane; i < s.splits; i += 64) st = join(st, part[(size_t)t * s.splits + i], s.scale2);
+  st = wave_join(st, s.scale2);
+  distill_loss_wave<T>(loss, lse, st, logits + (size_t)t * s.logits_stride, ids + (size_t)t * s.top_stride,
+                       top + (size_t)t * s.top_stride, s, t, lane);
+}
+
+// q of every entry into LDS, the weight of equal ids gathered at the first of them (-1 in `at` for the others and for
+// entries outside [begin, end)); returns whether the token has any weight at all.  All lanes of the workgroup call it.
+template <class T>
+__device__ __forceinline__ bool gather_entries(int *at, float *q, float *z, const T *__restrict__ row,
+                                               const int *__restrict__ ids, const float *__restrict__ top, int begin,
+                                               int end, const DistillShape &s) {
+  const int threads = blockDim.x, tid = threadIdx.x;
+  // every wavefront computes the statistics by itself: the list is short, and no exchange is needed
+  const Teacher te = teacher_stats(ids, top, s.top, s.vocab, s.scale2, tid & 63);
+  for (int k = tid; k < s.top; k += threads) {
+    const int id = ids[k];
+    const float w = teacher_weight(te, id, top[k], s.scale2);
+    const bool here = id >= begin && id < end && w != 0.0f;
+    at[k] = here ? id : -1;
+    q[k] = w;
+    z[k] = here ? (float)row[id] : 0.0f;
+  }
+  __syncthreads();
+  float total[DST_TOP_MAX / 64];
+  int n = 0;
+  for (int k = tid; k < s.top; k += threads, ++n) {
+    const int id = at[k];
+    float sum = 0.0f;
+    bool first = id >= 0;
+    if (first)
+      for (int j = 0; j < s.top; ++j)
+        if (at[j] == id) {
+          first = first && j >= k;
+          sum += q[j];
+        }
+    total[n] = first ? sum : -1.0f;
+  }
+  __syncthreads();
+  n = 0;
+  for (int k = tid; k < s.top; k += threads, ++n) {
+    if (total[n] < 0.0f) at[k] = -1;
+    q[k] = total[n];
+  }
+  __syncthreads();
+  return te.m != neg_inf();
+}
+
+// The gradient of one range of one token's scores.
+template <class T>
+__global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, const T *logits,
+                                                                   const int *__restrict__ ids,
+                                                                   const float *__restrict__ top,
+                                                                   const float *__restrict__ lse,
+                                                                   const float *__restrict__ loss_grad, DistillShape s) {
+  constexpr int V = Num<T>::V;
+  extern __shared__ float lists[];
+  int *at = (int *)lists;
+  float *q = lists + s.top, *z = q + s.top;
+  const int t = blockIdx.x / s.splits, cut = blockIdx.x % s.splits;
+  const int begin = cut * s.chunk, end = min(s.vocab, begin + s.chunk);
+  const T *row = logits + (size_t)t * s.logits_stride;
+  T *dst = dlogits + (size_t)t * s.logits_stride;
+  const bool weight = gather_entries<T>(at, q, z, row, ids + (size_t)t * s.top_stride, top + (size_t)t * s.top_stride, begin,
+                                        end, s);
+  const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f), l = lse[t];
+  for (int col = begin + threadIdx.x * V; col < end; col += DST_THREADS * V) {
+    float f[V];
+    load_vec<T>(f, row, col, end);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = weight ? g * probability(f[i], l, s) : 0.0f;
+    store_vec<T>(dst, f, col, end);
+  }
+  if (!weight) return;
+  __syncthreads();  // the entries of the list on top of what the row's lanes wrote
+  for (int k = threadIdx.x; k < s.top; k += DST_THREADS)
+    if (at[k] >= 0) dst[at[k]] = (T)(g * (probability(z[k], l, s) - q[k]));
+}
+
+static int check_distill(const cct_distill_loss_args *a, const char *who) {
+  CCT_REQUIRE(a != nullptr, "%s: null argument block", who);
+  CCT_REQUIRE(a->dtype == CCT_F32 || a->dtype == CCT_BF16, "%s: dtype %d is neither CCT_F32 nor CCT_BF16", who, a->dtype);
+  CCT_REQUIRE(a->tokens >= 0 && a->vocab > 0 && a->top > 0, "%s: tokens %d, vocab %d, top %d", who, a->tokens, a->vocab,
+              a->top);
+  CCT_REQUIRE(a->top <= DST_TOP_MAX, "%s: top %d is above %d", who, a->top, DST_TOP_MAX);
+  CCT_REQUIRE(a->tokens <= (1 << 20) && a->vocab <= (1 << 26), "%s: tokens %d, vocab %d: at most 2^20, 2^26", who,
+              a->tokens, a->vocab);
+  CCT_REQUIRE(a->temperature > 0.0f && a->temperature < __builtin_inff(), "%s: temperature %g is not a positive number", who,
+              (double)a->temperature);
+  CCT_REQUIRE((a->logits_stride == 0 || a->logits_stride >= (size_t)a->vocab) &&
+                  (a->top_stride == 0 || a->top_stride >= (size_t)a->top),
+              "%s: a row stride is smaller than its row", who);
+  return 0;
+}
+
+static DistillShape distill_shape(const cct_distill_loss_args *a) {
+  DistillShape s;
+  s.tokens = a->tokens;
+  s.vocab = a->vocab;
+  s.top = a->top;
+  s.temperature = a->temperature;
+  s.inv_t = (float)(1.0 / (double)a->temperature);
+  s.scale2 = (float)(1.4426950408889634 / (double)a->temperature);
+  s.logits_stride = a->logits_stride ? a->logits_stride : (size_t)a->vocab;
+  s.top_stride = a->top_stride ? a->top_stride : (size_t)a->top;
+  // enough ranges to give each of 256 CUs several workgroups, none shorter than 4096 elements
+  const int per = 8192 / (a->tokens > 0 ? a->tokens : 1) + 1;
+  int splits = (a->vocab + 4095) / 4096;
+  if (splits > per) splits = per;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  const int chunk = (a->vocab + splits - 1) / splits;
+  s.chunk = (chunk + 7) & ~7;
+  s.splits = (a->vocab + s.chunk - 1) / s.chunk;
+  return s;
+}
+
+static size_t distill_bytes(const cct_distill_loss_args *a) {
+  const DistillShape s = distill_shape(a);
+  return (size_t)s.tokens * s.splits * sizeof(SoftStat);
+}
+
+template <class T>
+static int distill_forward(float *loss, float *lse, const void *logits, const int *ids, const float *top,
+                           const DistillShape &s, void *ws) {
+  hipStream_t st = ctx().stream;
+  SoftStat *part = (SoftStat *)ws;
+  distill_stats_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 0, st>>>(part, (const T *)logits, s);
+  CCT_LAUNCH_CHECK();
+  distill_loss_kernel<T><<<(s.tokens + DST_WAVES - 1) / DST_WAVES, DST_THREADS, 0, st>>>(loss, lse, part,
+                                                                                       (const T *)logits, ids, top, s);
+  CCT_LAUNCH_CHECK();
+  note_kernel("distill_stats_kernel<%s> splits=%d", Num<T>::NAME, s.splits);
+  return 0;
+}
+
+template <class T>
+static int distill_backward(void *dlogits, const void *logits, const int *ids, const float *top, const float *lse,
+                            const float *loss_grad, const DistillShape &s) {
+  distill_grad_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 3 * s.top * sizeof(float), ctx().stream>>>(
+      (T *)dlogits, (const T *)logits, ids, top, lse, loss_grad, s);
+  CCT_LAUNCH_CHECK();
+  note_kernel("distill_grad_kernel<%s> splits=%d", Num<T>::NAME, s.splits);
+  return 0;
+}
+
+static int check_distill_workspace(const cct_distill_loss_args *a, const void *ws, size_t bytes, const char *who) {
+  const size_t need = distill_bytes(a);
+  CCT_REQUIRE(bytes >= need && (ws || need == 0) && ((uintptr_t)ws & 15) == 0,
+              "%s: the workspace holds %zu bytes and starts at %p; it needs %zu, aligned to 16", who, bytes, ws, need);
+  return 0;
+}
+
+}  // namespace cct
+
+using namespace cct;
+
+extern "C" size_t cct_hip_distill_loss_workspace_bytes(const cct_distill_loss_args *args) {
+  return check_distill(args, "distill_loss_workspace_bytes") ? 0 : distill_bytes(args);
+}
+
+extern "C" int cct_hip_distill_loss_forward(float *loss, float *lse, const void *logits, const int *top_ids,
+                                            const float *top_logits, const cct_distill_loss_args *args, void *workspace,
+                                            size_t workspace_bytes) {
+  if (int rc = check_distill(args, "distill_loss_forward")) return rc;
+  if (args->tokens == 0) return 0;
+  CCT_REQUIRE(loss && lse && logits && top_ids && top_logits, "distill_loss_forward: null array");
+  if (int rc = check_distill_workspace(args, workspace, workspace_bytes, "distill_loss_forward")) return rc;
+  CCT_ENSURE_INIT();
+  const DistillShape s = distill_shape(args);
+  return args->dtype == CCT_BF16 ? distill_forward<bf16>(loss, lse, logits, top_ids, top_logits, s, workspace)
+                                 : distill_forward<float>(loss, lse, logits, top_ids, top_logits, s, workspace);
+}
+
+extern "C" int cct_hip_distill_loss_backward(void *dlogits, const void *logits, const int *top_ids, const float *top_logits,
+                                             const float *lse, const float *loss_grad, const cct_distill_loss_args *args,
+                                             void *workspace, size_t workspace_bytes) {
+  if (int rc = check_distill(args, "distill_loss_backward")) return rc;
+  if (args->tokens == 0) return 0;
+  CCT_REQUIRE(dlogits && lse && logits && top_ids && top_logits, "distill_loss_backward: null array");
+  if (int rc = check_distill_workspace(args, workspace, workspace_bytes, "distill_loss_backward")) return rc;
+  CCT_ENSURE_INIT();
+  const DistillShape s = distill_shape(args);
+  return args->dtype == CCT_BF16 ? distill_backward<bf16>(dlogits, logits, top_ids, top_logits, lse, loss_grad, s)
+                                 : distill_backward<float>(dlogits, logits, top_ids, top_logits, lse, loss_grad, s);
+}
+
+extern "C" int cct_hip_distill_loss_forward_backward(float *loss, float *lse, void *dlogits, const void *logits,
+                                                     const int *top_ids, const float *top_logits, const float *loss_grad,
+                                                     const cct_distill_loss_args *args, void *workspace,
+                                                     size_t workspace_bytes) {
+  CCT_REQUIRE(dlogits || !args || args->tokens == 0, "distill_loss_forward_backward: null array");
+  if (int rc = cct_hip_distill_loss_forward(loss, lse, logits, top_ids, top_logits, args, workspace, workspace_bytes))
+    return rc;
+  return cct_hip_distill_loss_backward(dlogits, logits, top_ids, top_logits, lse, loss_grad, args, workspace,
+                                       workspace_bytes);
+}

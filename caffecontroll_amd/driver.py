@@ -5,11 +5,12 @@
 import ctypes as C
 
 from . import _lib
-from ._lib import (COL_MAJOR, NO_TRANS, ROW_MAJOR, TRANS, InverseLowerCubeArgs, LrnBackwardArgs,
-                   LrnForwardArgs, LrnForwardNormalizeArgs, PMapHelper, PoolArgs, check)
+from ._lib import (BF16, COL_MAJOR, F32, NO_TRANS, ROW_MAJOR, TRANS, DistillLossArgs, EmbeddingArgs,
+                   InverseLowerCubeArgs, LrnBackwardArgs, LrnForwardArgs, LrnForwardNormalizeArgs, PMapHelper, PoolArgs,
+                   VocabLossArgs, check)
 
-__all__ = ["HIPDriver", "conv_pmap", "lift_args", "remap_pmap", "ROW_MAJOR", "COL_MAJOR",
-           "NO_TRANS", "TRANS"]
+__all__ = ["HIPDriver", "conv_pmap", "lift_args", "remap_pmap", "embedding_args", "vocab_loss_args", "distill_loss_args",
+           "ROW_MAJOR", "COL_MAJOR", "NO_TRANS", "TRANS", "F32", "BF16"]
 
 
 def _p(x):
@@ -52,6 +53,21 @@ def remap_pmap(R, Cc, depth, batch):
     a.dBR, a.dBC = R, Cc
     a.sBR, a.sBC = min(16, R), min(16, Cc)
     return a
+
+
+def embedding_args(tokens, width, vocab, dtype=F32, scale=1.0, padding_id=-1, table_stride=0, out_stride=0):
+    """cct_embedding_args of include/cct_hip.h; strides in elements, 0 = dense rows."""
+    return EmbeddingArgs(tokens, width, vocab, dtype, scale, padding_id, table_stride, out_stride)
+
+
+def vocab_loss_args(tokens, width, vocab, dtype=F32, ignore_label=-1, piece=0, x_stride=0, w_stride=0):
+    """cct_vocab_loss_args of include/cct_hip.h; strides in elements, 0 = dense rows."""
+    return VocabLossArgs(tokens, width, vocab, dtype, ignore_label, piece, x_stride, w_stride)
+
+
+def distill_loss_args(tokens, vocab, top, dtype=F32, temperature=1.0, logits_stride=0, top_stride=0):
+    """cct_distill_loss_args of include/cct_hip.h; strides in elements, 0 = dense rows."""
+    return DistillLossArgs(tokens, vocab, top, dtype, temperature, logits_stride, top_stride)
 
 
 class HIPDriver:
@@ -358,6 +374,57 @@ class HIPDriver:
     def softmax_loss_backward(self, in_grad, prob, labels, len_per_image, batch, spatial=1):
         check(self.lib.cct_hip_softmax_loss_backward(_p(in_grad), _p(prob), _p(labels), len_per_image,
                                                      batch, spatial), "softmax_loss_backward")
+
+    # -- the vocabulary ends of a model (see include/cct_hip.h; args from embedding_args() and its siblings) ---
+    def embedding_forward(self, out, table, ids, args):
+        check(self.lib.cct_hip_embedding_forward(_p(out), _p(table), _p(ids), args), "embedding_forward")
+
+    def embedding_workspace_bytes(self, args):
+        return self.lib.cct_hip_embedding_workspace_bytes(args)
+
+    def embedding_backward(self, dtable, dout, ids, args, workspace, workspace_bytes, accumulate=False):
+        """accumulate: add to what dtable holds and leave rows without tokens alone, else write every row."""
+        check(self.lib.cct_hip_embedding_backward(_p(dtable), _p(dout), _p(ids), args, int(accumulate), _p(workspace),
+                                                  workspace_bytes), "embedding_backward")
+
+    def vocab_loss_workspace_bytes(self, args, training=True):
+        return self.lib.cct_hip_vocab_loss_workspace_bytes(args, int(training))
+
+    def vocab_loss_forward(self, loss, lse, x, w, bias, labels, args, workspace, workspace_bytes):
+        check(self.lib.cct_hip_vocab_loss_forward(_p(loss), _p(lse), _p(x), _p(w), _p(bias), _p(labels), args,
+                                                  _p(workspace), workspace_bytes), "vocab_loss_forward")
+
+    def vocab_loss_backward(self, dx, dw, db, x, w, bias, labels, lse, loss_grad, args, workspace, workspace_bytes):
+        check(self.lib.cct_hip_vocab_loss_backward(_p(dx), _p(dw), _p(db), _p(x), _p(w), _p(bias), _p(labels), _p(lse),
+                                                   _p(loss_grad), args, _p(workspace), workspace_bytes),
+              "vocab_loss_backward")
+
+    def vocab_loss_forward_backward(self, loss, lse, dx, dw, db, x, w, bias, labels, loss_grad, args, workspace,
+                                    workspace_bytes):
+        """The forward pass and the gradients in one call."""
+        check(self.lib.cct_hip_vocab_loss_forward_backward(_p(loss), _p(lse), _p(dx), _p(dw), _p(db), _p(x), _p(w),
+                                                           _p(bias), _p(labels), _p(loss_grad), args, _p(workspace),
+                                                           workspace_bytes), "vocab_loss_forward_backward")
+
+    def distill_loss_workspace_bytes(self, args):
+        return self.lib.cct_hip_distill_loss_workspace_bytes(args)
+
+    def distill_loss_forward(self, loss, lse, logits, top_ids, top_logits, args, workspace, workspace_bytes):
+        check(self.lib.cct_hip_distill_loss_forward(_p(loss), _p(lse), _p(logits), _p(top_ids), _p(top_logits), args,
+                                                    _p(workspace), workspace_bytes), "distill_loss_forward")
+
+    def distill_loss_backward(self, dlogits, logits, top_ids, top_logits, lse, loss_grad, args, workspace,
+                              workspace_bytes):
+        check(self.lib.cct_hip_distill_loss_backward(_p(dlogits), _p(logits), _p(top_ids), _p(top_logits), _p(lse),
+                                                     _p(loss_grad), args, _p(workspace), workspace_bytes),
+              "distill_loss_backward")
+
+    def distill_loss_forward_backward(self, loss, lse, dlogits, logits, top_ids, top_logits, loss_grad, args, workspace,
+                                      workspace_bytes):
+        """The forward pass and the gradient in one call."""
+        check(self.lib.cct_hip_distill_loss_forward_backward(_p(loss), _p(lse), _p(dlogits), _p(logits), _p(top_ids),
+                                                             _p(top_logits), _p(loss_grad), args, _p(workspace),
+                                                             workspace_bytes), "distill_loss_forward_backward")
 
     # -- timing -----------------------------------------------------------------------------
     def timer(self):

@@ -514,6 +514,93 @@ int cct_hip_softmax_loss_forward_backward(float *prob, float *in_grad, const flo
 int cct_hip_softmax_loss_backward(float *in_grad, const float *prob, const float *labels,
                                   int len_per_image, int batch, int spatial);
 
+/* ---- the vocabulary ends of a model: embedding, vocabulary loss, distillation ----------------- */
+/* Operators for models whose inputs and answers are entries of a large vocabulary.  They have no counterpart in the
+ * reference; they stand beside the inner-product layer (cct_hip_sgemm_new_bias) and the softmax loss
+ * (cct_hip_softmax_loss_forward), take matrices of fp32 or bf16 elements (every sum, softmax statistic and exponential in
+ * fp32, one rounding where a result is stored), 32-bit ids and labels, rows `stride` elements apart (0 = dense; what
+ * lies between the rows is neither read nor written), and a workspace of the caller's: it may hold anything before the
+ * call, must not be shared by calls that run at the same time, and nothing in it is needed after the call, so a captured graph
+ * and an eager call, or two graphs, are independent as soon as their workspaces are.  Workspaces start at a multiple
+ * of 16 bytes.  Results do not depend on timing: no floating-point atomics, fixed orders of summation.  Arguments
+ * are checked before anything is enqueued (CCT_HIP_EINVAL). */
+enum { CCT_F32 = 0, CCT_BF16 = 1 };
+
+/* Embedding: out[t] = scale * table[ids[t]] for t < tokens.  An id equal to padding_id gives a row of zeros and
+ * receives no gradient; any other id outside [0, vocab) is never used as an index: its row becomes NaN, and it
+ * receives no gradient.  (padding_id itself may be a valid row, which is then never read.) */
+typedef struct cct_embedding_args {
+  int tokens, width, vocab;
+  int dtype; /* of table, out, dtable and dout */
+  float scale;
+  int padding_id;
+  size_t table_stride, out_stride; /* elements between rows of table / dtable and of out / dout; 0 = width */
+} cct_embedding_args;
+int cct_hip_embedding_forward(void *out, const void *table, const int *ids, const cct_embedding_args *args);
+/* dtable[v] = scale * sum of dout[t] over the tokens with ids[t] == v, in the order of the tokens (long runs of one id
+ * in pieces that are added in order).  accumulate == 0: every row of dtable is written, zero where no token has the
+ * id.  accumulate != 0: the sum is added to what the row holds (in fp32, rounded once), and rows without tokens are
+ * left as they are -- for a table that is also the vocabulary loss's weight matrix, on top of its dw. */
+size_t cct_hip_embedding_workspace_bytes(const cct_embedding_args *args);
+int cct_hip_embedding_backward(void *dtable, const void *dout, const int *ids, const cct_embedding_args *args,
+                               int accumulate, void *workspace, size_t workspace_bytes);
+
+/* Vocabulary loss: the inner product l[t] = w x[t] + bias (w [vocab][width], bias [vocab] or NULL) and the softmax loss
+ * on it, in pieces of the vocabulary and without keeping the scores l:
+ *   lse[t] = log sum_v exp l[t][v],  loss[t] = lse[t] - l[t][labels[t]].
+ * A token whose label is ignore_label has loss 0 and takes no part in any gradient (its row of x may hold anything);
+ * its lse is still computed.  Any other label outside [0, vocab) is never used as an index: that token's loss is NaN, and its
+ * gradient is that of the lse alone, as in cct_hip_softmax_loss_backward.  A bias of -inf masks its row of the vocabulary.
+ * Gradients for G[t][v] = loss_grad[t] * (exp(l[t][v] - lse[t]) - [v == labels[t]]), loss_grad NULL = all ones:
+ *   dx = G w,  dw = G^T x,  db = column sums of G;  any of the three may be NULL.
+ * In bf16, G is rounded to bf16 as an operand of the two products (as an inner-product layer's output gradient
+ * is); everything else stays in fp32 up to the final store.
+ * forward_backward gives what forward and then backward give; while tokens * vocab * 4 bytes stay within 512 MiB it
+ * keeps the fp32 scores in the workspace from one to the other instead of computing them twice. */
+typedef struct cct_vocab_loss_args {
+  int tokens, width, vocab;
+  int dtype; /* of x, w, bias and their gradients */
+  int ignore_label;
+  int piece; /* rows of w taken at a time, rounded up to a multiple of 256; 0 = automatic.  A smaller piece needs less workspace */
+  size_t x_stride, w_stride; /* elements between rows of x / dx and of w / dw; 0 = width */
+} cct_vocab_loss_args;
+/* Bytes for the forward pass alone (training == 0) or for any of the three calls (training != 0); 0 for arguments that
+ * the calls refuse. */
+size_t cct_hip_vocab_loss_workspace_bytes(const cct_vocab_loss_args *args, int training);
+int cct_hip_vocab_loss_forward(float *loss, float *lse, const void *x, const void *w, const void *bias, const int *labels,
+                               const cct_vocab_loss_args *args, void *workspace, size_t workspace_bytes);
+int cct_hip_vocab_loss_backward(void *dx, void *dw, void *db, const void *x, const void *w, const void *bias,
+                                const int *labels, const float *lse, const float *loss_grad,
+                                const cct_vocab_loss_args *args, void *workspace, size_t workspace_bytes);
+int cct_hip_vocab_loss_forward_backward(float *loss, float *lse, void *dx, void *dw, void *db, const void *x, const void *w,
+                                        const void *bias, const int *labels, const float *loss_grad,
+                                        const cct_vocab_loss_args *args, void *workspace, size_t workspace_bytes);
+
+/* Distillation from a teacher's top logits: per token a list of `top` vocabulary entries and the teacher's logits for
+ * them.  With T the temperature, q = softmax(top_logits / T) over the list and p = softmax(logits / T) over the
+ * vocabulary:
+ *   lse[t] = log sum_v exp(logits[t][v] / T),  loss[t] = T^2 * sum_k q_k (log q_k - log p[top_ids[k]]),
+ *   dlogits[t][v] = loss_grad[t] * T * (p_v - sum of q_k over top_ids[k] == v),  loss_grad NULL = all ones.
+ * An entry with a negative id is absent (lists of different lengths); one with a top logit of -inf has no weight.
+ * A token without any entry of weight has loss 0 and gradient 0.  An id of vocab or above is never used as an index: that
+ * token's loss is NaN, and the gradient subtracts nothing for it.  An id may appear more than once.  dlogits may be
+ * logits itself. */
+typedef struct cct_distill_loss_args {
+  int tokens, vocab, top; /* top <= 1024 */
+  int dtype;              /* of logits and dlogits; top_logits are fp32 */
+  float temperature;
+  size_t logits_stride, top_stride; /* elements between rows of logits / dlogits and of both top lists; 0 = dense */
+} cct_distill_loss_args;
+size_t cct_hip_distill_loss_workspace_bytes(const cct_distill_loss_args *args);
+int cct_hip_distill_loss_forward(float *loss, float *lse, const void *logits, const int *top_ids, const float *top_logits,
+                                 const cct_distill_loss_args *args, void *workspace, size_t workspace_bytes);
+int cct_hip_distill_loss_backward(void *dlogits, const void *logits, const int *top_ids, const float *top_logits,
+                                  const float *lse, const float *loss_grad, const cct_distill_loss_args *args,
+                                  void *workspace, size_t workspace_bytes);
+int cct_hip_distill_loss_forward_backward(float *loss, float *lse, void *dlogits, const void *logits, const int *top_ids,
+                                          const float *top_logits, const float *loss_grad,
+                                          const cct_distill_loss_args *args, void *workspace, size_t workspace_bytes);
+
 /* ---- timing on the library's stream (used by the harness; hipEvent based) ---------------- */
 int cct_hip_timer_create(void **timer);
 int cct_hip_timer_destroy(void *timer);
