@@ -38,6 +38,8 @@ static void read_tuning_from_env() {
   g_tuning.gemm_nt = geti("CCT_HIP_GEMM_NT", 0);
   g_tuning.gemm_tile = geti("CCT_HIP_GEMM_TILE", -1);
   g_tuning.gemm_nodma = geti("CCT_HIP_GEMM_NODMA", 0);
+  g_tuning.vocab_tile = geti("CCT_HIP_VOCAB_TILE", 0);
+  g_tuning.vocab_keep = geti("CCT_HIP_VOCAB_KEEP", 0);
 }
 
 // per host thread, like the error text: a launch on one thread never rewrites what another thread reads
@@ -170,7 +172,8 @@ int cct_hip_set_tuning(const char *name, int value) {
       {"direct_tile", &t.direct_tile}, {"direct_waves", &t.direct_waves}, {"direct_tb", &t.direct_tb},
       {"direct_nospec", &t.direct_nospec}, {"direct_splits", &t.direct_splits}, {"direct_alds", &t.direct_alds},
       {"direct_wgrad_rows", &t.direct_wgrad_rows}, {"conv1x1_per_image", &t.conv1x1_per_image}, {"strided_wgrad", &t.strided_wgrad}, {"pool_plane", &t.pool_plane}, {"gemm_nt", &t.gemm_nt},
-      {"gemm_tile", &t.gemm_tile}, {"gemm_nodma", &t.gemm_nodma}};
+      {"gemm_tile", &t.gemm_tile}, {"gemm_nodma", &t.gemm_nodma}, {"vocab_tile", &t.vocab_tile},
+      {"vocab_keep", &t.vocab_keep}};
   for (const auto &e : table)
     if (!strcmp(e.name, name)) {
       *e.field = value;

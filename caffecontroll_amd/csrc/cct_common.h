@@ -27,7 +27,7 @@ struct Context {
 
 // Tuning overrides, for experiments and for tests that pin a kernel instance.  Read ONCE from the
 // environment when the library initialises (CCT_HIP_DIRECT_TILE, _DIRECT_WAVES, _DIRECT_TB,
-// _DIRECT_NOSPEC, _DIRECT_SPLITS, _DIRECT_ALDS, _DIRECT_WGRAD_ROWS, _STRIDED_WGRAD, _POOL_PLANE, _GEMM_NT, _GEMM_TILE, _GEMM_NODMA), changed afterwards only through
+// _DIRECT_NOSPEC, _DIRECT_SPLITS, _DIRECT_ALDS, _DIRECT_WGRAD_ROWS, _STRIDED_WGRAD, _POOL_PLANE, _GEMM_NT, _GEMM_TILE, _GEMM_NODMA, _VOCAB_TILE, _VOCAB_KEEP), changed afterwards only through
 // cct_hip_set_tuning(); the launch paths read this struct, never the environment.
 struct Tuning {
   int direct_tile = 0;    // "<map blocks><pixel blocks>" of conv_direct_kernel, 0 = model's choice
@@ -42,6 +42,8 @@ struct Tuning {
   int pool_plane = 0;     // 1: plane-tiled pooling kernels at any size
   int gemm_nt = 0;        // 1: non-temporal stores in the GEMM epilogue
   int gemm_tile = -1;     // index of the GEMM tile shape, -1 = model's choice
+  int vocab_tile = 0;     // vocabulary loss: tile of its products, 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 = 64 x 32, 0 = model's choice
+  int vocab_keep = 0;     // vocabulary loss: 1 = scores kept where they fit the limit, 2 = never, 0 = model's choice
   int gemm_nodma = 0;     // 1: GEMM operand tiles always staged through registers
 };
 Tuning &tuning();

@@ -1,18 +1,21 @@
 // Vocabulary loss: the softmax loss of an inner-product layer with a large vocabulary of outputs, without its scores.
 //
 //   l[t][v] = x[t] . w[v] + bias[v]      lse[t] = log sum_v exp l[t][v]      loss[t] = lse[t] - l[t][label[t]]
-//   G[t][v] = exp(l[t][v] - lse[t]) - [v == label[t]]
-//   dx[t] = g[t] * sum_v G[t][v] w[v]    dw[v] = sum_t g[t] G[t][v] x[t]     db[v] = sum_t g[t] G[t][v]
+//   G[t][v] = r[t] * (exp(l[t][v] - lse[t]) - [v == label[t]]),  r[t] = loss_grad[t] / c,  c = max |loss_grad|
+//   dx[t] = c * sum_v G[t][v] w[v]       dw[v] = c * sum_t G[t][v] x[t]      db[v] = c * sum_t G[t][v]
 //
-// Every product is one kernel, C[m][n] = sum_k A[m][k] B[n][k] with both operands contiguous along k, and four ways to
-// use a finished tile:
-//   STATS  m = vocabulary, n = token: maximum and sum of the tile's scores per token (a few bytes instead of the tile), the
-//          label's score, and the scores themselves where the caller keeps them for the gradient;
-//   GRAD   the same product again with lse known: G of a piece of the vocabulary, written as G[t][v] (the operand of dx)
-//          and as g[t] G[t][v] transposed (the operand of dw), and the column sums for db;
-//   SLAB   m = width, n = token, k = the piece's vocabulary: dx in fp32, added up over the pieces;
+// G is what bf16 products take as an operand, so it is rounded once.  The weights enter it relative to the largest of
+// them: equal weights (a mean over tokens) are then exactly 1 and add no rounding of their own, which would be the
+// same for every token and not average out.
+//
+// Every product is one kernel, C[m][n] = sum_k A[m][k] B[n][k], with operands that are contiguous along k or along
+// their rows, and four ways to use a finished tile:
+//   STATS  m = vocabulary, n = token: maximum and sum of the tile's scores per token (a few bytes instead of the tile) and
+//          the label's score;
+//   GRAD   the same product again with lse known: G of a piece of the vocabulary and the column sums for db;
+//   SLAB   fp32 parts of a result, cut along k and added up by a later kernel: dx over the pieces (m = width, n = token,
+//          k = vocabulary), and scores that are kept;
 //   OUT    m = width, n = vocabulary, k = token: dw of the piece, stored once in its own type.
-// The k-contiguous forms of w and x that the last two need (w piece and x transposed) are made by a copy kernel.
 //
 // Bound: matrix-core rate.  2 tokens*width*vocab operations for the loss, 4 more for the gradients and 2 for the scores
 // again where they were not kept.
@@ -24,12 +27,10 @@
 namespace cct {
 
 // ---- the product kernel ----------------------------------------------------------------------------------------
-// A workgroup owns a BM x BN tile of C and walks k in steps of 128 bytes (64 bf16 or 32 fp32 elements) through two LDS
-// stages.  Rows of a stage are 128 bytes, 16-byte chunk c of row r lies in slot c ^ ((r >> 1) & 7): the 16 lanes of a
-// fragment read (16 rows, one chunk) then touch all 64 banks once.  global -> LDS copies cannot permute what a lane
-// receives, so the lane that fills slot s of row r fetches chunk s ^ ((r >> 1) & 7).
-// Fragments of v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: lane l holds 16 bytes of row l % 16, chunk l / 16
-// of a 64-byte group; C element r of lane l is row 4 * (l / 16) + r, column l % 16.  For fp32 the four elements of a
+// A workgroup owns a BM x BN tile of C and walks k in steps of 64 bf16 or 32 fp32 elements through two LDS stages that
+// global -> LDS copies fill, 1 KB a wavefront at a time.
+// Fragments of v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: lane l holds 16 bytes of row l % 16, elements
+// along k of chunk l / 16; C element r of lane l is row 4 * (l / 16) + r, column l % 16.  For fp32 the four elements of a
 // chunk feed four MFMAs (the sum over k may run in any order as long as both operands use the same one).
 enum Use { USE_STATS = 0, USE_GRAD = 1, USE_SLAB = 2, USE_OUT = 3 };
 
@@ -38,37 +39,144 @@ struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;  // 16 x 16 blocks of a wavefront
-  static constexpr int JA = BM / 8 / WAVES, JB = BN / 8 / WAVES;  // 1 KB copies per wavefront and step
-  static constexpr int STAGE = (BM + BN) * 128;
+  static constexpr int STAGE = (BM + BN) * 128;               // bytes
   static_assert(BM % (WM * 16) == 0 && BN % (WN * 16) == 0, "wavefront tiles are whole blocks");
-  static_assert(JA * 8 * WAVES == BM && JB * 8 * WAVES == BN, "whole copies");
-  // copy i of an operand fills rows 8 i + lane / 8; with an even number of wavefronts the swizzle of a lane is the same
-  // for all of its copies
-  static_assert(WAVES % 2 == 0, "even number of wavefronts");
+  static_assert(WAVES % 2 == 0, "the swizzle of a lane's copies relies on an even number of wavefronts");
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// One operand's tile of R rows: its copies into LDS and its fragments.
+//
+// Contiguous along k (KC): an LDS row is 128 bytes of one operand row; 16-byte chunk c of row r lies in slot
+// c ^ ((r >> 1) & 7), so that the 16 lanes of a fragment read (16 rows, one chunk) touch all 64 banks once.
+//
+// Contiguous along the rows: an LDS row holds the R elements of one k.  bf16 fragments come from ds_read_b64_tr_b16, which
+// gives lane l four elements along k of column l % 16 out of the 4 x 16 elements that its group of 16 lanes points
+// at; fp32 fragments from single words.  32-byte pairs (bf16; 64-byte granules for fp32) of an LDS row are permuted by
+// k so that the eight k a half wavefront reads at once (four for fp32) lie in different banks.
+//
+// A copy cannot permute what a lane receives, so the lane that fills a slot fetches the chunk that belongs there.
+template <class T, int R, int WAVES, bool KC>
+struct Operand {
+  static constexpr int J = R / 8 / WAVES;          // copies of a wavefront per step
+  static constexpr int KS = 128 / (int)sizeof(T);  // k of a step
+  static constexpr int ROWB = R * (int)sizeof(T);  // bytes of an LDS row when contiguous along the rows
+  static_assert(J * 8 * WAVES == R, "whole copies");
+  static_assert(KC || R >= 64, "an LDS row holds the banks' permutation");
+
+  const char *base;
+  size_t step_bytes;
+  uint32_t offset[J];
+  uint32_t chunk;  // KC: byte of this lane's chunk within a step
+  int krow;        // else: k of this lane's first copy within a step
+
+  static __device__ __forceinline__ int swizzle(int k) {
+    if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+    return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : (((k >> 1) & 1) | ((k >> 3) & 1) << 1) << 1;
+  }
+
+  // rows [r0, ...) of an operand of `rows` rows, `ld` bytes apart along its slow direction; `row_bytes`: what may be read
+  // of that many bytes along the fast one when contiguous along the rows
+  __device__ __forceinline__ void init(const char *p, size_t ld, int r0, int rows, uint32_t row_bytes, int wave, int lane) {
+    if constexpr (KC) {
+      base = p + (size_t)r0 * ld;
+      step_bytes = 128;
+      const int row = wave * 8 + (lane >> 3);
+      chunk = ((uint32_t)(lane & 7) ^ ((uint32_t)(row >> 1) & 7u)) * 16u;
+      // rows past the end repeat the last one: their results are never used
+#pragma unroll
+      for (int j = 0; j < J; ++j) offset[j] = (uint32_t)min(row + j * WAVES * 8, rows - 1 - r0) * (uint32_t)ld + chunk;
+    } else {
+      base = p + (size_t)r0 * sizeof(T);
+      step_bytes = (size_t)KS * ld;
+      const int at = wave * 1024 + lane * 16;
+      krow = at / ROWB;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int k = krow + j * (WAVES * 1024 / ROWB);
+        const uint32_t c = (uint32_t)(((at % ROWB) >> 4) ^ swizzle(k)) * 16u;
+        offset[j] = (uint32_t)r0 * (uint32_t)sizeof(T) + c < row_bytes ? (uint32_t)k * (uint32_t)ld + c : kOutOfRange;
+      }
+    }
+  }
+
+  // step `step` into LDS at `dst`; what lies past the end of k becomes zero
+  __device__ __forceinline__ void stage(char *dst, int step, int K, uint32_t kbytes, int wave) const {
+    char *to = dst + wave * 1024;
+    if constexpr (KC) {
+      const uint32_t k = (uint32_t)step * 128u;
+      const rsrc_t r = make_rsrc(base);
+      const bool in = k + chunk < kbytes;
+#pragma unroll
+      for (int j = 0; j < J; ++j) lds_dma16(r, in ? offset[j] : kOutOfRange, k, (float *)(to + j * WAVES * 1024));
+    } else {
+      const rsrc_t r = make_rsrc(base + (size_t)step * step_bytes);
+      const int left = K - step * KS;
+      if (left >= KS) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) lds_dma16(r, offset[j], 0, (float *)(to + j * WAVES * 1024));
+      } else {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          lds_dma16(r, krow + j * (WAVES * 1024 / ROWB) < left ? offset[j] : kOutOfRange, 0,
+                    (float *)(to + j * WAVES * 1024));
+      }
+    }
+  }
+
+  // byte offsets of this lane's part of block b (16 rows), without the step's k
+  static __device__ __forceinline__ int frag_offset(int b, int lane) {
+    const int row = lane & 15, g = lane >> 4;
+    if (KC) return (b * 16 + row) * 128 + ((g ^ ((row >> 1) & 7)) * 16);
+    if (sizeof(T) == 4) return g * 4 * ROWB + ((b ^ g) << 6) + row * 4;
+    const int k = g * 8 + (row >> 2);
+    return k * ROWB + (((b << 1) ^ swizzle(k)) << 4) + (row & 3) * 8;
+  }
+  // the 16 bytes of half step `sub`; at = stage + frag_offset
+  static __device__ __forceinline__ f32x4 fragment(lds_char *tile, int at, int sub) {
+    typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    typedef __attribute__((address_space(3))) float lds_float;
+    if constexpr (KC) {
+      return *(lds_f32x4 *)(tile + (at ^ (sub * 64)));
+    } else if constexpr (sizeof(T) == 4) {
+      f32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = *(lds_float *)(tile + at + (sub * 16 + e) * ROWB);
+      return f;
+    } else {
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + at + sub * 32 * ROWB));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + at + (sub * 32 + 4) * ROWB));
+      return __builtin_bit_cast(f32x4, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
 };
 
 struct ProductArgs {
   const char *A, *B;
-  size_t lda, ldb;  // bytes between rows
-  int M, N;
-  uint32_t kbytes;  // bytes of a row of A and B that take part; multiple of 16
+  size_t lda, ldb;  // bytes between rows (between k for operands contiguous along the rows)
+  int M, N, K;
+  uint32_t kbytes;          // operands contiguous along k: bytes of a row that take part, a multiple of 16
+  uint32_t abytes, bbytes;  // operands contiguous along the rows: bytes of one k that may be read, multiples of 16
   int tiles_m, tiles_n, splits, steps_per_split;
   uint32_t blocks;
   // STATS, GRAD (m = rows v0 + m of the vocabulary, n = token)
   const void *bias;          // of the piece's first row, or null
   const int *labels;
-  int v0, vocab, ignore;
+  int v0, ignore;
   SoftStat *part;            // STATS: [tile of the whole vocabulary][token]
   int part_row;              // first tile of the piece
   float *label_score;        // STATS: [token]
-  float *scores;             // STATS: [token][ldg] raw scores, or null
-  const float *lse, *gscale; // GRAD; gscale: loss_grad or null
-  void *g, *gt;              // GRAD: [token][ldg], [vocabulary row][ldgt]
-  size_t ldg, ldgt;          // elements
-  int mpad, npad;            // GRAD: columns of g and of gt, whole 16-byte chunks (past M and N they are zero)
+  const float *lse, *weight, *wmax;  // GRAD; weight: loss_grad or null, wmax: its largest magnitude
+  void *g;                   // GRAD: [token][ldg]
+  size_t ldg;                // elements
+  int mpad;                  // GRAD: columns of g, whole 16-byte chunks (those past M are zero)
   float *db_part;            // GRAD: [tile_n][row of the piece] or null
   int db_ld;
-  // SLAB: C [split][N][M] fp32.  OUT: C [n][ldc] elements
+  // SLAB: C [split][N][ldc] fp32.  OUT: C [n][ldc] elements, times *wmax
   void *C;
   size_t ldc;
   int accumulate;
@@ -86,43 +194,52 @@ __device__ __forceinline__ void mfma_chunk<float>(f32x4 &c, const f32x4 &a, cons
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
 }
 
-// G of one score: the label's own entry is p - 1
-__device__ __forceinline__ float grad_entry(float score, float lse, bool is_label) {
-  const float p = exp2_fast((score - lse) * kLog2e);
-  return is_label ? p - 1.0f : p;
-}
-
-// A token's part in the gradient: its label's row (or -1), its lse and its weight; ignored tokens have weight 0 and
-// their G is 0 whatever their scores are.
+// A token's part in the gradient.  Ignored tokens have no part: their G is 0 whatever their scores are.
 struct TokenGrad {
   int label;
   float lse, weight;
   bool live;
 };
 __device__ __forceinline__ TokenGrad token_grad(int t, int tokens, const int *__restrict__ labels, int ignore,
-                                                const float *__restrict__ lse, const float *__restrict__ gscale) {
+                                                const float *__restrict__ lse, const float *__restrict__ weight,
+                                                const float *__restrict__ wmax) {
   TokenGrad g{-1, 0.0f, 0.0f, false};
   if (t < tokens) {
     g.label = labels[t];
     g.live = g.label != ignore;
     g.lse = lse[t];
-    g.weight = g.live ? (gscale ? gscale[t] : 1.0f) : 0.0f;
+    const float c = weight ? *wmax : 1.0f;
+    g.weight = !weight ? 1.0f : c > 0.0f ? weight[t] / c : 0.0f;
   }
   return g;
 }
-
-template <class T>
-__device__ __forceinline__ void store4(T *p, const float (&f)[4]) {
-  typedef T vec4 __attribute__((ext_vector_type(4)));
-  vec4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (T)f[i];
-  *reinterpret_cast<vec4 *>(p) = v;
+__device__ __forceinline__ float grad_entry(float score, const TokenGrad &tg, int v) {
+  if (!tg.live) return 0.0f;
+  const float p = exp2_fast((score - tg.lse) * kLog2e);
+  return tg.weight * (v == tg.label ? p - 1.0f : p);
 }
 
-template <class T, class S, int USE>
+// Four consecutive elements, of which those below `left` exist.
+template <class T>
+__device__ __forceinline__ void store4(T *p, const float (&f)[4], int left) {
+  typedef T vec4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (left >= 4) {
+    vec4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (T)f[i];
+    *reinterpret_cast<vec4 *>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = (T)f[i];
+  }
+}
+
+template <class T, class S, int USE, bool KA, bool KB>
 __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p) {
   extern __shared__ __align__(16) char lds[];
+  typedef Operand<T, S::BM, S::WAVES, KA> OpA;
+  typedef Operand<T, S::BN, S::WAVES, KB> OpB;
   constexpr int MI = S::MI, NI = S::NI;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / S::WN, wn = wave % S::WN;
@@ -135,64 +252,83 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int tm = (int)(band * 8u + in_band % band_m), tn = (int)(in_band / band_m);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
 
-  // global -> LDS copies: lane offsets within the tile's rows (rows past the end repeat the last one: their results
-  // are never used)
-  const rsrc_t ra = make_rsrc(p.A + (size_t)m0 * p.lda), rb = make_rsrc(p.B + (size_t)n0 * p.ldb);
-  const int crow = wave * 8 + (lane >> 3);
-  const uint32_t chunk = ((uint32_t)(lane & 7) ^ ((uint32_t)(crow >> 1) & 7u)) * 16u;
-  uint32_t va[S::JA], vb[S::JB];
-#pragma unroll
-  for (int j = 0; j < S::JA; ++j) va[j] = (uint32_t)min(crow + j * S::WAVES * 8, p.M - 1 - m0) * (uint32_t)p.lda + chunk;
-#pragma unroll
-  for (int j = 0; j < S::JB; ++j) vb[j] = (uint32_t)min(crow + j * S::WAVES * 8, p.N - 1 - n0) * (uint32_t)p.ldb + chunk;
-  auto stage = [&](int buf, int step) {
-    const uint32_t k = (uint32_t)step * 128u;
-    const bool in = k + chunk < p.kbytes;  // chunks past the end of k are filled with zeros
-    char *base = lds + buf * S::STAGE + wave * 1024;
-#pragma unroll
-    for (int j = 0; j < S::JA; ++j)
-      lds_dma16(ra, in ? va[j] : kOutOfRange, k, (float *)(base + j * S::WAVES * 1024));
-#pragma unroll
-    for (int j = 0; j < S::JB; ++j)
-      lds_dma16(rb, in ? vb[j] : kOutOfRange, k, (float *)(base + S::BM * 128 + j * S::WAVES * 1024));
-  };
+  OpA opa;
+  OpB opb;
+  opa.init(p.A, p.lda, m0, p.M, p.abytes, wave, lane);
+  opb.init(p.B, p.ldb, n0, p.N, p.bbytes, wave, lane);
 
   f32x4 acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int fa[MI], fb[NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) fa[i] = OpA::frag_offset(wm * MI + i, lane);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) fb[j] = OpB::frag_offset(wn * NI + j, lane);
 
-  const int frow = lane & 15, fgroup = lane >> 4, fswz = (frow >> 1) & 7;
-  const int fa = (wm * MI * 16 + frow) * 128, fb = S::BM * 128 + (wn * NI * 16 + frow) * 128;
-  const int steps = (int)((p.kbytes + 127u) / 128u);
+  const int steps = (p.K + OpA::KS - 1) / OpA::KS;
   const int s0 = (int)split * p.steps_per_split, s1 = min(steps, s0 + p.steps_per_split);
-  if (s0 < s1) stage(0, s0);
-  for (int s = s0; s < s1; ++s) {
+  auto stage = [&](int buf, int step) {
+    opa.stage(lds + buf * S::STAGE, step, p.K, p.kbytes, wave);
+    opb.stage(lds + buf * S::STAGE + S::BM * 128, step, p.K, p.kbytes, wave);
+  };
+  // A step is cut into phases of MH x NI blocks; while one phase's MFMAs run, the next one's fragments are read.  The last
+  // phase of a step reads the other stage, so the barrier stands before it: every wavefront then has all it needs of
+  // this stage in registers, and the copies of the step after next may overwrite it.
+  constexpr int MH = MI % 2 == 0 ? MI / 2 : MI, H = MI / MH, PHASES = 2 * H;
+  f32x4 a[2][MH], b[2][NI];
+  auto read_a = [&](int to, const int buf, int sub, int h) {
+    lds_char *t = (lds_char *)lds + buf * S::STAGE;
+#pragma unroll
+    for (int i = 0; i < MH; ++i) a[to][i] = OpA::fragment(t, fa[h * MH + i], sub);
+  };
+  auto read_b = [&](int to, const int buf, int sub) {
+    lds_char *t = (lds_char *)lds + buf * S::STAGE + S::BM * 128;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) b[to][j] = OpB::fragment(t, fb[j], sub);
+  };
+  if (s0 < s1) {
+    stage(0, s0);
     lds_dma_wait();
     __syncthreads();
+    if (s0 + 1 < s1) stage(1, s0 + 1);
+    read_a(0, 0, 0, 0);
+    read_b(0, 0, 0);
+  }
+  for (int s = s0; s < s1; ++s) {
     const int buf = (s - s0) & 1;
-    if (s + 1 < s1) stage(buf ^ 1, s + 1);
-    const char *base = lds + buf * S::STAGE;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const int slot = ((sub * 4 + fgroup) ^ fswz) * 16;
-      f32x4 a[MI], b[NI];
+    for (int q = 0; q < PHASES; ++q) {
+      const int sub = q / H, h = q % H;
+      if (q + 1 < PHASES) {
+        read_a((q + 1) & 1, buf, (q + 1) / H, (q + 1) % H);
+        if ((q + 1) % H == 0) read_b((q + 1) / H, buf, (q + 1) / H);
+      } else {
+        lds_dma_wait();
+        __syncthreads();
+        if (s + 2 < s1) stage(buf, s + 2);
+        if (s + 1 < s1) {
+          read_a(0, buf ^ 1, 0, 0);
+          read_b(0, buf ^ 1, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const f32x4 *>(base + fa + i * 2048 + slot);
+      for (int i = 0; i < MH; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const f32x4 *>(base + fb + j * 2048 + slot);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) mfma_chunk<T>(acc[i][j], a[i], b[j]);
+        for (int j = 0; j < NI; ++j) mfma_chunk<T>(acc[h * MH + i][j], a[q & 1][i], b[sub][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
   // this lane's elements: rows mrow + 16 i + r, columns ncol + 16 j
+  const int fgroup = lane >> 4, frow = lane & 15;
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
   if constexpr (USE == USE_STATS || USE == USE_GRAD) {
+    __syncthreads();  // the stages are done with
     if (p.bias) {
       const T *bias = (const T *)p.bias;
 #pragma unroll
@@ -207,7 +343,6 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   }
 
   if constexpr (USE == USE_STATS) {
-    __syncthreads();  // the stages are done with
     SoftStat *sh = (SoftStat *)lds;  // [WM][BN]
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -220,7 +355,6 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
         for (int r = 0; r < 4; ++r) {
           const int m = mrow + i * 16 + r;
           if (p.v0 + m == label && m < p.M) p.label_score[t] = acc[i][j][r];
-          if (p.scores && t < p.N && m < p.M) p.scores[(size_t)t * p.ldg + m] = acc[i][j][r];
           acc[i][j][r] = m < p.M ? acc[i][j][r] : neg_inf();
           st.m = fmaxf(st.m, acc[i][j][r]);
         }
@@ -244,7 +378,6 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   }
 
   if constexpr (USE == USE_GRAD) {
-    __syncthreads();
     float *sums = (float *)lds;  // [WN][BM] column sums for db
     float rows[MI][4];
 #pragma unroll
@@ -254,23 +387,17 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int t = ncol + j * 16;
-      const TokenGrad tg = token_grad(t, p.N, p.labels, p.ignore, p.lse, p.gscale);
+      const TokenGrad tg = token_grad(t, p.N, p.labels, p.ignore, p.lse, p.weight, p.wmax);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = mrow + i * 16;
         float g[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool live = tg.live && m + r < p.M;
-          g[r] = live ? grad_entry(acc[i][j][r], tg.lse, p.v0 + m + r == tg.label) : 0.0f;
+          g[r] = m + r < p.M ? grad_entry(acc[i][j][r], tg, p.v0 + m + r) : 0.0f;
+          rows[i][r] += g[r];
         }
-        if (t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float gw = g[r] * tg.weight;
-          rows[i][r] += gw;
-          if (m + r < p.M && t < p.npad) ((T *)p.gt)[(size_t)(m + r) * p.ldgt + t] = (T)gw;
-        }
+        if (t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g, 4);
       }
     }
     if (p.db_part) {
@@ -295,147 +422,213 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 
   if constexpr (USE == USE_SLAB || USE == USE_OUT) {
     typedef typename std::conditional<USE == USE_SLAB, float, T>::type Out;
+    const float scale = USE == USE_OUT && p.wmax ? *p.wmax : 1.0f;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int n = ncol + j * 16;
       if (n >= p.N) continue;
-      Out *row = (Out *)p.C + (USE == USE_SLAB ? ((size_t)split * p.N + n) * p.M : (size_t)n * p.ldc);
+      Out *row = (Out *)p.C + (USE == USE_SLAB ? ((size_t)split * p.N + n) * p.ldc : (size_t)n * p.ldc);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        const int m = mrow + i * 16;
+        const int m = mrow + i * 16, left = p.M - m;
+        if (left <= 0) continue;
+        float f[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (m + r < p.M) {
-            float v = acc[i][j][r];
-            if (USE == USE_SLAB && p.accumulate) v += (float)row[m + r];
-            row[m + r] = (Out)v;
-          }
+        for (int r = 0; r < 4; ++r) {
+          f[r] = USE == USE_OUT ? acc[i][j][r] * scale : acc[i][j][r];
+          if (USE == USE_SLAB && p.accumulate && r < left) f[r] += (float)row[m + r];
+        }
+        store4<Out>(row + m, f, left);
       }
     }
   }
 }
 
-// ---- copies ------------------------------------------------------------------------------------------------------
-// dst[c][r] = src[r][c] for c < cols, with columns [rows, rpad) of dst zero; tokens that the loss ignores count as rows of
-// zeros (labels given), so that whatever their x holds stays out of the products.
-template <class T>
-__global__ __launch_bounds__(256) void vocab_transpose_kernel(T *__restrict__ dst, const T *__restrict__ src, size_t ld_src,
-                                                              size_t ld_dst, int rows, int cols, int rpad,
-                                                              const int *__restrict__ labels, int ignore) {
-  __shared__ T tile[64][64 + 4 / sizeof(T)];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = r0 + y + i * 4, c = c0 + x;
-    const bool in = r < rows && c < cols && !(labels && labels[r] == ignore);
-    tile[y + i * 4][x] = in ? src[(size_t)r * ld_src + c] : (T)0.0f;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int c = c0 + y + i * 4, r = r0 + x;
-    if (c < cols && r < rpad) dst[(size_t)c * ld_dst + r] = tile[x][y + i * 4];
-  }
-}
-
+// ---- copies and statistics before the products ---------------------------------------------------------------------
 // dst[r][c] = src[r][c], rows of dst filled up to cpad with zeros: operands whose rows do not start at 16-byte
-// boundaries or are no whole number of 16-byte chunks
+// boundaries or are no whole number of 16-byte chunks.  With labels, the rows of ignored tokens become zero, so that
+// whatever their x holds stays out of dw; with weights, one workgroup more takes the largest magnitude of the live ones.
 template <class T>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, const T *__restrict__ src, size_t ld_src,
-                                                         int cols, int cpad) {
-  const size_t r = blockIdx.x;
+                                                         int rows, int cols, int cpad, const int *__restrict__ labels,
+                                                         int ignore, const float *__restrict__ weight,
+                                                         float *__restrict__ wmax) {
   constexpr int V = Num<T>::V;
+  if ((int)blockIdx.x == rows) {
+    __shared__ float sh[256];
+    float m = 0.0f;
+    for (int t = threadIdx.x; t < rows; t += 256)
+      if (labels[t] != ignore) m = fmaxf(m, fabsf(weight[t]));
+    sh[threadIdx.x] = m;
+    __syncthreads();
+    for (int d = 128; d > 0; d >>= 1) {
+      if ((int)threadIdx.x < d) sh[threadIdx.x] = fmaxf(sh[threadIdx.x], sh[threadIdx.x + d]);
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) *wmax = sh[0];
+    return;
+  }
+  const size_t r = blockIdx.x;
+  const bool live = !labels || labels[r] != ignore;
   for (int c = threadIdx.x * V; c < cpad; c += 256 * V) {
     float f[V];
-    load_vec<T>(f, src + r * ld_src, c, cols);
+    if (live) {
+      load_vec<T>(f, src + r * ld_src, c, cols);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = 0.0f;
+    }
     store_vec<T>(dst + r * cpad, f, c, cpad);
   }
 }
 
 // ---- joining -----------------------------------------------------------------------------------------------------
-// The tiles' statistics of each token, in order: 16 tokens per workgroup, 16 lanes each taking every 16th tile.
+__device__ __forceinline__ void store_loss(float *__restrict__ loss, float *__restrict__ lse, int t, float l, int label,
+                                           float score, int vocab, int ignore) {
+  lse[t] = l;
+  loss[t] = label == ignore ? 0.0f : (unsigned)label < (unsigned)vocab ? l - score : __builtin_nanf("");
+}
+
+// The tiles' statistics of each token: 16 tokens per workgroup, 16 lanes each taking every 16th tile (many tokens), or one
+// token per workgroup (few tokens, so that the launch is not one workgroup's walk over the tiles).
+template <int TOK>
 __global__ __launch_bounds__(256) void vocab_loss_kernel(float *__restrict__ loss, float *__restrict__ lse,
                                                          const SoftStat *__restrict__ part,
                                                          const float *__restrict__ label_score,
                                                          const int *__restrict__ labels, int tokens, int tiles, int vocab,
                                                          int ignore) {
-  __shared__ SoftStat sh[16][17];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, t = blockIdx.x * 16 + x;
+  constexpr int LANES = 256 / TOK;
+  __shared__ SoftStat sh[LANES][TOK + 1];
+  const int x = threadIdx.x % TOK, y = threadIdx.x / TOK, t = blockIdx.x * TOK + x;
   SoftStat st{neg_inf(), 0.0f};
-  if (t < tokens)
-    for (int i = y; i < tiles; i += 16) st = join(st, part[(size_t)i * tokens + t], kLog2e);
+  if (t < tokens) {
+    int i = y;
+    for (; i + 7 * LANES < tiles; i += 8 * LANES) {  // eight loads in flight
+      SoftStat v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(size_t)(i + k * LANES) * tokens + t];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) st = join(st, v[k], kLog2e);
+    }
+    for (; i < tiles; i += LANES) st = join(st, part[(size_t)i * tokens + t], kLog2e);
+  }
   sh[y][x] = st;
   __syncthreads();
-  if (y == 0 && t < tokens) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) st = join(st, sh[i][x], kLog2e);
-    const float l = log_sum(st, 1.0f);
-    const int label = labels[t];
-    lse[t] = l;
-    loss[t] = label == ignore ? 0.0f
-              : (unsigned)label < (unsigned)vocab ? l - label_score[t]
-                                                  : __builtin_nanf("");
+  for (int d = LANES / 2; d > 0; d >>= 1) {
+    if (y < d) sh[y][x] = join(sh[y][x], sh[y + d][x], kLog2e);
+    __syncthreads();
   }
+  if (y == 0 && t < tokens)
+    store_loss(loss, lse, t, log_sum(sh[0][x], 1.0f), labels[t], label_score[t], vocab, ignore);
 }
 
-// G and its transpose from kept scores, 64 x 64 entries a workgroup, and the column sums of the tile.
+// Kept scores of one token: the parts that the product was cut into are added up (in order) and the bias on top, then
+// lse and loss (forward), then G (backward) in T; fp32 G takes the place of the scores, and so does bf16's unrounded G where
+// db needs its column sums.  A workgroup per token; the second walk over the row finds it in a cache.
 template <class T>
-__global__ __launch_bounds__(256) void vocab_grad_kernel(T *__restrict__ g, T *__restrict__ gt,
-                                                         const float *__restrict__ scores, float *__restrict__ db_part,
-                                                         const int *__restrict__ labels, const float *__restrict__ lse,
-                                                         const float *__restrict__ gscale, int tokens, int vocab, int v0,
-                                                         int rows, int ignore, size_t ld_scores, size_t ldg, size_t ldgt,
-                                                         int mpad, int npad, int db_ld) {
-  __shared__ float tile[64][65];
-  __shared__ float sums[4][64];
-  const int m0 = blockIdx.x * 64, t0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const int m = m0 + x;
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int t = t0 + y + i * 4;
-    const TokenGrad tg = token_grad(t, tokens, labels, ignore, lse, gscale);
-    float v = 0.0f;
-    if (tg.live && m < rows) v = grad_entry(scores[(size_t)t * ld_scores + m], tg.lse, v0 + m == tg.label);
-    if (t < tokens && m < mpad) g[(size_t)t * ldg + m] = (T)v;
-    v *= tg.weight;
-    sum += v;
-    tile[y + i * 4][x] = v;
+__global__ __launch_bounds__(512) void vocab_row_kernel(float *__restrict__ loss, float *__restrict__ lse_out,
+                                                        const float *__restrict__ lse_in, T *__restrict__ g,
+                                                        float *__restrict__ scores, const T *__restrict__ bias,
+                                                        const int *__restrict__ labels, const float *__restrict__ weight,
+                                                        const float *__restrict__ wmax, int tokens, int vocab, int splits,
+                                                        size_t ld, int ignore, int mpad, int keep_g) {
+  __shared__ SoftStat sh[8];
+  __shared__ float lse_sh;
+  const int t = blockIdx.x, tid = threadIdx.x;
+  float *row = scores + (size_t)t * ld;
+  const size_t part = (size_t)tokens * ld;
+  const bool sum = splits > 1 || bias;
+  const int label = labels[t];
+  SoftStat st{neg_inf(), 0.0f};
+  // ld is a multiple of four and rows start at 16-byte boundaries
+  for (int c = tid * 4; c < vocab; c += 512 * 4) {
+    f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
+    if (sum) {
+      for (int i = 1; i < splits; ++i) v += *reinterpret_cast<const f32x4 *>(row + i * part + c);
+      if (bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < vocab) v[i] += (float)bias[c + i];
+      *reinterpret_cast<f32x4 *>(row + c) = v;
+    }
+    if (loss) {
+      float m = st.m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = c + i < vocab ? v[i] : neg_inf();
+        m = fmaxf(m, v[i]);
+      }
+      const float base = m == neg_inf() ? 0.0f : m;
+      float s = st.s * (st.m == m ? 1.0f : exp2_fast((st.m - base) * kLog2e));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += exp2_fast((v[i] - base) * kLog2e);
+      st = SoftStat{m, s};
+    }
   }
-  sums[y][x] = sum;
+  if (loss) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) st = shfl_xor_join(st, m, kLog2e);
+    if ((tid & 63) == 0) sh[tid >> 6] = st;
+    __syncthreads();  // (also: this row's sums are written)
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) st = join(st, sh[i], kLog2e);
+      const float l = log_sum(st, 1.0f);
+      lse_sh = l;
+      store_loss(loss, lse_out, t, l, label, (unsigned)label < (unsigned)vocab ? row[label] : 0.0f, vocab, ignore);
+    }
+  } else if (tid == 0) {
+    lse_sh = lse_in[t];
+  }
+  if (!g) return;
   __syncthreads();
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int mm = m0 + y + i * 4, t = t0 + x;
-    if (mm < rows && t < npad) gt[(size_t)mm * ldgt + t] = (T)tile[x][y + i * 4];
+  TokenGrad tg = token_grad(0, 1, labels + t, ignore, &lse_sh, weight ? weight + t : nullptr, wmax);
+  for (int c = tid * 4; c < mpad; c += 512 * 4) {
+    float f[4];
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = c + i < vocab ? grad_entry(v[i], tg, c + i) : 0.0f;
+    if (keep_g || std::is_same<T, float>::value) *reinterpret_cast<f32x4 *>(row + c) = f32x4{f[0], f[1], f[2], f[3]};
+    if (!std::is_same<T, float>::value) store4<T>(g + (size_t)t * ld + c, f, 4);
   }
-  if (db_part && y == 0 && m < rows)
-    db_part[(size_t)blockIdx.y * db_ld + m] = ((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x];
 }
 
-// dx[t] = weight * sum of the slabs, in order
+// Column sums of 64 tokens' G.
+__global__ __launch_bounds__(256) void vocab_colsum_kernel(float *__restrict__ part, const float *__restrict__ g, size_t ldg,
+                                                           int tokens, int rows, int ld) {
+  const int m = blockIdx.x * 256 + threadIdx.x, t0 = blockIdx.y * 64, t1 = min(tokens, t0 + 64);
+  if (m >= rows) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int t = t0; t < t1; ++t) s += g[(size_t)t * ldg + m];
+  part[(size_t)blockIdx.y * ld + m] = s;
+}
+
+// dx[t] = *wmax times the sum of the slabs, in order; nothing for ignored tokens
 template <class T>
 __global__ __launch_bounds__(256) void vocab_dx_kernel(T *__restrict__ dx, const float *__restrict__ slabs,
-                                                       const int *__restrict__ labels, const float *__restrict__ gscale,
-                                                       int ignore, int tokens, int width, size_t ldx, int splits) {
+                                                       const float *__restrict__ wmax, int tokens, int width, size_t ldx,
+                                                       size_t ld, int splits) {
   const int t = blockIdx.x;
-  const bool live = labels[t] != ignore;
-  const float weight = gscale ? gscale[t] : 1.0f;
-  for (int c = threadIdx.x; c < width; c += 256) {
-    float s = 0.0f;
-    for (int i = 0; i < splits; ++i) s += slabs[((size_t)i * tokens + t) * width + c];
-    dx[(size_t)t * ldx + c] = (T)(live ? s * weight : 0.0f);
-  }
+  const float weight = wmax ? *wmax : 1.0f;
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= width) return;
+  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4 *>(slabs + ((size_t)i * tokens + t) * ld + c);
+  const float f[4] = {s[0] * weight, s[1] * weight, s[2] * weight, s[3] * weight};
+  store4<T>(dx + (size_t)t * ldx + c, f, width - c);
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void vocab_db_kernel(T *__restrict__ db, const float *__restrict__ part, int rows, int ld,
-                                                       int tiles) {
+__global__ __launch_bounds__(256) void vocab_db_kernel(T *__restrict__ db, const float *__restrict__ part,
+                                                       const float *__restrict__ wmax, int rows, int ld, int tiles) {
   const int m = blockIdx.x * 256 + threadIdx.x;
   if (m >= rows) return;
   float s = 0.0f;
+#pragma unroll 4
   for (int i = 0; i < tiles; ++i) s += part[(size_t)i * ld + m];
-  db[m] = (T)s;
+  db[m] = (T)(wmax ? s * *wmax : s);
 }
 
 template <class T>
@@ -446,25 +639,58 @@ __global__ __launch_bounds__(256) void vocab_zero_kernel(T *__restrict__ p, size
 // ---- host --------------------------------------------------------------------------------------------------------
 typedef Shape<256, 256, 2, 4> ShapeL;
 typedef Shape<128, 128, 2, 2> ShapeM;
+typedef Shape<64, 64, 2, 2> ShapeN;
 typedef Shape<64, 32, 4, 1> ShapeS;
 
 static int idiv(int a, int b) { return (a + b - 1) / b; }
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Which tile: the largest that still gives most of the 256 CUs a workgroup (`splits_ok`: the launch may also be cut
-// along k); few columns take the narrow tile.
-enum ShapeId { SHAPE_L, SHAPE_M, SHAPE_S };
-static ShapeId choose_shape(int M, int N) {
-  if (N <= 32) return SHAPE_S;
-  if ((long)idiv(M, 256) * idiv(N, 256) >= 192) return SHAPE_L;
-  return SHAPE_M;
+// Which tile a product takes and into how many parts it is cut along k: the cheapest by a small model of the chip.  A
+// workgroup's step costs `alone` microseconds when it has a CU to itself and `full` when `occ` of them share it.
+struct TileCost {
+  int bm, bn, occ;
+  double alone[2], full[2];  // fp32, bf16
+};
+enum ShapeId { SHAPE_L, SHAPE_M, SHAPE_N, SHAPE_S, SHAPES };
+static const TileCost kTiles[SHAPES] = {
+    {ShapeL::BM, ShapeL::BN, 1, {8.5, 1.75}, {8.5, 1.75}},
+    {ShapeM::BM, ShapeM::BN, 2, {2.2, 0.80}, {4.1, 1.30}},
+    {ShapeN::BM, ShapeN::BN, 4, {0.7, 0.50}, {2.2, 0.90}},
+    {ShapeS::BM, ShapeS::BN, 6, {0.4, 0.40}, {1.8, 0.90}},
+};
+constexpr double kLaunchUs = 3.0, kBytesPerUs = 4.0e6;  // what a launch costs, and a pass over memory
+
+struct Choice {
+  ShapeId shape;
+  int splits;
+  double us;
+};
+static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow) {
+  const int ks = dtype == CCT_BF16 ? 64 : 32, d = dtype == CCT_BF16 ? 1 : 0;
+  const int steps = idiv(K, ks);
+  const int pinned = tuning().vocab_tile >= 1 && tuning().vocab_tile <= SHAPES ? tuning().vocab_tile : 0;
+  Choice best{SHAPE_M, 1, 1e30};
+  for (int s = 0; s < SHAPES; ++s) {
+    if (s == SHAPE_S && !narrow) continue;
+    if (pinned && s != (pinned == SHAPES && !narrow ? SHAPE_N : pinned - 1)) continue;
+    const TileCost &c = kTiles[s];
+    const double tiles = (double)idiv(M, c.bm) * idiv(N > 0 ? N : 1, c.bn);
+    for (int splits = 1; splits <= 64; splits *= 2) {
+      if (splits > 1 && (!may_split || steps < 4 * splits)) break;
+      const double w = tiles * splits, round = 256.0 * c.occ;
+      const double rounds = (double)(long)(w / round), per_cu = (double)(long)((w - rounds * round + 255.0) / 256.0);
+      const double last = per_cu * c.full[d] / c.occ;
+      const double step = rounds * c.full[d] + (per_cu > 0 ? (last > c.alone[d] ? last : c.alone[d]) : 0.0);
+      const double us = step * idiv(steps, splits) + kLaunchUs +
+                        (may_split ? 2.0 * splits * M * (double)N * 4.0 / kBytesPerUs : 0.0);
+      if (us < best.us) best = Choice{(ShapeId)s, splits, us};
+    }
+  }
+  return best;
 }
-static int shape_bm(ShapeId s) { return s == SHAPE_L ? ShapeL::BM : s == SHAPE_M ? ShapeM::BM : ShapeS::BM; }
-static int shape_bn(ShapeId s) { return s == SHAPE_L ? ShapeL::BN : s == SHAPE_M ? ShapeM::BN : ShapeS::BN; }
 
-constexpr size_t kKeepBytes = (size_t)512 << 20;   // fp32 scores kept between forward and backward of one call
-constexpr size_t kPieceBytes = (size_t)384 << 20;  // automatic piece: G, its transpose and w's transpose
-
+constexpr size_t kKeepBytes = (size_t)512 << 20;   // fp32 scores that may be kept
+constexpr size_t kPieceBytes = (size_t)384 << 20;  // automatic piece: G and w's packed copy
 // a tile's rows are addressed with 32-bit byte offsets: 256 rows of a piece's columns in fp32 are 2^30 bytes
 constexpr int kPieceMax = 1 << 20;
 
@@ -473,13 +699,12 @@ struct VocabPlan {
   size_t el, ldx, ldw;
   int unit;            // elements of a 128-byte step
   int piece, pieces;   // rows of w at a time
-  bool keep;           // forward_backward keeps the scores (one piece)
-  int np, hp, vp;      // row lengths of transposed and packed operands: tokens, width, piece rounded up to whole steps
-  int nk;              // tokens rounded up to whole 16-byte chunks: what the transposed operands hold of k
-  ShapeId fs, dxs, dws;
+  int hp, vp;          // row lengths of packed and of G: width, piece rounded up to whole steps
+  Choice stats, kept, dx, dw;
+  // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
+  bool keep_forward, keep_backward, keep_both;
   int stats_tiles;
-  int dx_splits;
-  size_t part, label_score, xpack, wpack, g, gt, wt, xt, slabs, db, scores, total_forward, total;
+  size_t part, label_score, xpack, wpack, scores, xlive, wmax, g, slabs, db, total_forward, total;
 };
 
 static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
@@ -492,87 +717,94 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.ldx = a->x_stride ? a->x_stride : (size_t)a->width;
   p.ldw = a->w_stride ? a->w_stride : (size_t)a->width;
   p.unit = 128 / (int)p.el;
-  p.np = idiv(p.tokens, p.unit) * p.unit;
   p.hp = idiv(p.width, p.unit) * p.unit;
-  p.nk = idiv(p.tokens, p.unit / 8) * (p.unit / 8);
+  const size_t n = p.tokens;
   const int vmax = idiv(p.vocab, 256) * 256;
   if (a->piece > 0) {
     p.piece = (int)min((((size_t)a->piece + 255) / 256) * 256, (size_t)kPieceMax);
   } else {
     // a power of two, so that the tiles of a piece fill whole rounds of the chip
-    const size_t row = (2 * (size_t)p.np + p.hp) * p.el;
-    size_t want = kPieceBytes / (row ? row : 1), rows = 1024;
+    const size_t row = (n + p.hp) * p.el, want = kPieceBytes / row;
+    size_t rows = 1024;
     while (rows * 2 <= want && rows < (size_t)vmax) rows *= 2;
-    p.piece = rows > (size_t)vmax ? vmax : (int)rows;
+    p.piece = (int)min(rows, (size_t)kPieceMax);
   }
   if (p.piece > vmax) p.piece = vmax;
-  if (p.piece > kPieceMax) p.piece = kPieceMax;
-  p.keep = a->piece <= 0 && vmax <= kPieceMax && (size_t)p.tokens * p.vocab * 4 <= kKeepBytes;
-  if (p.keep) p.piece = vmax;
+  // kept scores: all of the vocabulary at once
+  const bool may_keep = vmax <= kPieceMax && (a->piece <= 0 || p.piece == vmax);
+  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
+  p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, true, true);
+  const double score_bytes = (double)n * vmax * 4;
+  const double stats_us = p.stats.us * idiv(p.vocab, p.piece) + kLaunchUs;
+  const double join_us = kLaunchUs + score_bytes / kBytesPerUs, grad_us = score_bytes * 2 / kBytesPerUs;
+  const bool fits = may_keep && score_bytes * p.kept.splits <= (double)kKeepBytes;
+  p.keep_forward = fits && p.kept.us + join_us < stats_us;
+  p.keep_backward = fits && p.kept.us + join_us + grad_us < stats_us;
+  p.keep_both = fits && p.kept.us + join_us + grad_us < 2 * stats_us;
+  if (tuning().vocab_keep) p.keep_forward = p.keep_backward = p.keep_both = fits && tuning().vocab_keep == 1;
+  if (p.keep_forward || p.keep_backward || p.keep_both) p.piece = vmax;
   p.pieces = idiv(p.vocab, p.piece);
   p.vp = p.piece;
-  p.fs = choose_shape(p.piece, p.tokens);
+  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
   p.stats_tiles = 0;
-  for (int v = 0; v < p.vocab; v += p.piece)
-    p.stats_tiles += idiv(p.vocab - v < p.piece ? p.vocab - v : p.piece, shape_bm(p.fs));
-  p.dxs = choose_shape(p.width, p.tokens);
-  p.dws = choose_shape(p.width, p.piece);
-  const long dx_tiles = (long)idiv(p.width, shape_bm(p.dxs)) * idiv(p.tokens > 0 ? p.tokens : 1, shape_bn(p.dxs));
-  const int steps = p.vp / p.unit;
-  // short of workgroups: cut along the vocabulary, no part shorter than eight steps
-  long splits = 512 / dx_tiles;
-  if (splits > steps / 8) splits = steps / 8;
-  if (splits > 64) splits = 64;
-  p.dx_splits = splits < 1 ? 1 : (int)splits;
+  for (int v = 0; v < p.vocab; v += p.piece) p.stats_tiles += idiv(min(p.piece, p.vocab - v), kTiles[p.stats.shape].bm);
+  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, true, true);
+  p.dw = choose(p.width, p.piece, p.tokens, p.dtype, false, false);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += align256(bytes);
     return here;
   };
-  const size_t n = p.tokens;
+  const bool keep_any = p.keep_backward || p.keep_both;
   p.part = take((size_t)p.stats_tiles * n * sizeof(SoftStat));
   p.label_score = take(n * 4);
   p.xpack = take(n * p.hp * p.el);
   p.wpack = take((size_t)p.piece * p.hp * p.el);
+  const size_t score_space = (size_t)p.kept.splits * n * vmax * 4;
+  p.scores = take(p.keep_forward ? score_space : 0);
   p.total_forward = at;
+  if (!p.keep_forward) p.scores = take(keep_any ? score_space : 0);
+  p.xlive = take(n * p.hp * p.el);
+  p.wmax = take(4);
   p.g = take(n * p.vp * p.el);
-  p.gt = take((size_t)p.vp * p.np * p.el);
-  p.wt = take((size_t)p.width * p.vp * p.el);
-  p.xt = take((size_t)p.width * p.np * p.el);
-  p.slabs = take((size_t)p.dx_splits * n * p.width * 4);
+  p.slabs = take((size_t)p.dx.splits * n * p.hp * 4);
   p.db = take((size_t)idiv(p.tokens, 32) * p.vp * 4);
-  p.scores = take(p.keep ? n * p.vp * 4 : 0);
   p.total = at;
   return p;
 }
 
-template <class T, class S, int USE>
+template <class T, class S, int USE, bool KA, bool KB>
 static int launch_product(ProductArgs &p) {
-  auto kern = vocab_product_kernel<T, S, USE>;
+  auto kern = vocab_product_kernel<T, S, USE, KA, KB>;
   static LdsGrant grant;
   const size_t bytes = 2 * S::STAGE;
   if (int rc = grant_dynamic_lds((const void *)kern, bytes, grant)) return rc;
   p.tiles_m = idiv(p.M, S::BM);
   p.tiles_n = idiv(p.N, S::BN);
-  const int steps = (int)((p.kbytes + 127u) / 128u);
+  const int steps = idiv(p.K, 128 / (int)sizeof(T));
   p.steps_per_split = idiv(steps, p.splits);
   const unsigned long blocks = (unsigned long)p.tiles_m * p.tiles_n * p.splits;
   CCT_REQUIRE(blocks * S::THREADS < (1ul << 32), "vocab_loss: %lu workgroups are too many for one launch", blocks);
   p.blocks = (uint32_t)blocks;
   kern<<<p.blocks, S::THREADS, bytes, ctx().stream>>>(p);
   CCT_LAUNCH_CHECK();
-  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d>, %d> splits=%d", Num<T>::NAME, S::BM, S::BN, S::WM, S::WN, USE,
-              p.splits);
+  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d>, %d, %s, %s> splits=%d", Num<T>::NAME, S::BM, S::BN, S::WM,
+              S::WN, USE, KA ? "true" : "false", KB ? "true" : "false", p.splits);
   return 0;
 }
 
-template <class T, int USE>
-static int product(ShapeId s, ProductArgs &p) {
-  switch (s) {
-    case SHAPE_L: return launch_product<T, ShapeL, USE>(p);
-    case SHAPE_M: return launch_product<T, ShapeM, USE>(p);
-    default: return launch_product<T, ShapeS, USE>(p);
+template <class T, int USE, bool KA, bool KB>
+static int product(const Choice &c, ProductArgs &p) {
+  p.splits = c.splits;
+  switch (c.shape) {
+    case SHAPE_L: return launch_product<T, ShapeL, USE, KA, KB>(p);
+    case SHAPE_M: return launch_product<T, ShapeM, USE, KA, KB>(p);
+    case SHAPE_N: return launch_product<T, ShapeN, USE, KA, KB>(p);
+    default:
+      // an operand that is contiguous along its rows needs 64 of them
+      if constexpr (KB) return launch_product<T, ShapeS, USE, KA, KB>(p);
+      return launch_product<T, ShapeN, USE, KA, KB>(p);
   }
 }
 
@@ -583,7 +815,7 @@ struct VocabCall {
   void *dx, *dw, *db;
   const void *x, *w, *bias;
   const int *labels;
-  const float *gscale;
+  const float *weight;
   int ignore;
   char *ws;
   bool forward, backward;
@@ -598,135 +830,151 @@ template <class T>
 static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   hipStream_t st = ctx().stream;
   const int n = p.tokens;
-  const bool keep = p.keep && c.forward && c.backward;
+  const bool keep = c.forward && c.backward ? p.keep_both : c.forward ? p.keep_forward : p.keep_backward;
   SoftStat *part = (SoftStat *)(c.ws + p.part);
-  float *label_score = (float *)(c.ws + p.label_score);
-  T *g = (T *)(c.ws + p.g), *gt = (T *)(c.ws + p.gt), *wt = (T *)(c.ws + p.wt), *xt = (T *)(c.ws + p.xt);
+  float *label_score = (float *)(c.ws + p.label_score), *scores = (float *)(c.ws + p.scores);
   float *slabs = (float *)(c.ws + p.slabs), *db_part = (float *)(c.ws + p.db);
+  T *g = (T *)(c.ws + p.g), *xlive = (T *)(c.ws + p.xlive);
+  if (keep && p.el == 4) g = (T *)scores;  // fp32 G takes the scores' place
+  const size_t packed = p.hp * p.el;
+  const bool direct_x = direct_rows(c.x, p.ldx, p.width, p.el), direct_w = direct_rows(c.w, p.ldw, p.width, p.el);
   const char *x = (const char *)c.x;
   size_t ldx = p.ldx * p.el;
-  uint32_t kbytes = (uint32_t)(p.width * p.el);
-  if (!direct_rows(c.x, p.ldx, p.width, p.el) || !direct_rows(c.w, p.ldw, p.width, p.el)) {
-    // both operands are packed when one has to be: they walk k alike
+  if (!direct_x) {
     T *xp = (T *)(c.ws + p.xpack);
-    vocab_pack_kernel<T><<<n, 256, 0, st>>>(xp, (const T *)c.x, p.ldx, p.width, p.hp);
+    vocab_pack_kernel<T><<<n, 256, 0, st>>>(xp, (const T *)c.x, p.ldx, n, p.width, p.hp, nullptr, 0, nullptr, nullptr);
     CCT_LAUNCH_CHECK();
     x = (const char *)xp;
-    ldx = p.hp * p.el;
-    kbytes = (uint32_t)(p.hp * p.el);
+    ldx = packed;
   }
-  const bool pack = x != (const char *)c.x;
-  auto scores_of = [&](int v0, int rows, ProductArgs &a) -> int {
-    a = ProductArgs{};
-    a.A = (const char *)c.w + (size_t)v0 * p.ldw * p.el;
-    a.lda = p.ldw * p.el;
-    if (pack) {
-      T *wp = (T *)(c.ws + p.wpack);
-      vocab_pack_kernel<T><<<rows, 256, 0, st>>>(wp, (const T *)a.A, p.ldw, p.width, p.hp);
-      CCT_LAUNCH_CHECK();
-      a.A = (const char *)wp;
-      a.lda = p.hp * p.el;
-    }
+  const float *wmax = nullptr;
+  if (c.backward) {
+    if (c.weight) wmax = (const float *)(c.ws + p.wmax);
+    vocab_pack_kernel<T><<<n + (c.weight ? 1 : 0), 256, 0, st>>>(xlive, (const T *)c.x, p.ldx, n, p.width, p.hp, c.labels,
+                                                                c.ignore, c.weight, (float *)(c.ws + p.wmax));
+    CCT_LAUNCH_CHECK();
+  }
+  // the piece's rows of w as an operand
+  const size_t ldw = direct_w ? p.ldw * p.el : packed;
+  auto rows_of_w = [&](int v0, int rows, const char **out) -> int {
+    *out = (const char *)c.w + (size_t)v0 * p.ldw * p.el;
+    if (direct_w) return 0;
+    T *wp = (T *)(c.ws + p.wpack);
+    vocab_pack_kernel<T><<<rows, 256, 0, st>>>(wp, (const T *)*out, p.ldw, rows, p.width, p.hp, nullptr, 0, nullptr, nullptr);
+    CCT_LAUNCH_CHECK();
+    *out = (const char *)wp;
+    return 0;
+  };
+  auto score_args = [&](const char *w, int v0, int rows) {
+    ProductArgs a{};
+    a.A = w;
+    a.lda = ldw;
     a.B = x;
     a.ldb = ldx;
     a.M = rows;
     a.N = n;
-    a.kbytes = kbytes;
-    a.splits = 1;
+    a.K = p.width;
+    a.kbytes = (uint32_t)((p.width * p.el + 15) & ~(size_t)15);
     a.bias = c.bias ? (const char *)c.bias + (size_t)v0 * p.el : nullptr;
     a.labels = c.labels;
     a.v0 = v0;
-    a.vocab = p.vocab;
     a.ignore = c.ignore;
-    a.ldg = p.vp;
-    return 0;
+    return a;
   };
-  if (c.forward) {
+  const char *w = nullptr;
+  const int chunk = p.unit / 8;
+  if (keep) {
+    if (int rc = rows_of_w(0, p.vocab, &w)) return rc;
+    ProductArgs a = score_args(w, 0, p.vocab);
+    a.C = scores;
+    a.ldc = p.vp;
+    if (int rc = product<T, USE_SLAB, true, true>(p.kept, a)) return rc;
+    vocab_row_kernel<T><<<n, 512, 0, st>>>(c.forward ? c.loss : nullptr, c.lse, c.lse_in, c.backward ? g : nullptr, scores,
+                                          (const T *)c.bias, c.labels, c.weight, wmax, n, p.vocab, p.kept.splits, p.vp,
+                                          c.ignore, idiv(p.vocab, chunk) * chunk, c.db ? 1 : 0);
+    CCT_LAUNCH_CHECK();
+    if (c.db) {
+      vocab_colsum_kernel<<<dim3(idiv(p.vocab, 256), idiv(n, 64)), 256, 0, st>>>(db_part, scores, p.vp, n, p.vocab, p.vp);
+      CCT_LAUNCH_CHECK();
+      vocab_db_kernel<T><<<idiv(p.vocab, 256), 256, 0, st>>>((T *)c.db, db_part, wmax, p.vocab, p.vp, idiv(n, 64));
+      CCT_LAUNCH_CHECK();
+    }
+  } else if (c.forward) {
     int tiles = 0;
     for (int v0 = 0; v0 < p.vocab; v0 += p.piece) {
       const int rows = min(p.piece, p.vocab - v0);
-      ProductArgs a;
-      if (int rc = scores_of(v0, rows, a)) return rc;
+      if (int rc = rows_of_w(v0, rows, &w)) return rc;
+      ProductArgs a = score_args(w, v0, rows);
       a.part = part;
       a.part_row = tiles;
       a.label_score = label_score;
-      a.scores = keep ? (float *)(c.ws + p.scores) : nullptr;
-      if (int rc = product<T, USE_STATS>(p.fs, a)) return rc;
+      if (int rc = product<T, USE_STATS, true, true>(p.stats, a)) return rc;
       tiles += a.tiles_m;
     }
-    vocab_loss_kernel<<<idiv(n, 16), 256, 0, st>>>(c.loss, c.lse, part, label_score, c.labels, n, tiles, p.vocab, c.ignore);
+    if (n >= 2048)
+      vocab_loss_kernel<16><<<idiv(n, 16), 256, 0, st>>>(c.loss, c.lse, part, label_score, c.labels, n, tiles, p.vocab,
+                                                        c.ignore);
+    else
+      vocab_loss_kernel<1><<<n, 256, 0, st>>>(c.loss, c.lse, part, label_score, c.labels, n, tiles, p.vocab, c.ignore);
     CCT_LAUNCH_CHECK();
   }
   if (!c.backward) return 0;
   const float *lse = c.forward ? c.lse : c.lse_in;
-  if (c.dw) {
-    vocab_transpose_kernel<T><<<dim3(idiv(p.np, 64), idiv(p.width, 64)), 256, 0, st>>>(
-        xt, (const T *)c.x, p.ldx, p.np, n, p.width, p.nk, c.labels, c.ignore);
-    CCT_LAUNCH_CHECK();
-  }
   for (int v0 = 0; v0 < p.vocab; v0 += p.piece) {
-    const int rows = min(p.piece, p.vocab - v0);
-    const int mpad = idiv(rows, p.unit / 8) * (p.unit / 8);
-    int db_tiles;
-    if (keep) {
-      vocab_grad_kernel<T><<<dim3(idiv(mpad, 64), idiv(p.np, 64)), 256, 0, st>>>(
-          g, gt, (const float *)(c.ws + p.scores), c.db ? db_part : nullptr, c.labels, lse, c.gscale, n, p.vocab, v0, rows,
-          c.ignore, p.vp, p.vp, p.np, mpad, p.nk, p.vp);
-      CCT_LAUNCH_CHECK();
-      db_tiles = idiv(p.np, 64);
-    } else {
-      ProductArgs a;
-      if (int rc = scores_of(v0, rows, a)) return rc;
+    const int rows = min(p.piece, p.vocab - v0), mpad = idiv(rows, chunk) * chunk;
+    if (!keep) {
+      if (int rc = rows_of_w(v0, rows, &w)) return rc;
+      ProductArgs a = score_args(w, v0, rows);
       a.lse = lse;
-      a.gscale = c.gscale;
+      a.weight = c.weight;
+      a.wmax = wmax;
       a.g = g;
-      a.gt = gt;
-      a.ldgt = p.np;
+      a.ldg = p.vp;
       a.mpad = mpad;
-      a.npad = p.nk;
       a.db_part = c.db ? db_part : nullptr;
       a.db_ld = p.vp;
-      if (int rc = product<T, USE_GRAD>(p.fs, a)) return rc;
-      db_tiles = a.tiles_n;
-    }
-    if (c.db) {
-      vocab_db_kernel<T><<<idiv(rows, 256), 256, 0, st>>>((T *)c.db + v0, db_part, rows, p.vp, db_tiles);
-      CCT_LAUNCH_CHECK();
+      if (int rc = product<T, USE_GRAD, true, true>(p.stats, a)) return rc;
+      if (c.db) {
+        vocab_db_kernel<T><<<idiv(rows, 256), 256, 0, st>>>((T *)c.db + v0, db_part, wmax, rows, p.vp, a.tiles_n);
+        CCT_LAUNCH_CHECK();
+      }
     }
     if (c.dx) {
-      vocab_transpose_kernel<T><<<dim3(idiv(mpad, 64), idiv(p.width, 64)), 256, 0, st>>>(
-          wt, (const T *)c.w + (size_t)v0 * p.ldw, p.ldw, p.vp, rows, p.width, mpad, nullptr, 0);
-      CCT_LAUNCH_CHECK();
       ProductArgs a{};
-      a.A = (const char *)wt;
-      a.lda = p.vp * p.el;
+      a.A = w;
+      a.lda = ldw;
+      a.abytes = (uint32_t)(direct_w ? p.width * p.el : packed);
       a.B = (const char *)g;
       a.ldb = p.vp * p.el;
       a.M = p.width;
       a.N = n;
+      a.K = rows;
       a.kbytes = (uint32_t)(mpad * p.el);
-      a.splits = p.dx_splits;
       a.C = slabs;
+      a.ldc = p.hp;
       a.accumulate = v0 > 0;
-      if (int rc = product<T, USE_SLAB>(p.dxs, a)) return rc;
+      if (int rc = product<T, USE_SLAB, false, true>(p.dx, a)) return rc;
     }
     if (c.dw) {
       ProductArgs a{};
-      a.A = (const char *)xt;
-      a.lda = p.np * p.el;
-      a.B = (const char *)gt;
-      a.ldb = p.np * p.el;
+      a.A = (const char *)xlive;
+      a.lda = packed;
+      a.abytes = (uint32_t)packed;
+      a.B = (const char *)g;
+      a.ldb = p.vp * p.el;
+      a.bbytes = (uint32_t)(mpad * p.el);
       a.M = p.width;
       a.N = rows;
-      a.kbytes = (uint32_t)(p.nk * p.el);
-      a.splits = 1;
+      a.K = n;
+      a.wmax = wmax;
       a.C = (T *)c.dw + (size_t)v0 * p.ldw;
       a.ldc = p.ldw;
-      if (int rc = product<T, USE_OUT>(p.dws, a)) return rc;
+      if (int rc = product<T, USE_OUT, false, false>(p.dw, a)) return rc;
     }
   }
   if (c.dx) {
-    vocab_dx_kernel<T><<<n, 256, 0, st>>>((T *)c.dx, slabs, c.labels, c.gscale, c.ignore, n, p.width, p.ldx, p.dx_splits);
+    vocab_dx_kernel<T><<<dim3(n, idiv(p.width, 1024)), 256, 0, st>>>((T *)c.dx, slabs, wmax, n, p.width, p.ldx, p.hp,
+                                                                    p.dx.splits);
     CCT_LAUNCH_CHECK();
   }
   return 0;
@@ -823,7 +1071,7 @@ extern "C" int cct_hip_vocab_loss_backward(void *dx, void *dw, void *db, const v
   c.w = w;
   c.bias = bias;
   c.labels = labels;
-  c.gscale = loss_grad;
+  c.weight = loss_grad;
   c.ignore = args->ignore_label;
   c.ws = (char *)workspace;
   c.backward = true;
@@ -851,7 +1099,7 @@ extern "C" int cct_hip_vocab_loss_forward_backward(float *loss, float *lse, void
   c.w = w;
   c.bias = bias;
   c.labels = labels;
-  c.gscale = loss_grad;
+  c.weight = loss_grad;
   c.ignore = args->ignore_label;
   c.ws = (char *)workspace;
   c.forward = c.backward = true;

@@ -109,7 +109,9 @@ int cct_hip_set_stream(void *hip_stream);
  * apply, 2 = the one-image-per-step kernel always, 0 = automatic), "strided_wgrad" (tile of the strided weight-gradient kernel: pieces of an output row
  * x 1000 + column blocks x 100 + column groups x 10 + row blocks, 0 = automatic), "pool_plane", "gemm_nt", "gemm_tile" (-1 = automatic), "gemm_nodma" (1 = GEMM
  * operand tiles always staged through registers), "conv1x1_per_image" (1 x 1 layers, forward and data gradient: 1 = one
- * product per image, 2 = one product over the pixels of all images, 0 = automatic).  The
+ * product per image, 2 = one product over the pixels of all images, 0 = automatic), "vocab_tile" (tile of the
+ * vocabulary loss's products: 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 = 64 x 32, 0 = automatic), "vocab_keep"
+ * (1 = its scores are kept where they fit the limit, 2 = never, 0 = automatic; both also change what its workspace must hold).  The
  * environment variables CCT_HIP_<NAME IN CAPITALS> give the initial values; they are read once,
  * when the library initialises, never on a launch path.  No counterpart in the reference. */
 int cct_hip_set_tuning(const char *name, int value);
@@ -555,13 +557,13 @@ int cct_hip_embedding_backward(void *dtable, const void *dout, const int *ids, c
  *   dx = G w,  dw = G^T x,  db = column sums of G;  any of the three may be NULL.
  * In bf16, G is rounded to bf16 as an operand of the two products (as an inner-product layer's output gradient
  * is); everything else stays in fp32 up to the final store.
- * forward_backward gives what forward and then backward give; while tokens * vocab * 4 bytes stay within 512 MiB it
- * keeps the fp32 scores in the workspace from one to the other instead of computing them twice. */
+ * forward_backward gives what forward and then backward give, to rounding.  Where that is cheaper, and the fp32 scores
+ * take at most 512 MiB, a call keeps them in the workspace while it runs instead of reducing them tile by tile. */
 typedef struct cct_vocab_loss_args {
   int tokens, width, vocab;
   int dtype; /* of x, w, bias and their gradients */
   int ignore_label;
-  int piece; /* rows of w taken at a time, rounded up to a multiple of 256; 0 = automatic.  A smaller piece needs less workspace */
+  int piece; /* rows of w taken at a time, rounded up to a multiple of 256; 0 = automatic */
   size_t x_stride, w_stride; /* elements between rows of x / dx and of w / dw; 0 = width */
 } cct_vocab_loss_args;
 /* Bytes for the forward pass alone (training == 0) or for any of the three calls (training != 0); 0 for arguments that

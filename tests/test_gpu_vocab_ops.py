@@ -7,7 +7,7 @@ log2 e, and the instruction's own step)."""
 import numpy as np
 import pytest
 
-from gpu_util import driver, host
+from gpu_util import driver, host, tuning
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -231,6 +231,7 @@ class Vocab:
             ep = p * (el + self.else_[:, None] + 8 * U * (big + np.abs(self.lse))[:, None] + 2.0 ** -22)
             ep[~live] = 0.0
         gs = self.gs.astype(np.float64) * live
+        size = np.abs(gs)                                            # bounds go by the magnitude of the weights
         x = np.where(live[:, None], self.x64, 0.0)
         h = HALF[self.dtype]
         eg = ep + h * (np.abs(g) + ep) + U * np.abs(g)               # the operands' rounding
@@ -240,11 +241,11 @@ class Vocab:
         self.g = g
         wsafe = self.w64
         self.dx = gs[:, None] * (g @ wsafe)
-        self.edx = gs[:, None] * ((eg + 2 * (self.vocab + 70) * U * np.abs(g)) @ np.abs(wsafe))
+        self.edx = size[:, None] * ((eg + 2 * (self.vocab + 70) * U * np.abs(g)) @ np.abs(wsafe))
         self.dw = (g * gs[:, None]).T @ x
-        self.edw = ((eg + 2 * (self.tokens + 70) * U * np.abs(g)) * gs[:, None]).T @ np.abs(x)
+        self.edw = ((eg + 2 * (self.tokens + 70) * U * np.abs(g)) * size[:, None]).T @ np.abs(x)
         self.db = (g * gs[:, None]).sum(0)
-        self.edb = ((ep + 3 * TINY + (self.tokens + 4) * U * np.abs(g)) * gs[:, None]).sum(0)
+        self.edb = ((ep + 3 * TINY + (self.tokens + 4) * U * np.abs(g)) * size[:, None]).sum(0)
         for name in ("dx", "dw", "db"):
             value, e = getattr(self, name), getattr(self, "e" + name)
             setattr(self, "e" + name, e + h * (np.abs(value) + e) + 1e-38)
@@ -321,6 +322,29 @@ def test_vocab_loss_with_the_largest_tiles(dtype, tokens, width, vocab, piece):
     v.check_loss()
     v.backward(piece)
     v.check_gradients()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("keep", [1, 2])
+@pytest.mark.parametrize("tokens, width, vocab", [(3, 8, 5), (100, 264, 700), (333, 77, 515), (70, 1048, 1030)])
+def test_vocab_loss_every_tile_with_scores_kept_or_not(dtype, tile, keep, tokens, width, vocab):
+    v = Vocab(dtype, tokens, width, vocab, bias=tokens != 100).reference()
+    with tuning("vocab_tile", tile), tuning("vocab_keep", keep):
+        v.outputs()
+        v.forward()
+        v.check_loss()
+        v.backward()
+        v.check_gradients()
+        v.outputs()
+        v.both()
+        v.check_loss()
+        v.check_gradients()
+        if keep == 2:
+            v.outputs()
+            v.both(piece=256)
+            v.check_loss()
+            v.check_gradients()
 
 
 @pytest.mark.parametrize("dtype", BOTH)
@@ -410,6 +434,27 @@ def test_vocab_loss_of_a_fully_masked_row_is_nan_alone():
     near(values(v.o_lse)[keep], v.lse[keep], v.else_[keep])
     near(values(v.o_loss)[keep], v.loss[keep], v.eloss[keep])
     assert values(v.o_lse)[2] == -np.inf and np.isnan(values(v.o_loss)[2])
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("kind", ["equal", "zero", "negative", "far apart"])
+def test_vocab_loss_weights(dtype, kind):
+    v = Vocab(dtype, 60, 72, 400, bias=True)
+    rng = np.random.default_rng(2)
+    if kind == "equal":
+        v.gs[:] = 1.0 / 57
+    elif kind == "zero":
+        v.gs[:] = 0.0
+    elif kind == "negative":
+        v.gs = -v.gs
+    else:
+        v.gs = (10.0 ** rng.uniform(-12, 6, 60)).astype(np.float32)
+    v.reference()
+    for keep in (1, 2):
+        with tuning("vocab_keep", keep):
+            v.outputs()
+            v.both()
+            v.check_gradients()
 
 
 @pytest.mark.parametrize("dtype", BOTH)

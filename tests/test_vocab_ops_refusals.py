@@ -95,7 +95,7 @@ def test_vocab_loss_refuses_arrays_and_workspaces(drv):
 
 
 def test_vocab_loss_workspace_stays_bounded():
-    """The workspace goes by tokens and piece, not by tokens * vocab; a smaller piece needs less."""
+    """The workspace goes by tokens and piece, not by tokens * vocab; pieces smaller than the automatic ones need less."""
     d = HIPDriver.__new__(HIPDriver)
     d.lib = _lib.load()
     small, large = (d.vocab_loss_workspace_bytes(vocab_loss_args(8192, 4096, v, BF16)) for v in (131072, 4 * 131072))
@@ -103,7 +103,7 @@ def test_vocab_loss_workspace_stays_bounded():
     assert large - small <= 3 * 131072 // 64 * 8192 * 8
     assert small < 2 << 30 < 8192 * 131072 * 4
     pieces = [d.vocab_loss_workspace_bytes(vocab_loss_args(8192, 4096, 131072, BF16, piece=p)) for p in (256, 1024, 4096)]
-    assert pieces[0] < pieces[1] < pieces[2]
+    assert max(pieces) < small
 
 
 @pytest.mark.parametrize("bad, match", [
