@@ -45,6 +45,22 @@ struct Shape {
 };
 
 typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes a lane from global memory into LDS: lane l's land at dst + 16 l; an offset past the descriptor's 2^31 bytes fetches
+// nothing and writes zeros.  The instruction itself instead of its builtin: the compiler would wait for all copies
+// in flight before every ds_read_b64_tr_b16, whose address it cannot tell from theirs (a product with such an operand: 1.43
+// instead of 0.96 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 (the
+// LDS address) is used by nothing else in these kernels.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, uint32_t offset, lds_char *dst) {
+  const uint64_t at = (uint64_t)base;
+  const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, kOutOfRange, 0x00020000u};
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"((uint32_t)(uintptr_t)dst),
+      "v"(lane_offset), "s"(rsrc), "s"(offset)
+      : "memory");
+}
+__device__ __forceinline__ void copy_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -103,27 +119,15 @@ struct Operand {
     }
   }
 
-  // step `step` into LDS at `dst`; what lies past the end of k becomes zero
-  __device__ __forceinline__ void stage(char *dst, int step, int K, uint32_t kbytes, int wave) const {
-    char *to = dst + wave * 1024;
+  // copy j of step `step` into LDS at `dst`; what lies past the end of k becomes zero
+  __device__ __forceinline__ void copy(lds_char *dst, int j, int step, int K, uint32_t kbytes, int wave) const {
+    lds_char *to = dst + wave * 1024 + j * WAVES * 1024;
     if constexpr (KC) {
       const uint32_t k = (uint32_t)step * 128u;
-      const rsrc_t r = make_rsrc(base);
-      const bool in = k + chunk < kbytes;
-#pragma unroll
-      for (int j = 0; j < J; ++j) lds_dma16(r, in ? offset[j] : kOutOfRange, k, (float *)(to + j * WAVES * 1024));
+      copy16(base, k + chunk < kbytes ? offset[j] : kOutOfRange, k, to);
     } else {
-      const rsrc_t r = make_rsrc(base + (size_t)step * step_bytes);
       const int left = K - step * KS;
-      if (left >= KS) {
-#pragma unroll
-        for (int j = 0; j < J; ++j) lds_dma16(r, offset[j], 0, (float *)(to + j * WAVES * 1024));
-      } else {
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          lds_dma16(r, krow + j * (WAVES * 1024 / ROWB) < left ? offset[j] : kOutOfRange, 0,
-                    (float *)(to + j * WAVES * 1024));
-      }
+      copy16(base + (size_t)step * step_bytes, krow + j * (WAVES * 1024 / ROWB) < left ? offset[j] : kOutOfRange, 0, to);
     }
   }
 
@@ -182,16 +186,13 @@ struct ProductArgs {
   int accumulate;
 };
 
-template <class T>
-__device__ __forceinline__ void mfma_chunk(f32x4 &c, const f32x4 &a, const f32x4 &b);
-template <>
-__device__ __forceinline__ void mfma_chunk<bf16>(f32x4 &c, const f32x4 &a, const f32x4 &b) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma_bf16(const f32x4 &a, const f32x4 &b, const f32x4 &c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-template <>
-__device__ __forceinline__ void mfma_chunk<float>(f32x4 &c, const f32x4 &a, const f32x4 &b) {
+__device__ __forceinline__ f32x4 mfma_f32(const f32x4 &a, const f32x4 &b, f32x4 c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
 }
 
 // A token's part in the gradient.  Ignored tokens have no part: their G is 0 whatever their scores are.
@@ -271,56 +272,89 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int steps = (p.K + OpA::KS - 1) / OpA::KS;
   const int s0 = (int)split * p.steps_per_split, s1 = min(steps, s0 + p.steps_per_split);
   auto stage = [&](int buf, int step) {
-    opa.stage(lds + buf * S::STAGE, step, p.K, p.kbytes, wave);
-    opb.stage(lds + buf * S::STAGE + S::BM * 128, step, p.K, p.kbytes, wave);
-  };
-  // A step is cut into phases of MH x NI blocks; while one phase's MFMAs run, the next one's fragments are read.  The last
-  // phase of a step reads the other stage, so the barrier stands before it: every wavefront then has all it needs of
-  // this stage in registers, and the copies of the step after next may overwrite it.
-  constexpr int MH = MI % 2 == 0 ? MI / 2 : MI, H = MI / MH, PHASES = 2 * H;
-  f32x4 a[2][MH], b[2][NI];
-  auto read_a = [&](int to, const int buf, int sub, int h) {
-    lds_char *t = (lds_char *)lds + buf * S::STAGE;
 #pragma unroll
-    for (int i = 0; i < MH; ++i) a[to][i] = OpA::fragment(t, fa[h * MH + i], sub);
-  };
-  auto read_b = [&](int to, const int buf, int sub) {
-    lds_char *t = (lds_char *)lds + buf * S::STAGE + S::BM * 128;
+    for (int j = 0; j < OpA::J; ++j) opa.copy((lds_char *)lds + buf * S::STAGE, j, step, p.K, p.kbytes, wave);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) b[to][j] = OpB::fragment(t, fb[j], sub);
+    for (int j = 0; j < OpB::J; ++j) opb.copy((lds_char *)lds + buf * S::STAGE + S::BM * 128, j, step, p.K, p.kbytes, wave);
   };
-  if (s0 < s1) {
-    stage(0, s0);
-    lds_dma_wait();
-    __syncthreads();
-    if (s0 + 1 < s1) stage(1, s0 + 1);
-    read_a(0, 0, 0, 0);
-    read_b(0, 0, 0);
-  }
-  for (int s = s0; s < s1; ++s) {
-    const int buf = (s - s0) & 1;
+  if constexpr (std::is_same<T, float>::value) {
+    // fp32: a step's MFMAs take eight times as long as its reads; one barrier per step and the compiler's own order
+    if (s0 < s1) stage(0, s0);
+    for (int s = s0; s < s1; ++s) {
+      copy_wait();
+      __syncthreads();
+      const int buf = (s - s0) & 1;
+      if (s + 1 < s1) stage(buf ^ 1, s + 1);
+      lds_char *ta = (lds_char *)lds + buf * S::STAGE, *tb = ta + S::BM * 128;
 #pragma unroll
-    for (int q = 0; q < PHASES; ++q) {
-      const int sub = q / H, h = q % H;
-      if (q + 1 < PHASES) {
-        read_a((q + 1) & 1, buf, (q + 1) / H, (q + 1) % H);
-        if ((q + 1) % H == 0) read_b((q + 1) / H, buf, (q + 1) / H);
-      } else {
-        lds_dma_wait();
-        __syncthreads();
-        if (s + 2 < s1) stage(buf, s + 2);
-        if (s + 1 < s1) {
-          read_a(0, buf ^ 1, 0, 0);
-          read_b(0, buf ^ 1, 0);
+      for (int sub = 0; sub < 2; ++sub) {
+        f32x4 a[MI], b[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = OpA::fragment(ta, fa[i], sub);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b[j] = OpB::fragment(tb, fb[j], sub);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = mfma_f32(a[i], b[j], acc[i][j]);
+      }
+    }
+  } else {
+    // A step is cut into phases of MH x NI blocks; while one phase's MFMAs run, the next one's fragments are read.  The last
+    // phase of a step reads the other stage, so the barrier stands before it: every wavefront then has all it needs of
+    // this stage in registers, and the copies of the step after next may overwrite it.  Reads and copies stand between
+    // the MFMAs in the order of the source, so that neither unit gets a burst that holds the other up.
+    constexpr int MH = MI % 2 == 0 ? MI / 2 : MI, H = MI / MH, PHASES = 2 * H, MFMAS = MH * NI;
+    f32x4 a[2][MH], b[2][NI];
+    auto read = [&](int item, int to, int buf, int sub, int h) {  // items 0..MH-1: A, then B
+      lds_char *t = (lds_char *)lds + buf * S::STAGE;
+      if (item < MH)
+        a[to][item] = OpA::fragment(t, fa[h * MH + item], sub);
+      else
+        b[sub][item - MH] = OpB::fragment(t + S::BM * 128, fb[item - MH], sub);
+    };
+    if (s0 < s1) {
+      stage(0, s0);
+      copy_wait();
+      __syncthreads();
+      if (s0 + 1 < s1) stage(1, s0 + 1);
+#pragma unroll
+      for (int i = 0; i < MH + NI; ++i) read(i, 0, 0, 0, 0);
+    }
+    for (int s = s0; s < s1; ++s) {
+      const int buf = (s - s0) & 1;
+#pragma unroll
+      for (int q = 0; q < PHASES; ++q) {
+        const bool last = q + 1 == PHASES;
+        const int sub = q / H, h = q % H, nsub = last ? 0 : (q + 1) / H, nh = last ? 0 : (q + 1) % H;
+        if (last) {
+          copy_wait();
+          __syncthreads();
+        }
+        const int reads = MH + (nh == 0 ? NI : 0), copies = last ? OpA::J + OpB::J : 0, items = reads + copies;
+#pragma unroll
+        for (int m = 0; m < MFMAS; ++m) {
+#pragma unroll
+          for (int it = 0; it < items; ++it) {
+            if (it * MFMAS / items != m) continue;
+            // the last phase alternates between copies and reads
+            const int c = last ? (it < 2 * min(copies, reads) ? ((it & 1) ? -1 : it / 2) : (copies > reads ? it - reads : -1)) : -1;
+            const int r = last ? (it < 2 * min(copies, reads) ? it / 2 : it - copies) : it;
+            // past the end both are harmless: the copies fetch nothing, and what is read is not used
+            if (c >= 0 && c < OpA::J)
+              opa.copy((lds_char *)lds + buf * S::STAGE, c, s + 2, p.K, p.kbytes, wave);
+            else if (c >= 0)
+              opb.copy((lds_char *)lds + buf * S::STAGE + S::BM * 128, c - OpA::J, s + 2, p.K, p.kbytes, wave);
+            else
+              read(r, (q + 1) & 1, last ? buf ^ 1 : buf, nsub, nh);
+          }
+          const int i = m / NI, j = m % NI;
+          acc[h * MH + i][j] = mfma_bf16(a[q & 1][i], b[sub][j], acc[h * MH + i][j]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < MH; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) mfma_chunk<T>(acc[h * MH + i][j], a[q & 1][i], b[sub][j]);
-      __builtin_amdgcn_sched_barrier(0);
     }
+    copy_wait();  // no copy may land after this workgroup's use of its LDS
   }
 
   // this lane's elements: rows mrow + 16 i + r, columns ncol + 16 j
@@ -446,18 +480,32 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 
 // ---- copies and statistics before the products ---------------------------------------------------------------------
 // dst[r][c] = src[r][c], rows of dst filled up to cpad with zeros: operands whose rows do not start at 16-byte
-// boundaries or are no whole number of 16-byte chunks.  With labels, the rows of ignored tokens become zero, so that
-// whatever their x holds stays out of dw; with weights, one workgroup more takes the largest magnitude of the live ones.
+// boundaries or are no whole number of 16-byte chunks.
 template <class T>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, const T *__restrict__ src, size_t ld_src,
-                                                         int rows, int cols, int cpad, const int *__restrict__ labels,
-                                                         int ignore, const float *__restrict__ weight,
-                                                         float *__restrict__ wmax) {
+                                                         int cols, int cpad) {
   constexpr int V = Num<T>::V;
-  if ((int)blockIdx.x == rows) {
-    __shared__ float sh[256];
+  const size_t r = blockIdx.x;
+  for (int c = threadIdx.x * V; c < cpad; c += 256 * V) {
+    float f[V];
+    load_vec<T>(f, src + r * ld_src, c, cols);
+    store_vec<T>(dst + r * cpad, f, c, cpad);
+  }
+}
+
+// xt[c][t] = x[t][c], columns of xt zero for tokens past the end and for ignored ones, so that whatever their x holds stays
+// out of dw.  With weights, one workgroup more takes the largest magnitude of those of the other tokens.
+template <class T>
+__global__ __launch_bounds__(256) void vocab_xt_kernel(T *__restrict__ xt, const T *__restrict__ x, size_t ldx, size_t ldt,
+                                                       int tokens, int width, int tpad, int tiles_t,
+                                                       const int *__restrict__ labels, int ignore,
+                                                       const float *__restrict__ weight, float *__restrict__ wmax,
+                                                       int tiles) {
+  __shared__ T tile[64][64 + 4 / sizeof(T)];
+  if ((int)blockIdx.x == tiles) {
+    float *sh = (float *)tile;
     float m = 0.0f;
-    for (int t = threadIdx.x; t < rows; t += 256)
+    for (int t = threadIdx.x; t < tokens; t += 256)
       if (labels[t] != ignore) m = fmaxf(m, fabsf(weight[t]));
     sh[threadIdx.x] = m;
     __syncthreads();
@@ -468,17 +516,19 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, co
     if (threadIdx.x == 0) *wmax = sh[0];
     return;
   }
-  const size_t r = blockIdx.x;
-  const bool live = !labels || labels[r] != ignore;
-  for (int c = threadIdx.x * V; c < cpad; c += 256 * V) {
-    float f[V];
-    if (live) {
-      load_vec<T>(f, src + r * ld_src, c, cols);
-    } else {
+  const int t0 = (int)(blockIdx.x % tiles_t) * 64, c0 = (int)(blockIdx.x / tiles_t) * 64;
+  const int lane = threadIdx.x & 63, y = threadIdx.x >> 6;
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 0.0f;
-    }
-    store_vec<T>(dst + r * cpad, f, c, cpad);
+  for (int i = 0; i < 16; ++i) {
+    const int t = t0 + y + i * 4, c = c0 + lane;
+    const bool in = t < tokens && c < width && labels[t] != ignore;
+    tile[y + i * 4][lane] = in ? x[(size_t)t * ldx + c] : (T)0.0f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = c0 + y + i * 4, t = t0 + lane;
+    if (c < width && t < tpad) xt[(size_t)c * ldt + t] = tile[lane][y + i * 4];
   }
 }
 
@@ -638,6 +688,7 @@ __global__ __launch_bounds__(256) void vocab_zero_kernel(T *__restrict__ p, size
 
 // ---- host --------------------------------------------------------------------------------------------------------
 typedef Shape<256, 256, 2, 4> ShapeL;
+typedef Shape<256, 256, 4, 2> ShapeLA;  // the same tile with fewer fragments of A per wavefront: A contiguous along its rows
 typedef Shape<128, 128, 2, 2> ShapeM;
 typedef Shape<64, 64, 2, 2> ShapeN;
 typedef Shape<64, 32, 4, 1> ShapeS;
@@ -699,12 +750,12 @@ struct VocabPlan {
   size_t el, ldx, ldw;
   int unit;            // elements of a 128-byte step
   int piece, pieces;   // rows of w at a time
-  int hp, vp;          // row lengths of packed and of G: width, piece rounded up to whole steps
+  int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, kept, dx, dw;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward, keep_both;
   int stats_tiles;
-  size_t part, label_score, xpack, wpack, scores, xlive, wmax, g, slabs, db, total_forward, total;
+  size_t part, label_score, xpack, wpack, scores, xt, wmax, g, slabs, db, total_forward, total;
 };
 
 static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
@@ -718,6 +769,7 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.ldw = a->w_stride ? a->w_stride : (size_t)a->width;
   p.unit = 128 / (int)p.el;
   p.hp = idiv(p.width, p.unit) * p.unit;
+  p.np = (idiv(p.tokens, p.unit) + 1) * p.unit;
   const size_t n = p.tokens;
   const int vmax = idiv(p.vocab, 256) * 256;
   if (a->piece > 0) {
@@ -744,7 +796,7 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   if (tuning().vocab_keep) p.keep_forward = p.keep_backward = p.keep_both = fits && tuning().vocab_keep == 1;
   if (p.keep_forward || p.keep_backward || p.keep_both) p.piece = vmax;
   p.pieces = idiv(p.vocab, p.piece);
-  p.vp = p.piece;
+  p.vp = p.piece + p.unit;
   p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
   p.stats_tiles = 0;
   for (int v = 0; v < p.vocab; v += p.piece) p.stats_tiles += idiv(min(p.piece, p.vocab - v), kTiles[p.stats.shape].bm);
@@ -761,11 +813,11 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.label_score = take(n * 4);
   p.xpack = take(n * p.hp * p.el);
   p.wpack = take((size_t)p.piece * p.hp * p.el);
-  const size_t score_space = (size_t)p.kept.splits * n * vmax * 4;
+  const size_t score_space = (size_t)p.kept.splits * n * p.vp * 4;
   p.scores = take(p.keep_forward ? score_space : 0);
   p.total_forward = at;
   if (!p.keep_forward) p.scores = take(keep_any ? score_space : 0);
-  p.xlive = take(n * p.hp * p.el);
+  p.xt = take((size_t)p.width * p.np * p.el);
   p.wmax = take(4);
   p.g = take(n * p.vp * p.el);
   p.slabs = take((size_t)p.dx.splits * n * p.hp * 4);
@@ -798,7 +850,7 @@ template <class T, int USE, bool KA, bool KB>
 static int product(const Choice &c, ProductArgs &p) {
   p.splits = c.splits;
   switch (c.shape) {
-    case SHAPE_L: return launch_product<T, ShapeL, USE, KA, KB>(p);
+    case SHAPE_L: return launch_product<T, typename std::conditional<KA, ShapeL, ShapeLA>::type, USE, KA, KB>(p);
     case SHAPE_M: return launch_product<T, ShapeM, USE, KA, KB>(p);
     case SHAPE_N: return launch_product<T, ShapeN, USE, KA, KB>(p);
     default:
@@ -834,15 +886,16 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   SoftStat *part = (SoftStat *)(c.ws + p.part);
   float *label_score = (float *)(c.ws + p.label_score), *scores = (float *)(c.ws + p.scores);
   float *slabs = (float *)(c.ws + p.slabs), *db_part = (float *)(c.ws + p.db);
-  T *g = (T *)(c.ws + p.g), *xlive = (T *)(c.ws + p.xlive);
+  T *g = (T *)(c.ws + p.g), *xt = (T *)(c.ws + p.xt);
   if (keep && p.el == 4) g = (T *)scores;  // fp32 G takes the scores' place
   const size_t packed = p.hp * p.el;
+  const int chunk = p.unit / 8;  // elements of 16 bytes
   const bool direct_x = direct_rows(c.x, p.ldx, p.width, p.el), direct_w = direct_rows(c.w, p.ldw, p.width, p.el);
   const char *x = (const char *)c.x;
   size_t ldx = p.ldx * p.el;
   if (!direct_x) {
     T *xp = (T *)(c.ws + p.xpack);
-    vocab_pack_kernel<T><<<n, 256, 0, st>>>(xp, (const T *)c.x, p.ldx, n, p.width, p.hp, nullptr, 0, nullptr, nullptr);
+    vocab_pack_kernel<T><<<n, 256, 0, st>>>(xp, (const T *)c.x, p.ldx, p.width, p.hp);
     CCT_LAUNCH_CHECK();
     x = (const char *)xp;
     ldx = packed;
@@ -850,8 +903,10 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   const float *wmax = nullptr;
   if (c.backward) {
     if (c.weight) wmax = (const float *)(c.ws + p.wmax);
-    vocab_pack_kernel<T><<<n + (c.weight ? 1 : 0), 256, 0, st>>>(xlive, (const T *)c.x, p.ldx, n, p.width, p.hp, c.labels,
-                                                                c.ignore, c.weight, (float *)(c.ws + p.wmax));
+    const int tiles_t = idiv(n, 64), tiles = tiles_t * idiv(p.width, 64);
+    vocab_xt_kernel<T><<<tiles + (c.weight ? 1 : 0), 256, 0, st>>>(xt, (const T *)c.x, p.ldx, p.np, n, p.width, idiv(n, chunk) * chunk, tiles_t,
+                                                                  c.labels, c.ignore, c.weight,
+                                                                  (float *)(c.ws + p.wmax), tiles);
     CCT_LAUNCH_CHECK();
   }
   // the piece's rows of w as an operand
@@ -860,7 +915,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     *out = (const char *)c.w + (size_t)v0 * p.ldw * p.el;
     if (direct_w) return 0;
     T *wp = (T *)(c.ws + p.wpack);
-    vocab_pack_kernel<T><<<rows, 256, 0, st>>>(wp, (const T *)*out, p.ldw, rows, p.width, p.hp, nullptr, 0, nullptr, nullptr);
+    vocab_pack_kernel<T><<<rows, 256, 0, st>>>(wp, (const T *)*out, p.ldw, p.width, p.hp);
     CCT_LAUNCH_CHECK();
     *out = (const char *)wp;
     return 0;
@@ -882,7 +937,6 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     return a;
   };
   const char *w = nullptr;
-  const int chunk = p.unit / 8;
   if (keep) {
     if (int rc = rows_of_w(0, p.vocab, &w)) return rc;
     ProductArgs a = score_args(w, 0, p.vocab);
@@ -957,9 +1011,9 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     }
     if (c.dw) {
       ProductArgs a{};
-      a.A = (const char *)xlive;
-      a.lda = packed;
-      a.abytes = (uint32_t)packed;
+      a.A = (const char *)xt;
+      a.lda = p.np * p.el;
+      a.kbytes = (uint32_t)(idiv(n, chunk) * chunk * p.el);
       a.B = (const char *)g;
       a.ldb = p.vp * p.el;
       a.bbytes = (uint32_t)(mpad * p.el);
@@ -969,7 +1023,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
       a.wmax = wmax;
       a.C = (T *)c.dw + (size_t)v0 * p.ldw;
       a.ldc = p.ldw;
-      if (int rc = product<T, USE_OUT, false, false>(p.dw, a)) return rc;
+      if (int rc = product<T, USE_OUT, true, false>(p.dw, a)) return rc;
     }
   }
   if (c.dx) {
