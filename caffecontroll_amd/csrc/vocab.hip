@@ -214,10 +214,21 @@ __device__ __forceinline__ TokenGrad token_grad(int t, int tokens, const int *__
   }
   return g;
 }
-__device__ __forceinline__ float grad_entry(float score, const TokenGrad &tg, int v) {
-  if (!tg.live) return 0.0f;
+__device__ __forceinline__ float grad_entry(float score, const TokenGrad &tg, bool is_label) {
   const float p = exp2_fast((score - tg.lse) * kLog2e);
-  return tg.weight * (v == tg.label ? p - 1.0f : p);
+  return tg.live ? tg.weight * (p - (is_label ? 1.0f : 0.0f)) : 0.0f;
+}
+
+// Sum over the 16 lanes of a row of lanes, in all of them (rotations by 8, 4, 2, 1 within the row).
+template <int ROT>
+__device__ __forceinline__ float row_rotate(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + ROT, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_sum16(float v) {
+  v += row_rotate<8>(v);
+  v += row_rotate<4>(v);
+  v += row_rotate<2>(v);
+  return v + row_rotate<1>(v);
 }
 
 // Four consecutive elements, of which those below `left` exist.
@@ -374,6 +385,15 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
           for (int j = 0; j < NI; ++j) acc[i][j][r] += b;
         }
     }
+    if (m0 + S::BM > p.M) {  // rows past the piece have no part in any sum
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (mrow + i * 16 + r >= p.M)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j][r] = neg_inf();
+    }
   }
 
   if constexpr (USE == USE_STATS) {
@@ -382,16 +402,18 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
     for (int j = 0; j < NI; ++j) {
       const int t = ncol + j * 16;
       const int label = t < p.N ? p.labels[t] : -1;
+      // the label among this lane's rows: 16 i + r, or out of their range
+      const int at = label >= p.v0 && label < p.v0 + p.M ? label - p.v0 - mrow : -1;
+      float score = 0.0f;
       SoftStat st{neg_inf(), 0.0f};
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int m = mrow + i * 16 + r;
-          if (p.v0 + m == label && m < p.M) p.label_score[t] = acc[i][j][r];
-          acc[i][j][r] = m < p.M ? acc[i][j][r] : neg_inf();
+          score = at == i * 16 + r ? acc[i][j][r] : score;
           st.m = fmaxf(st.m, acc[i][j][r]);
         }
+      if (at >= 0 && at < MI * 16 && (at & 15) < 4) p.label_score[t] = score;
       const float base = st.m == neg_inf() ? 0.0f : st.m;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
@@ -413,23 +435,19 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 
   if constexpr (USE == USE_GRAD) {
     float *sums = (float *)lds;  // [WN][BM] column sums for db
-    float rows[MI][4];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) rows[i][r] = 0.0f;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int t = ncol + j * 16;
       const TokenGrad tg = token_grad(t, p.N, p.labels, p.ignore, p.lse, p.weight, p.wmax);
+      const int at = tg.label >= p.v0 && tg.label < p.v0 + p.M ? tg.label - p.v0 - mrow : -1;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = mrow + i * 16;
         float g[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          g[r] = m + r < p.M ? grad_entry(acc[i][j][r], tg, p.v0 + m + r) : 0.0f;
-          rows[i][r] += g[r];
+          g[r] = grad_entry(acc[i][j][r], tg, at == i * 16 + r);
+          acc[i][j][r] = g[r];
         }
         if (t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g, 4);
       }
@@ -439,9 +457,11 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          float row = acc[i][0][r];
 #pragma unroll
-          for (int d = 1; d < 16; d <<= 1) rows[i][r] += __shfl_xor(rows[i][r], d, 64);
-          if (frow == 0) sums[wn * S::BM + (wm * MI + i) * 16 + fgroup * 4 + r] = rows[i][r];
+          for (int j = 1; j < NI; ++j) row += acc[i][j][r];
+          row = row_sum16(row);
+          if (frow == 0) sums[wn * S::BM + (wm * MI + i) * 16 + fgroup * 4 + r] = row;
         }
       __syncthreads();
       for (int m = tid; m < S::BM; m += S::THREADS) {
@@ -493,8 +513,41 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, co
   }
 }
 
-// xt[c][t] = x[t][c], columns of xt zero for tokens past the end and for ignored ones, so that whatever their x holds stays
-// out of dw.  With weights, one workgroup more takes the largest magnitude of those of the other tokens.
+// The largest magnitude among the weights of the tokens that are not ignored, by one workgroup.
+__device__ __forceinline__ void largest_weight(float *__restrict__ wmax, float *sh, const float *__restrict__ weight,
+                                               const int *__restrict__ labels, int tokens, int ignore) {
+  float m = 0.0f;
+  for (int t = threadIdx.x; t < tokens; t += 256)
+    if (labels[t] != ignore) m = fmaxf(m, fabsf(weight[t]));
+  sh[threadIdx.x] = m;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) sh[threadIdx.x] = fmaxf(sh[threadIdx.x], sh[threadIdx.x + d]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *wmax = sh[0];
+}
+
+// x as dw's operand, zero for ignored tokens, so that whatever their x holds stays out of the product.  bf16: transposed,
+// xt[c][t] = x[t][c] for t < tpad (zero past the end), since a transposed read of both operands from LDS is slower than
+// of one.  fp32: xl[t][c] for c < cpad.  With weights, one workgroup more takes the largest of them.
+template <class T>
+__global__ __launch_bounds__(256) void vocab_live_kernel(T *__restrict__ xl, const T *__restrict__ x, size_t ldx, int tokens,
+                                                         int width, int cpad, const int *__restrict__ labels, int ignore,
+                                                         const float *__restrict__ weight, float *__restrict__ wmax) {
+  constexpr int V = Num<T>::V;
+  __shared__ float sh[256];
+  const int t = blockIdx.x;
+  if (t == tokens) return largest_weight(wmax, sh, weight, labels, tokens, ignore);
+  const bool live = labels[t] != ignore;
+  for (int c = threadIdx.x * V; c < cpad; c += 256 * V) {
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = 0.0f;
+    if (live) load_vec<T>(f, x + (size_t)t * ldx, c, width);
+    store_vec<T>(xl + (size_t)t * cpad, f, c, cpad);
+  }
+}
 template <class T>
 __global__ __launch_bounds__(256) void vocab_xt_kernel(T *__restrict__ xt, const T *__restrict__ x, size_t ldx, size_t ldt,
                                                        int tokens, int width, int tpad, int tiles_t,
@@ -503,17 +556,7 @@ __global__ __launch_bounds__(256) void vocab_xt_kernel(T *__restrict__ xt, const
                                                        int tiles) {
   __shared__ T tile[64][64 + 4 / sizeof(T)];
   if ((int)blockIdx.x == tiles) {
-    float *sh = (float *)tile;
-    float m = 0.0f;
-    for (int t = threadIdx.x; t < tokens; t += 256)
-      if (labels[t] != ignore) m = fmaxf(m, fabsf(weight[t]));
-    sh[threadIdx.x] = m;
-    __syncthreads();
-    for (int d = 128; d > 0; d >>= 1) {
-      if ((int)threadIdx.x < d) sh[threadIdx.x] = fmaxf(sh[threadIdx.x], sh[threadIdx.x + d]);
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) *wmax = sh[0];
+    largest_weight(wmax, (float *)tile, weight, labels, tokens, ignore);
     return;
   }
   const int t0 = (int)(blockIdx.x % tiles_t) * 64, c0 = (int)(blockIdx.x / tiles_t) * 64;
@@ -572,7 +615,7 @@ __global__ __launch_bounds__(256) void vocab_loss_kernel(float *__restrict__ los
     store_loss(loss, lse, t, log_sum(sh[0][x], 1.0f), labels[t], label_score[t], vocab, ignore);
 }
 
-// Kept scores of one token: the parts that the product was cut into are added up (in order) and the bias on top, then
+// Kept scores of one token: the parts that the product was cut into are added up in order, then
 // lse and loss (forward), then G (backward) in T; fp32 G takes the place of the scores, and so does bf16's unrounded G where
 // db needs its column sums.  A workgroup per token; the second walk over the row finds it in a cache.
 template <class T>
@@ -587,20 +630,21 @@ __global__ __launch_bounds__(512) void vocab_row_kernel(float *__restrict__ loss
   const int t = blockIdx.x, tid = threadIdx.x;
   float *row = scores + (size_t)t * ld;
   const size_t part = (size_t)tokens * ld;
-  const bool sum = splits > 1 || bias;
   const int label = labels[t];
+  auto add_bias = [&](f32x4 &v, int c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < vocab) v[i] += (float)bias[c + i];
+  };
   SoftStat st{neg_inf(), 0.0f};
   // ld is a multiple of four and rows start at 16-byte boundaries
-  for (int c = tid * 4; c < vocab; c += 512 * 4) {
+  for (int c = tid * 4; c < vocab && (loss || splits > 1); c += 512 * 4) {
     f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
-    if (sum) {
+    if (splits > 1) {
       for (int i = 1; i < splits; ++i) v += *reinterpret_cast<const f32x4 *>(row + i * part + c);
-      if (bias)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + i < vocab) v[i] += (float)bias[c + i];
       *reinterpret_cast<f32x4 *>(row + c) = v;
     }
+    if (bias) add_bias(v, c);
     if (loss) {
       float m = st.m;
 #pragma unroll
@@ -625,7 +669,8 @@ __global__ __launch_bounds__(512) void vocab_row_kernel(float *__restrict__ loss
       for (int i = 1; i < 8; ++i) st = join(st, sh[i], kLog2e);
       const float l = log_sum(st, 1.0f);
       lse_sh = l;
-      store_loss(loss, lse_out, t, l, label, (unsigned)label < (unsigned)vocab ? row[label] : 0.0f, vocab, ignore);
+      const bool in = (unsigned)label < (unsigned)vocab;
+      store_loss(loss, lse_out, t, l, label, in ? row[label] + (bias ? (float)bias[label] : 0.0f) : 0.0f, vocab, ignore);
     }
   } else if (tid == 0) {
     lse_sh = lse_in[t];
@@ -635,23 +680,33 @@ __global__ __launch_bounds__(512) void vocab_row_kernel(float *__restrict__ loss
   TokenGrad tg = token_grad(0, 1, labels + t, ignore, &lse_sh, weight ? weight + t : nullptr, wmax);
   for (int c = tid * 4; c < mpad; c += 512 * 4) {
     float f[4];
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
+    f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
+    if (bias) add_bias(v, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = c + i < vocab ? grad_entry(v[i], tg, c + i) : 0.0f;
+    for (int i = 0; i < 4; ++i) f[i] = c + i < vocab ? grad_entry(v[i], tg, c + i == label) : 0.0f;
     if (keep_g || std::is_same<T, float>::value) *reinterpret_cast<f32x4 *>(row + c) = f32x4{f[0], f[1], f[2], f[3]};
     if (!std::is_same<T, float>::value) store4<T>(g + (size_t)t * ld + c, f, 4);
   }
 }
 
-// Column sums of 64 tokens' G.
-__global__ __launch_bounds__(256) void vocab_colsum_kernel(float *__restrict__ part, const float *__restrict__ g, size_t ldg,
-                                                           int tokens, int rows, int ld) {
-  const int m = blockIdx.x * 256 + threadIdx.x, t0 = blockIdx.y * 64, t1 = min(tokens, t0 + 64);
-  if (m >= rows) return;
+// db = *wmax times the column sums of kept G: 64 columns a workgroup, its 16 wavefronts taking every 16th token each.
+template <class T>
+__global__ __launch_bounds__(1024) void vocab_colsum_kernel(T *__restrict__ db, const float *__restrict__ g, size_t ldg,
+                                                            const float *__restrict__ wmax, int tokens, int rows) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, m = blockIdx.x * 64 + lane;
   float s = 0.0f;
+  if (m < rows) {
 #pragma unroll 8
-  for (int t = t0; t < t1; ++t) s += g[(size_t)t * ldg + m];
-  part[(size_t)blockIdx.y * ld + m] = s;
+    for (int t = y; t < tokens; t += 16) s += g[(size_t)t * ldg + m];
+  }
+  sh[y][lane] = s;
+  __syncthreads();
+  if (y == 0 && m < rows) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sh[i][lane];
+    db[m] = (T)(wmax ? s * *wmax : s);
+  }
 }
 
 // dx[t] = *wmax times the sum of the slabs, in order; nothing for ignored tokens
@@ -697,19 +752,21 @@ static int idiv(int a, int b) { return (a + b - 1) / b; }
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Which tile a product takes and into how many parts it is cut along k: the cheapest by a small model of the chip.  A
-// workgroup's step costs `alone` microseconds when it has a CU to itself and `full` when `occ` of them share it.
+// workgroup's step costs `alone` microseconds when it has a CU to itself and `full` when `occ` of them share it; `finish`
+// is what a round of tiles pays before and after its steps.  Measured with each tile pinned: tokens 256, width 4096, 1000
+// rows (alone) and tokens 2048, width 2048, 32768 rows (full).
 struct TileCost {
   int bm, bn, occ;
-  double alone[2], full[2];  // fp32, bf16
+  double alone[2], full[2], finish;  // fp32, bf16
 };
 enum ShapeId { SHAPE_L, SHAPE_M, SHAPE_N, SHAPE_S, SHAPES };
 static const TileCost kTiles[SHAPES] = {
-    {ShapeL::BM, ShapeL::BN, 1, {8.5, 1.75}, {8.5, 1.75}},
-    {ShapeM::BM, ShapeM::BN, 2, {2.2, 0.80}, {4.1, 1.30}},
-    {ShapeN::BM, ShapeN::BN, 4, {0.7, 0.50}, {2.2, 0.90}},
-    {ShapeS::BM, ShapeS::BN, 6, {0.4, 0.40}, {1.8, 0.90}},
+    {ShapeL::BM, ShapeL::BN, 1, {7.35, 1.28}, {7.50, 1.62}, 10.0},
+    {ShapeM::BM, ShapeM::BN, 2, {2.06, 0.72}, {3.88, 1.05}, 6.0},
+    {ShapeN::BM, ShapeN::BN, 4, {0.65, 0.50}, {1.97, 0.67}, 3.0},
+    {ShapeS::BM, ShapeS::BN, 6, {0.46, 0.50}, {1.50, 0.71}, 2.0},
 };
-constexpr double kLaunchUs = 3.0, kBytesPerUs = 4.0e6;  // what a launch costs, and a pass over memory
+constexpr double kLaunchUs = 3.0, kBytesPerUs = 5.0e6;  // what a launch costs, and a pass over memory
 
 struct Choice {
   ShapeId shape;
@@ -732,7 +789,9 @@ static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow
       const double rounds = (double)(long)(w / round), per_cu = (double)(long)((w - rounds * round + 255.0) / 256.0);
       const double last = per_cu * c.full[d] / c.occ;
       const double step = rounds * c.full[d] + (per_cu > 0 ? (last > c.alone[d] ? last : c.alone[d]) : 0.0);
-      const double us = step * idiv(steps, splits) + kLaunchUs +
+      // (parts are written by the product and read by what joins them)
+      const double work = step * idiv(steps, splits), bytes = ((double)M + N) * K * (d ? 2 : 4);
+      const double us = (work * kBytesPerUs > bytes ? work : bytes / kBytesPerUs) + kLaunchUs + c.finish * (rounds + (per_cu > 0 ? 1 : 0)) +
                         (may_split ? 2.0 * splits * M * (double)N * 4.0 / kBytesPerUs : 0.0);
       if (us < best.us) best = Choice{(ShapeId)s, splits, us};
     }
@@ -753,9 +812,9 @@ struct VocabPlan {
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, kept, dx, dw;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
-  bool keep_forward, keep_backward, keep_both;
+  bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
   int stats_tiles;
-  size_t part, label_score, xpack, wpack, scores, xt, wmax, g, slabs, db, total_forward, total;
+  size_t part, label_score, xpack, wpack, scores, xl, wmax, g, slabs, db, total_forward, total;
 };
 
 static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
@@ -788,13 +847,20 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, true, true);
   const double score_bytes = (double)n * vmax * 4;
   const double stats_us = p.stats.us * idiv(p.vocab, p.piece) + kLaunchUs;
-  const double join_us = kLaunchUs + score_bytes / kBytesPerUs, grad_us = score_bytes * 2 / kBytesPerUs;
+  // (the choice's own cost has the scores written and read once; G is written on top, in place of the scores in fp32)
+  const double join_us = kLaunchUs, grad_us = (double)n * vmax * p.el / kBytesPerUs;
   const bool fits = may_keep && score_bytes * p.kept.splits <= (double)kKeepBytes;
   p.keep_forward = fits && p.kept.us + join_us < stats_us;
-  p.keep_backward = fits && p.kept.us + join_us + grad_us < stats_us;
-  p.keep_both = fits && p.kept.us + join_us + grad_us < 2 * stats_us;
-  if (tuning().vocab_keep) p.keep_forward = p.keep_backward = p.keep_both = fits && tuning().vocab_keep == 1;
-  if (p.keep_forward || p.keep_backward || p.keep_both) p.piece = vmax;
+  bool keep_any = p.keep_forward;
+  for (int db = 0; db < 2; ++db) {
+    // the column sums read the kept G (in bf16 it is written in fp32 for them), those of a GRAD product come with it
+    const double db_us = db ? kLaunchUs + score_bytes * (p.el == 4 ? 1 : 2) / kBytesPerUs : 0.0;
+    p.keep_backward[db] = fits && p.kept.us + join_us + grad_us + db_us < stats_us;
+    p.keep_both[db] = fits && p.kept.us + join_us + grad_us + db_us < 2 * stats_us;
+    if (tuning().vocab_keep) p.keep_forward = p.keep_backward[db] = p.keep_both[db] = fits && tuning().vocab_keep == 1;
+    keep_any = keep_any || p.keep_forward || p.keep_backward[db] || p.keep_both[db];
+  }
+  if (keep_any) p.piece = vmax;
   p.pieces = idiv(p.vocab, p.piece);
   p.vp = p.piece + p.unit;
   p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
@@ -808,7 +874,6 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     at += align256(bytes);
     return here;
   };
-  const bool keep_any = p.keep_backward || p.keep_both;
   p.part = take((size_t)p.stats_tiles * n * sizeof(SoftStat));
   p.label_score = take(n * 4);
   p.xpack = take(n * p.hp * p.el);
@@ -817,7 +882,7 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.scores = take(p.keep_forward ? score_space : 0);
   p.total_forward = at;
   if (!p.keep_forward) p.scores = take(keep_any ? score_space : 0);
-  p.xt = take((size_t)p.width * p.np * p.el);
+  p.xl = take((p.el == 2 ? (size_t)p.width * p.np : n * p.hp) * p.el);
   p.wmax = take(4);
   p.g = take(n * p.vp * p.el);
   p.slabs = take((size_t)p.dx.splits * n * p.hp * 4);
@@ -882,11 +947,13 @@ template <class T>
 static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   hipStream_t st = ctx().stream;
   const int n = p.tokens;
-  const bool keep = c.forward && c.backward ? p.keep_both : c.forward ? p.keep_forward : p.keep_backward;
+  const int db = c.db ? 1 : 0;
+  const bool keep = c.forward && c.backward ? p.keep_both[db] : c.forward ? p.keep_forward : p.keep_backward[db];
   SoftStat *part = (SoftStat *)(c.ws + p.part);
   float *label_score = (float *)(c.ws + p.label_score), *scores = (float *)(c.ws + p.scores);
   float *slabs = (float *)(c.ws + p.slabs), *db_part = (float *)(c.ws + p.db);
-  T *g = (T *)(c.ws + p.g), *xt = (T *)(c.ws + p.xt);
+  T *g = (T *)(c.ws + p.g), *xl = (T *)(c.ws + p.xl);
+  constexpr bool kXt = !std::is_same<T, float>::value;  // x transposed for dw
   if (keep && p.el == 4) g = (T *)scores;  // fp32 G takes the scores' place
   const size_t packed = p.hp * p.el;
   const int chunk = p.unit / 8;  // elements of 16 bytes
@@ -903,10 +970,16 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   const float *wmax = nullptr;
   if (c.backward) {
     if (c.weight) wmax = (const float *)(c.ws + p.wmax);
-    const int tiles_t = idiv(n, 64), tiles = tiles_t * idiv(p.width, 64);
-    vocab_xt_kernel<T><<<tiles + (c.weight ? 1 : 0), 256, 0, st>>>(xt, (const T *)c.x, p.ldx, p.np, n, p.width, idiv(n, chunk) * chunk, tiles_t,
-                                                                  c.labels, c.ignore, c.weight,
-                                                                  (float *)(c.ws + p.wmax), tiles);
+    float *wm = (float *)(c.ws + p.wmax);
+    if constexpr (kXt) {
+      const int tiles_t = idiv(n, 64), tiles = tiles_t * idiv(p.width, 64);
+      vocab_xt_kernel<T><<<tiles + (c.weight ? 1 : 0), 256, 0, st>>>(xl, (const T *)c.x, p.ldx, p.np, n, p.width,
+                                                                    idiv(n, chunk) * chunk, tiles_t, c.labels, c.ignore,
+                                                                    c.weight, wm, tiles);
+    } else {
+      vocab_live_kernel<T><<<n + (c.weight ? 1 : 0), 256, 0, st>>>(xl, (const T *)c.x, p.ldx, n, p.width, p.hp, c.labels,
+                                                                  c.ignore, c.weight, wm);
+    }
     CCT_LAUNCH_CHECK();
   }
   // the piece's rows of w as an operand
@@ -948,9 +1021,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
                                           c.ignore, idiv(p.vocab, chunk) * chunk, c.db ? 1 : 0);
     CCT_LAUNCH_CHECK();
     if (c.db) {
-      vocab_colsum_kernel<<<dim3(idiv(p.vocab, 256), idiv(n, 64)), 256, 0, st>>>(db_part, scores, p.vp, n, p.vocab, p.vp);
-      CCT_LAUNCH_CHECK();
-      vocab_db_kernel<T><<<idiv(p.vocab, 256), 256, 0, st>>>((T *)c.db, db_part, wmax, p.vocab, p.vp, idiv(n, 64));
+      vocab_colsum_kernel<T><<<idiv(p.vocab, 64), 1024, 0, st>>>((T *)c.db, scores, p.vp, wmax, n, p.vocab);
       CCT_LAUNCH_CHECK();
     }
   } else if (c.forward) {
@@ -1011,8 +1082,9 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     }
     if (c.dw) {
       ProductArgs a{};
-      a.A = (const char *)xt;
-      a.lda = p.np * p.el;
+      a.A = (const char *)xl;
+      a.lda = kXt ? p.np * p.el : packed;
+      a.abytes = (uint32_t)packed;
       a.kbytes = (uint32_t)(idiv(n, chunk) * chunk * p.el);
       a.B = (const char *)g;
       a.ldb = p.vp * p.el;
@@ -1023,7 +1095,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
       a.wmax = wmax;
       a.C = (T *)c.dw + (size_t)v0 * p.ldw;
       a.ldc = p.ldw;
-      if (int rc = product<T, USE_OUT, true, false>(p.dw, a)) return rc;
+      if (int rc = product<T, USE_OUT, kXt, false>(p.dw, a)) return rc;
     }
   }
   if (c.dx) {
