@@ -138,12 +138,19 @@ __global__ __launch_bounds__(DST_THREADS) void distill_loss_kernel(float *__rest
                        top + (size_t)t * s.top_stride, s, t, lane);
 }
 
-// q of every entry into LDS, the weight of equal ids gathered at the first of them (-1 in `at` for the others and for
-// entries outside [begin, end)); returns whether the token has any weight at all.  All lanes of the workgroup call it.
+// A token's list in LDS, as the gradient needs it: for the first entry of every id in [begin, end), the id, its score and the
+// weight of all entries with that id; -1 as the id of every other entry.  Returns whether the token has any weight at
+// all.  All lanes of the workgroup call it.
+struct EntryLists {
+  int *id, *seen;  // `seen`: the ids before equal ones are merged
+  float *q, *sum, *z;
+};
+__device__ __forceinline__ EntryLists entry_lists(float *lds, int top) {
+  return EntryLists{(int *)lds, (int *)lds + top, lds + 2 * top, lds + 3 * top, lds + 4 * top};
+}
 template <class T>
-__device__ __forceinline__ bool gather_entries(int *at, float *q, float *z, const T *__restrict__ row,
-                                               const int *__restrict__ ids, const float *__restrict__ top, int begin,
-                                               int end, const DistillShape &s) {
+__device__ __forceinline__ bool gather_entries(const EntryLists &e, const T *row, const int *__restrict__ ids,
+                                               const float *__restrict__ top, int begin, int end, const DistillShape &s) {
   const int threads = blockDim.x, tid = threadIdx.x;
   // every wavefront computes the statistics by itself: the list is short, and no exchange is needed
   const Teacher te = teacher_stats(ids, top, s.top, s.vocab, s.scale2, tid & 63);
@@ -151,33 +158,32 @@ __device__ __forceinline__ bool gather_entries(int *at, float *q, float *z, cons
     const int id = ids[k];
     const float w = teacher_weight(te, id, top[k], s.scale2);
     const bool here = id >= begin && id < end && w != 0.0f;
-    at[k] = here ? id : -1;
-    q[k] = w;
-    z[k] = here ? (float)row[id] : 0.0f;
+    e.seen[k] = here ? id : -1;
+    e.q[k] = w;
+    e.z[k] = here ? (float)row[id] : 0.0f;
   }
   __syncthreads();
-  float total[DST_TOP_MAX / 64];
-  int n = 0;
-  for (int k = tid; k < s.top; k += threads, ++n) {
-    const int id = at[k];
+  for (int k = tid; k < s.top; k += threads) {
+    const int id = e.seen[k];
     float sum = 0.0f;
     bool first = id >= 0;
-    if (first)
-      for (int j = 0; j < s.top; ++j)
-        if (at[j] == id) {
-          first = first && j >= k;
-          sum += q[j];
-        }
-    total[n] = first ? sum : -1.0f;
-  }
-  __syncthreads();
-  n = 0;
-  for (int k = tid; k < s.top; k += threads, ++n) {
-    if (total[n] < 0.0f) at[k] = -1;
-    q[k] = total[n];
+    for (int j = 0; first && j < s.top; ++j)
+      if (e.seen[j] == id) {
+        first = j >= k;
+        sum += e.q[j];
+      }
+    e.id[k] = first ? id : -1;
+    e.sum[k] = sum;
   }
   __syncthreads();
   return te.m != neg_inf();
+}
+
+// The entries of a list on top of what the row's lanes wrote.
+template <class T>
+__device__ __forceinline__ void store_entries(T *dst, const EntryLists &e, float g, float lse, const DistillShape &s) {
+  for (int k = threadIdx.x; k < s.top; k += blockDim.x)
+    if (e.id[k] >= 0) dst[e.id[k]] = (T)(g * (probability(e.z[k], lse, s) - e.sum[k]));
 }
 
 // The gradient of one range of one token's scores.
@@ -189,14 +195,13 @@ __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, c
                                                                    const float *__restrict__ loss_grad, DistillShape s) {
   constexpr int V = Num<T>::V;
   extern __shared__ float lists[];
-  int *at = (int *)lists;
-  float *q = lists + s.top, *z = q + s.top;
+  const EntryLists e = entry_lists(lists, s.top);
   const int t = blockIdx.x / s.splits, cut = blockIdx.x % s.splits;
   const int begin = cut * s.chunk, end = min(s.vocab, begin + s.chunk);
   const T *row = logits + (size_t)t * s.logits_stride;
   T *dst = dlogits + (size_t)t * s.logits_stride;
-  const bool weight = gather_entries<T>(at, q, z, row, ids + (size_t)t * s.top_stride, top + (size_t)t * s.top_stride, begin,
-                                        end, s);
+  const bool weight =
+      gather_entries<T>(e, row, ids + (size_t)t * s.top_stride, top + (size_t)t * s.top_stride, begin, end, s);
   const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f), l = lse[t];
   for (int col = begin + threadIdx.x * V; col < end; col += DST_THREADS * V) {
     float f[V];
@@ -206,9 +211,89 @@ __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, c
     store_vec<T>(dst, f, col, end);
   }
   if (!weight) return;
-  __syncthreads();  // the entries of the list on top of what the row's lanes wrote
-  for (int k = threadIdx.x; k < s.top; k += DST_THREADS)
-    if (at[k] >= 0) dst[at[k]] = (T)(g * (probability(z[k], l, s) - q[k]));
+  __syncthreads();
+  store_entries<T>(dst, e, g, l, s);
+}
+
+// Loss and gradient of whole rows, each read once: a workgroup keeps its row in registers from the statistics to the
+// gradient, and fetches its next row into the registers that the gradient has left.  ITEMS vectors a lane.
+template <class T, int THREADS, int ITEMS>
+__global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict__ loss, float *__restrict__ lse, T *dlogits,
+                                                              const T *logits, const int *__restrict__ ids,
+                                                              const float *__restrict__ top,
+                                                              const float *__restrict__ loss_grad, DistillShape s) {
+  constexpr int V = Num<T>::V, WAVES = THREADS / 64;
+  typedef typename Num<T>::vec vec;
+  extern __shared__ float lists[];
+  __shared__ SoftStat sh[WAVES];
+  const EntryLists e = entry_lists(lists, s.top);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int whole = s.vocab / V * V;  // the vectors; what is left of the row is one element a lane
+  const int tail = whole + tid < s.vocab ? whole + tid : -1;
+  vec v[ITEMS];
+  T rest = (T)0.0f;
+  auto fetch = [&](int i, const T *row) {
+    const int col = (i * THREADS + tid) * V;
+    if (col < whole) v[i] = *reinterpret_cast<const vec *>(row + col);
+  };
+  const T *row = logits + (size_t)blockIdx.x * s.logits_stride;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) fetch(i, row);
+  if (tail >= 0) rest = row[tail];
+  for (int t = blockIdx.x; t < s.tokens; t += gridDim.x) {
+    row = logits + (size_t)t * s.logits_stride;
+    const int *list = ids + (size_t)t * s.top_stride;
+    const float *weights = top + (size_t)t * s.top_stride;
+    const bool some = gather_entries<T>(e, row, list, weights, 0, s.vocab, s);
+    // the row's maximum, then the sum under it
+    float m = tail >= 0 ? (float)rest : neg_inf();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if ((i * THREADS + tid) * V < whole)
+#pragma unroll
+        for (int k = 0; k < V; ++k) m = fmaxf(m, (float)v[i][k]);
+    const float base = m == neg_inf() ? 0.0f : m;
+    float sum = tail >= 0 ? exp2_fast(((float)rest - base) * s.scale2) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if ((i * THREADS + tid) * V < whole)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum += exp2_fast(((float)v[i][k] - base) * s.scale2);
+    SoftStat st = wave_join(SoftStat{m, sum}, s.scale2);
+    if (lane == 0) sh[wave] = st;
+    __syncthreads();
+    st = lane < WAVES ? sh[lane] : SoftStat{neg_inf(), 0.0f};
+#pragma unroll
+    for (int d = WAVES / 2; d > 0; d >>= 1) st = shfl_xor_join(st, d, s.scale2);
+    st.m = __shfl(st.m, 0, 64);
+    st.s = __shfl(st.s, 0, 64);
+    const float l = log_sum(st, s.inv_t);
+    // the loss before the gradient may overwrite its scores (dlogits == logits)
+    if (wave == 0) distill_loss_wave<T>(loss, lse, st, row, list, weights, s, t, lane);
+    __syncthreads();
+    const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f);
+    T *dst = dlogits + (size_t)t * s.logits_stride;
+    const int next = t + (int)gridDim.x;
+    const T *next_row = logits + (size_t)min(next, s.tokens - 1) * s.logits_stride;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int col = (i * THREADS + tid) * V;
+      if (col < whole) {
+        vec out;
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = (T)(some ? g * probability((float)v[i][k], l, s) : 0.0f);
+        __builtin_nontemporal_store(out, reinterpret_cast<vec *>(dst + col));
+      }
+      if (next < s.tokens) fetch(i, next_row);
+    }
+    if (tail >= 0) {
+      dst[tail] = (T)(some ? g * probability((float)rest, l, s) : 0.0f);
+      if (next < s.tokens) rest = next_row[tail];
+    }
+    __syncthreads();
+    if (some) store_entries<T>(dst, e, g, l, s);
+    __syncthreads();  // the lists are done with
+  }
 }
 
 static int check_distill(const cct_distill_loss_args *a, const char *who) {
@@ -271,11 +356,37 @@ static int distill_forward(float *loss, float *lse, const void *logits, const in
 template <class T>
 static int distill_backward(void *dlogits, const void *logits, const int *ids, const float *top, const float *lse,
                             const float *loss_grad, const DistillShape &s) {
-  distill_grad_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 3 * s.top * sizeof(float), ctx().stream>>>(
+  distill_grad_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 5 * s.top * sizeof(float), ctx().stream>>>(
       (T *)dlogits, (const T *)logits, ids, top, lse, loss_grad, s);
   CCT_LAUNCH_CHECK();
   note_kernel("distill_grad_kernel<%s> splits=%d", Num<T>::NAME, s.splits);
   return 0;
+}
+
+// Rows that one workgroup holds in its registers (16 vectors a lane at most), where there are enough of them to fill the
+// chip; few long rows are cut into ranges instead, and longer rows are read twice.
+template <class T>
+static int distill_both(float *loss, float *lse, void *dlogits, const void *logits, const int *ids, const float *top,
+                        const float *loss_grad, const DistillShape &s, void *ws) {
+  const int vecs = s.vocab / Num<T>::V;
+#define CCT_DISTILL_ROW(THREADS, ITEMS, GROUPS)                                                                            \
+  if (vecs <= THREADS * ITEMS) {                                                                                         \
+    const int grid = min(s.tokens, 256 * GROUPS);                                                                        \
+    distill_row_kernel<T, THREADS, ITEMS><<<grid, THREADS, 5 * s.top * sizeof(float), ctx().stream>>>(                     \
+        loss, lse, (T *)dlogits, (const T *)logits, ids, top, loss_grad, s);                                              \
+    CCT_LAUNCH_CHECK();                                                                                                   \
+    note_kernel("distill_row_kernel<%s, %d, %d> grid=%d", Num<T>::NAME, THREADS, ITEMS, grid);                             \
+    return 0;                                                                                                             \
+  }
+  if (s.tokens >= 128 || s.splits == 1) {
+    CCT_DISTILL_ROW(256, 4, 8)
+    CCT_DISTILL_ROW(512, 8, 2)
+    CCT_DISTILL_ROW(1024, 8, 1)
+    CCT_DISTILL_ROW(1024, 16, 1)
+  }
+#undef CCT_DISTILL_ROW
+  if (int rc = distill_forward<T>(loss, lse, logits, ids, top, s, ws)) return rc;
+  return distill_backward<T>(dlogits, logits, ids, top, lse, loss_grad, s);
 }
 
 static int check_distill_workspace(const cct_distill_loss_args *a, const void *ws, size_t bytes, const char *who) {
@@ -323,9 +434,14 @@ extern "C" int cct_hip_distill_loss_forward_backward(float *loss, float *lse, vo
                                                      const int *top_ids, const float *top_logits, const float *loss_grad,
                                                      const cct_distill_loss_args *args, void *workspace,
                                                      size_t workspace_bytes) {
-  CCT_REQUIRE(dlogits || !args || args->tokens == 0, "distill_loss_forward_backward: null array");
-  if (int rc = cct_hip_distill_loss_forward(loss, lse, logits, top_ids, top_logits, args, workspace, workspace_bytes))
-    return rc;
-  return cct_hip_distill_loss_backward(dlogits, logits, top_ids, top_logits, lse, loss_grad, args, workspace,
-                                       workspace_bytes);
+  const char *who = "distill_loss_forward_backward";
+  if (int rc = check_distill(args, who)) return rc;
+  if (args->tokens == 0) return 0;
+  CCT_REQUIRE(loss && lse && dlogits && logits && top_ids && top_logits, "%s: null array", who);
+  if (int rc = check_distill_workspace(args, workspace, workspace_bytes, who)) return rc;
+  CCT_ENSURE_INIT();
+  const DistillShape s = distill_shape(args);
+  return args->dtype == CCT_BF16
+             ? distill_both<bf16>(loss, lse, dlogits, logits, top_ids, top_logits, loss_grad, s, workspace)
+             : distill_both<float>(loss, lse, dlogits, logits, top_ids, top_logits, loss_grad, s, workspace);
 }

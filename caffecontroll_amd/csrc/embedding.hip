@@ -55,30 +55,53 @@ __device__ __forceinline__ uint32_t sort_key(int id, int padding, int vocab) {
   return id == padding || (unsigned)id >= (unsigned)vocab ? (uint32_t)vocab : (uint32_t)id;
 }
 
-// Few tokens: a token's place is the number of tokens that come before it, counted directly.  EMB_RANK_LANES lanes share
-// a token, the ids pass through LDS in blocks.  tokens^2 comparisons over the whole chip in one launch.
+// Few tokens: a token's place is the number of tokens that come before it, counted directly.  All keys lie in LDS; 16 lanes
+// share a token and take four keys at a time.  Of a workgroup's 16 tokens, those before the first of them come earlier
+// with an equal key too, those behind the last one do not, so but for one stretch of 16 every key costs one comparison.
+// tokens^2 comparisons over the whole chip in one launch: 5 us at 4096 tokens.
 constexpr int EMB_RANK_MAX = 8192;
 constexpr int EMB_RANK_LANES = 16;
-constexpr int EMB_RANK_BLOCK = 2048;
+constexpr int EMB_RANK_TOKENS = EMB_THREADS / EMB_RANK_LANES;
 __global__ __launch_bounds__(EMB_THREADS) void embedding_rank_kernel(uint32_t *__restrict__ keys, int *__restrict__ order,
                                                                      const int *__restrict__ ids, int tokens,
                                                                      int padding, int vocab) {
-  __shared__ uint32_t block[EMB_RANK_BLOCK];
-  const int lane = threadIdx.x % EMB_RANK_LANES;
-  const int t = blockIdx.x * (EMB_THREADS / EMB_RANK_LANES) + threadIdx.x / EMB_RANK_LANES;
-  const uint32_t key = t < tokens ? sort_key(ids[t], padding, vocab) : 0u;
-  int before = 0;
-  for (int base = 0; base < tokens; base += EMB_RANK_BLOCK) {
-    const int n = min(EMB_RANK_BLOCK, tokens - base);
-    __syncthreads();
-    for (int i = threadIdx.x; i < EMB_RANK_BLOCK; i += EMB_THREADS)
-      block[i] = i < n ? sort_key(ids[base + i], padding, vocab) : 0xFFFFFFFFu;
-    __syncthreads();
-    for (int i = lane; i < n; i += EMB_RANK_LANES) {
-      const uint32_t other = block[i];
-      before += (other < key || (other == key && base + i < t)) ? 1 : 0;
+  extern __shared__ __align__(16) uint32_t all[];
+  const int lane = threadIdx.x % EMB_RANK_LANES, t0 = blockIdx.x * EMB_RANK_TOKENS;
+  const int t = t0 + threadIdx.x / EMB_RANK_LANES;
+  const int pad = (tokens + 63) & ~63;
+  typedef int i4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#pragma unroll 4
+  for (int i = threadIdx.x * 4; i < pad; i += EMB_THREADS * 4) {
+    i4 v = {0, 0, 0, 0};
+    if (i + 4 <= tokens) {
+      v = *reinterpret_cast<const i4 *>(ids + i);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < tokens) v[k] = ids[i + k];
     }
+    u4 u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = i + k < tokens ? sort_key(v[k], padding, vocab) : 0xFFFFFFFFu;  // behind every key
+    *reinterpret_cast<u4 *>(all + i) = u;
   }
+  __syncthreads();
+  const uint32_t key = t < tokens ? all[t] : 0u;
+  int before = 0;
+  auto count = [&](int from, int to, uint32_t below) {
+#pragma unroll 4
+    for (int i = from + lane * 4; i < to; i += EMB_RANK_LANES * 4) {
+      const u4 k = *reinterpret_cast<const u4 *>(all + i);
+      before += (k[0] < below) + (k[1] < below) + (k[2] < below) + (k[3] < below);
+    }
+  };
+  count(0, t0, key + 1);                          // (t0 is a multiple of 16, vocab + 1 does not overflow)
+  if (t0 + lane < tokens) {
+    const uint32_t k = all[t0 + lane];
+    before += k < key || (k == key && t0 + lane < t);
+  }
+  count(t0 + EMB_RANK_TOKENS, pad, key);
 #pragma unroll
   for (int m = EMB_RANK_LANES / 2; m > 0; m >>= 1) before += __shfl_xor(before, m, 64);
   if (lane == 0 && t < tokens) {
@@ -87,11 +110,13 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_rank_kernel(uint32_t *_
   }
 }
 
-// Many tokens: least-significant-digit radix sort, 9 bits a pass.  One workgroup per tile of 4096 tokens counts its
+// Many tokens: least-significant-digit radix sort, 9 bits a pass.  One workgroup per tile of 1024 tokens counts its
 // digits; the second launch of a pass turns the tiles' counts into places (digits ascending, tiles ascending within a
-// digit) and moves the tile in order, so every pass is stable.
+// digit) and moves the tile in order, so every pass is stable.  Above EMB_TILES_MAX tiles a launch between them adds up the
+// tiles' counts once, instead of every workgroup for itself.
 constexpr int EMB_BITS = 9, EMB_BINS = 1 << EMB_BITS;
-constexpr int EMB_ITEMS = 16, EMB_TILE = EMB_THREADS * EMB_ITEMS;
+constexpr int EMB_ITEMS = 4, EMB_TILE = EMB_THREADS * EMB_ITEMS;
+constexpr uint32_t EMB_TILES_MAX = 128;
 constexpr int EMB_WAVES = EMB_THREADS / 64;
 
 // The token (and its key) at a place of a pass's input: the first pass reads the ids themselves.
@@ -115,6 +140,27 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_count_kernel(uint32_t *
   for (int i = threadIdx.x; i < EMB_BINS; i += EMB_THREADS) counts[(size_t)blockIdx.x * EMB_BINS + i] = bins[i];
 }
 
+// counts[tile] becomes the sum over the tiles before it, and a row behind the last tile holds all of them.
+__global__ __launch_bounds__(EMB_BINS) void embedding_scan_kernel(uint32_t *__restrict__ counts, uint32_t tiles) {
+  uint32_t sum = 0, tile = 0;
+  for (; tile + 8 <= tiles; tile += 8) {
+    uint32_t c[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = counts[(size_t)(tile + k) * EMB_BINS + threadIdx.x];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      counts[(size_t)(tile + k) * EMB_BINS + threadIdx.x] = sum;
+      sum += c[k];
+    }
+  }
+  for (; tile < tiles; ++tile) {
+    const uint32_t c = counts[(size_t)tile * EMB_BINS + threadIdx.x];
+    counts[(size_t)tile * EMB_BINS + threadIdx.x] = sum;
+    sum += c;
+  }
+  counts[(size_t)tiles * EMB_BINS + threadIdx.x] = sum;
+}
+
 __global__ __launch_bounds__(EMB_THREADS) void embedding_move_kernel(uint32_t *__restrict__ keys_out,
                                                                      int *__restrict__ order_out,
                                                                      const uint32_t *__restrict__ keys,
@@ -131,12 +177,21 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_move_kernel(uint32_t *_
   uint32_t all[PER], before[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) all[j] = before[j] = 0;
-  for (uint32_t tile = 0; tile < gridDim.x; ++tile) {
+  if (gridDim.x > EMB_TILES_MAX) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const uint32_t c = counts[(size_t)tile * EMB_BINS + tid * PER + j];
-      all[j] += c;
-      before[j] += tile < blockIdx.x ? c : 0u;
+      before[j] = counts[(size_t)blockIdx.x * EMB_BINS + tid * PER + j];
+      all[j] = counts[(size_t)gridDim.x * EMB_BINS + tid * PER + j];
+    }
+  } else {
+#pragma unroll 16
+    for (uint32_t tile = 0; tile < gridDim.x; ++tile) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const uint32_t c = counts[(size_t)tile * EMB_BINS + tid * PER + j];
+        all[j] += c;
+        before[j] += tile < blockIdx.x ? c : 0u;
+      }
     }
   }
   uint32_t mine = 0;
@@ -158,7 +213,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_move_kernel(uint32_t *_
   }
   for (int i = tid; i < EMB_WAVES * EMB_BINS; i += EMB_THREADS) (&seen[0][0])[i] = 0;
   __syncthreads();
-  // wavefront w takes the tile's tokens [w * 1024, ...) 64 at a time, in order: a token's rank within its wavefront's
+  // wavefront w takes the tile's tokens [w * 256, ...) 64 at a time, in order: a token's rank within its wavefront's
   // part is the count of its digit so far plus the lanes of the same digit below it
   uint32_t key[EMB_ITEMS], rank[EMB_ITEMS];
   const int first = blockIdx.x * EMB_TILE + wave * (EMB_ITEMS * 64) + lane;
@@ -217,26 +272,56 @@ __device__ __forceinline__ int lower_bound(const uint32_t *__restrict__ keys, in
   return lo;
 }
 
-// sum of dout[order[p]] over the places [p0, p1), columns [col, col + V)
-template <class T>
-__device__ __forceinline__ void sum_rows(float (&acc)[Num<T>::V], const T *__restrict__ dout,
-                                         const int *__restrict__ order, int p0, int p1, int col, const EmbShape &s) {
+// The same by a whole wavefront, 64 places at a time.
+__device__ __forceinline__ int wave_lower_bound(const uint32_t *__restrict__ keys, int n, uint32_t key, int lane) {
+  int lo = 0, len = n;
+  while (len > 0) {
+    const int step = (len + 63) >> 6;
+    const int at = lane * step;
+    const int below = __popcll(__ballot(at < len && keys[lo + min(at, len - 1)] < key));
+    if (below == 0) return lo;
+    const int skip = (below - 1) * step + 1;
+    len = min(step - 1, len - skip);
+    lo += skip;
+  }
+  return lo;
+}
+
+// Sums of dout[order[p]] over the places [p0, p1): TRIPS vectors of a row at columns col, col + stride, ...
+template <class T, int TRIPS>
+__device__ __forceinline__ void sum_rows(float (&acc)[TRIPS][Num<T>::V], const T *__restrict__ dout,
+                                         const int *__restrict__ order, int p0, int p1, int col, int stride,
+                                         const EmbShape &s) {
   constexpr int V = Num<T>::V;
+#pragma unroll
+  for (int k = 0; k < TRIPS; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[k][i] = 0.0f;
   int p = p0;
   for (; p + 4 <= p1; p += 4) {  // four rows in flight, added in order
-    float f[4][V];
+    float f[4][TRIPS][V];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load_vec<T>(f[j], dout + (size_t)order[p + j] * s.out_stride, col, s.width);
+    for (int j = 0; j < 4; ++j) {
+      const T *row = dout + (size_t)order[p + j] * s.out_stride;
+#pragma unroll
+      for (int k = 0; k < TRIPS; ++k) load_vec<T>(f[j][k], row, col + k * stride, s.width);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += f[j][i];
+      for (int k = 0; k < TRIPS; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[k][i] += f[j][k][i];
   }
   for (; p < p1; ++p) {
-    float f[V];
-    load_vec<T>(f, dout + (size_t)order[p] * s.out_stride, col, s.width);
+    const T *row = dout + (size_t)order[p] * s.out_stride;
+    float f[TRIPS][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += f[i];
+    for (int k = 0; k < TRIPS; ++k) load_vec<T>(f[k], row, col + k * stride, s.width);
+#pragma unroll
+    for (int k = 0; k < TRIPS; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[k][i] += f[k][i];
   }
 }
 
@@ -248,120 +333,147 @@ __device__ __forceinline__ void store_row(T *__restrict__ row, float (&acc)[Num<
   if (accumulate) load_vec<T>(old, row, col, s.width);
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = accumulate ? old[i] + acc[i] * s.scale : acc[i] * s.scale;
-  store_vec<T>(row, acc, col, s.width);
+  store_vec_stream<T>(row, acc, col, s.width);
 }
 
 // An id with more than EMB_RUN tokens is summed in pieces of EMB_RUN sorted places.  Piece j covers places
 // [j * EMB_RUN, (j + 1) * EMB_RUN) and can hold parts of two such ids: slot 0 the one that holds its first place, slot 1
 // one that begins inside.  Ids with fewer tokens are summed whole by the workgroup that owns their row.
-constexpr int EMB_RUN = 64;
-constexpr int EMB_ROWS = 8;  // rows of the table per workgroup and trip, at least
+constexpr int EMB_RUN = 16;
+constexpr int EMB_ROWS = 8;  // rows of the table per workgroup, at least
+constexpr int EMB_PLACES = EMB_ROWS * EMB_RUN;  // tokens of a workgroup's rows that it holds in LDS
+// what the joining launch needs to know of the long id that begins in a piece; first == last: there is none
+struct EmbRun {
+  int first, last;  // its places
+  int id;
+};
 
 template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(T *__restrict__ dtable, float *__restrict__ parts,
+                                                                    EmbRun *__restrict__ runs,
                                                                     const T *__restrict__ dout,
                                                                     const uint32_t *__restrict__ keys,
                                                                     const int *__restrict__ order, EmbShape s,
-                                                                    int accumulate, int log_lanes, int row_blocks) {
+                                                                    int accumulate, int log_lanes, int pieces) {
   constexpr int V = Num<T>::V;
   __shared__ int bounds[EMB_THREADS + 1];
+  __shared__ int window[2];
+  __shared__ int places[EMB_PLACES];
   const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes;
   const int groups = EMB_THREADS >> log_lanes;
-  if ((int)blockIdx.x < row_blocks) {
+  if ((int)blockIdx.x >= pieces) {
     const int rows = max(EMB_ROWS, groups);
-    const int v0 = blockIdx.x * rows, n = min(rows, s.vocab - v0);
-    for (int i = tid; i <= n; i += EMB_THREADS) bounds[i] = lower_bound(keys, s.tokens, (uint32_t)(v0 + i));
+    const int v0 = ((int)blockIdx.x - pieces) * rows, n = min(rows, s.vocab - v0);
+    if (tid < 128) {
+      const int at = wave_lower_bound(keys, s.tokens, (uint32_t)(v0 + (tid < 64 ? 0 : n)), tid & 63);
+      if ((tid & 63) == 0) window[tid >> 6] = at;
+    }
+    __syncthreads();
+    const int lo = window[0], len = window[1] - lo;
+    for (int i = tid; i < min(len, EMB_PLACES); i += EMB_THREADS) places[i] = order[lo + i];
+    for (int i = tid; i <= n; i += EMB_THREADS) bounds[i] = lo + lower_bound(keys + lo, len, (uint32_t)(v0 + i));
     __syncthreads();
     for (int r = group; r < n; r += groups) {
       const int p0 = bounds[r], p1 = bounds[r + 1];
       if (p1 - p0 > EMB_RUN || (accumulate && p1 == p0)) continue;
       T *row = dtable + (size_t)(v0 + r) * s.table_stride;
-      for (int col = lane * V; col < s.width; col += lanes * V) {
-        float acc[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-        sum_rows<T>(acc, dout, order, p0, p1, col, s);
-        store_row<T>(row, acc, col, s, accumulate);
+      // (a workgroup with a long id among its rows may have places beyond those in LDS)
+      const bool held = p1 - lo <= EMB_PLACES;
+      const int stride = lanes * V;
+      for (int col = lane * V; col < s.width; col += 2 * stride) {
+        float acc[2][V];
+        if (held)
+          sum_rows<T, 2>(acc, dout, places, p0 - lo, p1 - lo, col, stride, s);
+        else
+          sum_rows<T, 2>(acc, dout, order, p0, p1, col, stride, s);
+        store_row<T>(row, acc[0], col, s, accumulate);
+        store_row<T>(row, acc[1], col + stride, s, accumulate);
       }
     }
     return;
   }
-  const int piece = blockIdx.x - row_blocks;
-  if (tid < 2) {
-    const int a = piece * EMB_RUN, b = min(a + EMB_RUN, s.tokens);
-    const uint32_t key = keys[tid == 0 ? a : b - 1];
-    int p0 = lower_bound(keys, s.tokens, key), p1 = lower_bound(keys, s.tokens, key + 1);
-    const bool take = key < (uint32_t)s.vocab && p1 - p0 > EMB_RUN && (tid == 0 || p0 > a);
-    bounds[2 * tid] = take ? max(p0, a) : 0;
-    bounds[2 * tid + 1] = take ? min(p1, b) : 0;
-  }
+  const int piece = blockIdx.x, a = piece * EMB_RUN, b = min(a + EMB_RUN, s.tokens);
+  // wavefronts 0 and 1: the id at the piece's first place; 2 and 3: the one at its last
+  const uint32_t key = keys[tid < 128 ? a : b - 1];
+  const int at = wave_lower_bound(keys, s.tokens, key + ((tid >> 6) & 1), tid & 63);
+  if ((tid & 63) == 0) bounds[tid >> 6] = at;
   __syncthreads();
+  if (tid == 128) {
+    const bool begins = key < (uint32_t)s.vocab && bounds[3] - bounds[2] > EMB_RUN && bounds[2] >= a;
+    runs[piece] = begins ? EmbRun{bounds[2], bounds[3], (int)key} : EmbRun{0, 0, 0};
+  }
   for (int slot = 0; slot < 2; ++slot) {
-    const int p0 = bounds[2 * slot], p1 = bounds[2 * slot + 1];
-    if (p0 == p1) continue;
+    const int r0 = bounds[2 * slot], r1 = bounds[2 * slot + 1];
+    if (r1 - r0 <= EMB_RUN || keys[r0] >= (uint32_t)s.vocab || (slot == 1 && r0 <= a)) continue;
+    const int p0 = max(r0, a), p1 = min(r1, b);
     float *dst = parts + ((size_t)piece * 2 + slot) * s.width;
     for (int col = tid * V; col < s.width; col += EMB_THREADS * V) {
-      float acc[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-      sum_rows<T>(acc, dout, order, p0, p1, col, s);
+      float acc[1][V];
+      sum_rows<T, 1>(acc, dout, order, p0, p1, col, 0, s);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (col + i < s.width) dst[col + i] = acc[i];
+        if (col + i < s.width) dst[col + i] = acc[0][i];
     }
   }
 }
 
-// The pieces of a long id, added in order: the workgroup of the piece in which it begins, four columns groups of lanes
-// taking every fourth piece each.
+// The pieces of a long id, added in order: workgroups of the EMB_JOIN pieces among which it begins, 256 columns each, their
+// four wavefronts taking every fourth piece.  (One workgroup per piece and 256 columns are mostly workgroups that find
+// nothing: 36 us for 65536 tokens of width 4096.)
+constexpr int EMB_JOIN = 8;
 template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(T *__restrict__ dtable,
                                                                      const float *__restrict__ parts,
-                                                                     const uint32_t *__restrict__ keys, EmbShape s,
-                                                                     int accumulate) {
-  __shared__ int bounds[3];
-  __shared__ float sums[4][64];
-  const int tid = threadIdx.x, piece = blockIdx.x;
-  if (tid == 0) {
-    // an id that begins in this piece and has more than EMB_RUN tokens holds the piece's last place
-    const int last = piece * EMB_RUN + EMB_RUN - 1;
-    int p0 = 0, p1 = 0, key = 0;
-    if (last < s.tokens) {
-      key = (int)keys[last];
-      p0 = lower_bound(keys, s.tokens, (uint32_t)key);
-      p1 = lower_bound(keys, s.tokens, (uint32_t)key + 1);
-      if (key >= s.vocab || p1 - p0 <= EMB_RUN || p0 < piece * EMB_RUN) p0 = p1 = 0;
+                                                                     const EmbRun *__restrict__ runs, EmbShape s,
+                                                                     int accumulate, int pieces) {
+  __shared__ f32x4 sums[3][64];
+  const int tid = threadIdx.x, lane = tid & 63, group = tid >> 6;
+  const int first = blockIdx.x * EMB_JOIN, last = min(first + EMB_JOIN, pieces);
+  for (int piece = first; piece < last; ++piece) {
+    const EmbRun run = runs[piece];
+    if (run.first == run.last) continue;
+    const int end = (run.last - 1) / EMB_RUN;
+    for (int c0 = blockIdx.y * 256; c0 < s.width; c0 += gridDim.y * 256) {
+      const int col = c0 + lane * 4;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      auto add = [&](int j) {
+        float f[4];
+        load_vec<float>(f, parts + (size_t)(j * 2 + (j == piece && run.first != piece * EMB_RUN)) * s.width, col, s.width);
+        acc += f32x4{f[0], f[1], f[2], f[3]};
+      };
+      int j = piece + group;
+      if (j <= end) add(j);
+      j += 4;
+      if (col + 4 <= s.width)
+        for (; j + 28 <= end; j += 32) {  // eight loads in flight, added in order
+          Num<float>::vec v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            v[k] = *reinterpret_cast<const Num<float>::vec *>(parts + (size_t)(j + 4 * k) * 2 * s.width + col);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc += f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
+        }
+      for (; j <= end; j += 4) add(j);
+      __syncthreads();
+      if (group > 0) sums[group - 1][lane] = acc;
+      __syncthreads();
+      if (group == 0) {
+        acc = ((acc + sums[0][lane]) + sums[1][lane]) + sums[2][lane];
+        T *dst = dtable + (size_t)run.id * s.table_stride + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < s.width) dst[i] = (T)(accumulate ? (float)dst[i] + acc[i] * s.scale : acc[i] * s.scale);
+      }
     }
-    bounds[0] = p0;
-    bounds[1] = p1;
-    bounds[2] = key;
-  }
-  __syncthreads();
-  const int p0 = bounds[0], p1 = bounds[1];
-  if (p0 == p1) return;
-  const int end = (p1 - 1) / EMB_RUN;
-  const int lane = tid & 63, group = tid >> 6, col = blockIdx.y * 64 + lane;
-  const bool have = col < s.width;
-  float acc = 0.0f;
-  for (int j = piece + group; j <= end && have; j += 4) {
-    const int slot = j == piece && p0 != piece * EMB_RUN ? 1 : 0;
-    acc += parts[((size_t)j * 2 + slot) * s.width + col];
-  }
-  sums[group][lane] = acc;
-  __syncthreads();
-  if (group == 0 && have) {
-    acc = ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
-    T *dst = dtable + (size_t)bounds[2] * s.table_stride + col;
-    *dst = (T)(accumulate ? (float)*dst + acc * s.scale : acc * s.scale);
   }
 }
 
-// Lanes that share a row: as many as it has 16-byte vectors, up to a workgroup.
+// Lanes that share a row: as many as it has 16-byte vectors, up to 2^most.
 template <class T>
-static int row_lanes_log2(int width) {
+static int row_lanes_log2(int width, int most) {
   const int vecs = (width + Num<T>::V - 1) / Num<T>::V;
   int l = 0;
-  while ((1 << l) < vecs && l < 8) ++l;
+  while ((1 << l) < vecs && l < most) ++l;
   return l;
 }
 
@@ -388,7 +500,7 @@ static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // keys and order (twice: the radix passes alternate), the tiles' digit counts, the pieces' sums
 struct EmbWorkspace {
-  size_t keys[2], order[2], counts, parts, total;
+  size_t keys[2], order[2], counts, parts, runs, total;
 };
 static EmbWorkspace embedding_layout(const cct_embedding_args *a) {
   EmbWorkspace w;
@@ -404,15 +516,16 @@ static EmbWorkspace embedding_layout(const cct_embedding_args *a) {
     w.keys[i] = take(i == 0 || radix ? n * 4 : 0);
     w.order[i] = take(i == 0 || radix ? n * 4 : 0);
   }
-  w.counts = take(radix ? tiles * EMB_BINS * 4 : 0);
+  w.counts = take(radix ? (tiles + 1) * EMB_BINS * 4 : 0);
   w.parts = take(a->tokens > EMB_RUN ? (n + EMB_RUN - 1) / EMB_RUN * 2 * a->width * sizeof(float) : 0);
+  w.runs = take(a->tokens > EMB_RUN ? (n + EMB_RUN - 1) / EMB_RUN * sizeof(EmbRun) : 0);
   w.total = at;
   return w;
 }
 
 template <class T>
 static int embedding_forward(void *out, const void *table, const int *ids, const EmbShape &s) {
-  const int l = row_lanes_log2<T>(s.width);
+  const int l = row_lanes_log2<T>(s.width, 8);
   const int per = EMB_THREADS >> l;
   const unsigned blocks = (s.tokens + per - 1) / per;
   // one trip over a row per workgroup where few rows would leave the chip empty
@@ -429,8 +542,9 @@ static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const Em
   uint32_t *k[2] = {(uint32_t *)(ws + w.keys[0]), (uint32_t *)(ws + w.keys[1])};
   int *o[2] = {(int *)(ws + w.order[0]), (int *)(ws + w.order[1])};
   if (s.tokens <= EMB_RANK_MAX) {
-    const int per = EMB_THREADS / EMB_RANK_LANES;
-    embedding_rank_kernel<<<(s.tokens + per - 1) / per, EMB_THREADS, 0, st>>>(k[0], o[0], ids, s.tokens, s.padding, s.vocab);
+    const int blocks = (s.tokens + EMB_RANK_TOKENS - 1) / EMB_RANK_TOKENS;
+    const size_t lds = ((size_t)s.tokens + 63) / 64 * 64 * sizeof(uint32_t);
+    embedding_rank_kernel<<<blocks, EMB_THREADS, lds, st>>>(k[0], o[0], ids, s.tokens, s.padding, s.vocab);
     CCT_LAUNCH_CHECK();
     *keys = k[0];
     *order = o[0];
@@ -445,6 +559,10 @@ static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const Em
     const int *oin = from < 0 ? nullptr : o[from];
     embedding_count_kernel<<<tiles, EMB_THREADS, 0, st>>>(counts, kin, ids, s.tokens, s.padding, s.vocab, shift);
     CCT_LAUNCH_CHECK();
+    if (tiles > EMB_TILES_MAX) {
+      embedding_scan_kernel<<<1, EMB_BINS, 0, st>>>(counts, tiles);
+      CCT_LAUNCH_CHECK();
+    }
     embedding_move_kernel<<<tiles, EMB_THREADS, 0, st>>>(k[to], o[to], kin, oin, ids, counts, s.tokens, s.padding, s.vocab,
                                                          shift);
     CCT_LAUNCH_CHECK();
@@ -463,17 +581,20 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
   int *order = nullptr;
   if (s.tokens > 0)
     if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
-  const int l = row_lanes_log2<T>(s.width), rows = max(EMB_ROWS, EMB_THREADS >> l);
+  const int l = row_lanes_log2<T>(s.width, 8), rows = max(EMB_ROWS, EMB_THREADS >> l);
   const int row_blocks = (s.vocab + rows - 1) / rows;
   const int pieces = s.tokens > EMB_RUN ? (s.tokens + EMB_RUN - 1) / EMB_RUN : 0;
   float *parts = (float *)(ws + w.parts);
-  embedding_sum_kernel<T><<<row_blocks + pieces, EMB_THREADS, 0, st>>>((T *)dtable, parts, (const T *)dout, keys, order, s,
-                                                                      accumulate, l, row_blocks);
+  EmbRun *runs = (EmbRun *)(ws + w.runs);
+  // the pieces first: they take the longest
+  embedding_sum_kernel<T><<<pieces + row_blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
+                                                                      s, accumulate, l, pieces);
   CCT_LAUNCH_CHECK();
   note_kernel("embedding_sum_kernel<%s> rows per workgroup=%d pieces=%d", Num<T>::NAME, rows, pieces);
   if (pieces) {
-    embedding_join_kernel<T><<<dim3(pieces, (s.width + 63) / 64), EMB_THREADS, 0, st>>>((T *)dtable, parts, keys, s,
-                                                                                       accumulate);
+    const int cols = min((s.width + 255) / 256, 64);
+    embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, s,
+                                                                                                 accumulate, pieces);
     CCT_LAUNCH_CHECK();
   }
   return 0;

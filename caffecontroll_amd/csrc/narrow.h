@@ -59,6 +59,22 @@ __device__ __forceinline__ void store_vec(T *__restrict__ row, const float (&f)[
   }
 }
 
+// The same past the caches, for results that are large and not read again soon.
+template <class T>
+__device__ __forceinline__ void store_vec_stream(T *__restrict__ row, const float (&f)[Num<T>::V], int col, int width) {
+  constexpr int V = Num<T>::V;
+  if (col + V <= width) {
+    typename Num<T>::vec v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)f[i];
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Num<T>::vec *>(row + col));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (col + i < width) row[col + i] = (T)f[i];
+  }
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
