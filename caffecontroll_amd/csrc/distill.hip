@@ -77,6 +77,8 @@ __device__ __forceinline__ float probability(float score, float lse, const Disti
 struct Teacher {
   float m, s;   // maximum and sum over the valid entries
   bool bad;     // an entry names a row outside the vocabulary
+  // whether any entry has weight (one that is NaN has: the token's results are NaN then)
+  __device__ __forceinline__ bool some() const { return m != neg_inf() || s != 0.0f; }
 };
 __device__ __forceinline__ Teacher teacher_stats(const int *__restrict__ ids, const float *__restrict__ top, int n,
                                                  int vocab, float scale2, int lane) {
@@ -94,7 +96,7 @@ __device__ __forceinline__ Teacher teacher_stats(const int *__restrict__ ids, co
 
 // q of one entry; 0 where it has no weight
 __device__ __forceinline__ float teacher_weight(const Teacher &te, int id, float top, float scale2) {
-  if (id < 0 || te.m == neg_inf()) return 0.0f;
+  if (id < 0 || !te.some()) return 0.0f;
   return exp2_fast((top - te.m) * scale2) / te.s;
 }
 
@@ -176,7 +178,7 @@ __device__ __forceinline__ bool gather_entries(const EntryLists &e, const T *row
     e.sum[k] = sum;
   }
   __syncthreads();
-  return te.m != neg_inf();
+  return te.some();
 }
 
 // The entries of a list on top of what the row's lanes wrote.
@@ -216,7 +218,10 @@ __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, c
 }
 
 // Loss and gradient of whole rows, each read once: a workgroup keeps its row in registers from the statistics to the
-// gradient, and fetches its next row into the registers that the gradient has left.  ITEMS vectors a lane.
+// gradient, and fetches its next row into the registers that the gradient has left.  ITEMS vectors a lane; one entry of the
+// list a lane (top <= THREADS).  The statistics are taken vector by vector as they arrive, with a running maximum: the
+// exponentials (two per score, 16 us of a 128 K row's 26 us of traffic) then run beside the loads and stores, where a pass for the
+// maximum first had them wait for the whole row (4096 rows of 131072 bf16 scores: 585 us).
 template <class T, int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict__ loss, float *__restrict__ lse, T *dlogits,
                                                               const T *logits, const int *__restrict__ ids,
@@ -224,57 +229,104 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
                                                               const float *__restrict__ loss_grad, DistillShape s) {
   constexpr int V = Num<T>::V, WAVES = THREADS / 64;
   typedef typename Num<T>::vec vec;
-  extern __shared__ float lists[];
-  __shared__ SoftStat sh[WAVES];
-  const EntryLists e = entry_lists(lists, s.top);
+  __shared__ SoftStat sh_row[WAVES], sh_top[WAVES];
+  __shared__ float sh_loss[WAVES];
+  __shared__ int sh_id[THREADS];
+  __shared__ float sh_q[THREADS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int whole = s.vocab / V * V;  // the vectors; what is left of the row is one element a lane
   const int tail = whole + tid < s.vocab ? whole + tid : -1;
+  const bool entry = tid < s.top;
   vec v[ITEMS];
   T rest = (T)0.0f;
+  int id = -1;
+  float weight = 0.0f, z = 0.0f;
   auto fetch = [&](int i, const T *row) {
     const int col = (i * THREADS + tid) * V;
     if (col < whole) v[i] = *reinterpret_cast<const vec *>(row + col);
   };
-  const T *row = logits + (size_t)blockIdx.x * s.logits_stride;
+  {
+    const int t = blockIdx.x;
+    const T *row = logits + (size_t)t * s.logits_stride;
+    if (entry) {
+      id = ids[(size_t)t * s.top_stride + tid];
+      weight = top[(size_t)t * s.top_stride + tid];
+    }
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) fetch(i, row);
-  if (tail >= 0) rest = row[tail];
+    for (int i = 0; i < ITEMS; ++i) fetch(i, row);
+    if (tail >= 0) rest = row[tail];
+    if (id >= 0 && id < s.vocab) z = (float)row[id];
+  }
   for (int t = blockIdx.x; t < s.tokens; t += gridDim.x) {
-    row = logits + (size_t)t * s.logits_stride;
-    const int *list = ids + (size_t)t * s.top_stride;
-    const float *weights = top + (size_t)t * s.top_stride;
-    const bool some = gather_entries<T>(e, row, list, weights, 0, s.vocab, s);
-    // the row's maximum, then the sum under it
-    float m = tail >= 0 ? (float)rest : neg_inf();
+    const bool inside = id >= 0 && id < s.vocab;
+    // this lane's part of the row, and the teacher's weights
+    SoftStat st{neg_inf(), 0.0f};
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-      if ((i * THREADS + tid) * V < whole)
+      if ((i * THREADS + tid) * V < whole) {
+        float f[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) m = fmaxf(m, (float)v[i][k]);
-    const float base = m == neg_inf() ? 0.0f : m;
-    float sum = tail >= 0 ? exp2_fast(((float)rest - base) * s.scale2) : 0.0f;
+        for (int k = 0; k < V; ++k) f[k] = (float)v[i][k];
+        add_values<V>(st, f, s.scale2);
+      }
+    if (tail >= 0) {
+      const float f[1] = {(float)rest};
+      add_values<1>(st, f, s.scale2);
+    }
+    st = wave_join(st, s.scale2);
+    SoftStat te{id >= 0 ? weight : neg_inf(), 0.0f};
+    te.s = te.m == neg_inf() ? 0.0f : 1.0f + (weight - weight);  // NaN for a weight that is one, or infinite
+    te = wave_join(te, s.scale2);
+    if (lane == 0) {
+      sh_row[wave] = st;
+      sh_top[wave] = te;
+    }
+    const bool bad = __syncthreads_or(entry && id >= s.vocab);
+    st = lane < WAVES ? sh_row[lane] : SoftStat{neg_inf(), 0.0f};
+    te = lane < WAVES ? sh_top[lane] : SoftStat{neg_inf(), 0.0f};
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if ((i * THREADS + tid) * V < whole)
-#pragma unroll
-        for (int k = 0; k < V; ++k) sum += exp2_fast(((float)v[i][k] - base) * s.scale2);
-    SoftStat st = wave_join(SoftStat{m, sum}, s.scale2);
-    if (lane == 0) sh[wave] = st;
-    __syncthreads();
-    st = lane < WAVES ? sh[lane] : SoftStat{neg_inf(), 0.0f};
-#pragma unroll
-    for (int d = WAVES / 2; d > 0; d >>= 1) st = shfl_xor_join(st, d, s.scale2);
+    for (int d = WAVES / 2; d > 0; d >>= 1) {
+      st = shfl_xor_join(st, d, s.scale2);
+      te = shfl_xor_join(te, d, s.scale2);
+    }
     st.m = __shfl(st.m, 0, 64);
     st.s = __shfl(st.s, 0, 64);
+    te.m = __shfl(te.m, 0, 64);
+    te.s = __shfl(te.s, 0, 64);
     const float l = log_sum(st, s.inv_t);
-    // the loss before the gradient may overwrite its scores (dlogits == logits)
-    if (wave == 0) distill_loss_wave<T>(loss, lse, st, row, list, weights, s, t, lane);
+    const Teacher teacher{te.m, te.s, false};
+    const bool some = teacher.some();
+    // this lane's entry
+    const float q = teacher_weight(teacher, id, weight, s.scale2);
+    float term = 0.0f;
+    if (inside && q != 0.0f)
+      term = q * (((weight - te.m) * s.inv_t - __builtin_log2f(te.s) * kLn2) - __builtin_fmaf(z, s.inv_t, -l));
+    const bool mine = inside && q != 0.0f;
+    sh_id[tid] = mine ? id : -1;
+    sh_q[tid] = q;
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) term += __shfl_xor(term, m, 64);
+    if (lane == 0) sh_loss[wave] = term;
     __syncthreads();
+    // equal ids are one entry of the gradient: the first of them, with the weight of all
+    bool first = mine;
+    float sum = 0.0f;
+    for (int j = 0; first && j < s.top; ++j)
+      if (sh_id[j] == id) {
+        first = j >= tid;
+        sum += sh_q[j];
+      }
     const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f);
     T *dst = dlogits + (size_t)t * s.logits_stride;
+    const float entry_grad = g * (probability(z, l, s) - sum);
+    const int entry_id = id;
     const int next = t + (int)gridDim.x;
-    const T *next_row = logits + (size_t)min(next, s.tokens - 1) * s.logits_stride;
+    const bool more = next < s.tokens;
+    const T *next_row = logits + (size_t)(more ? next : t) * s.logits_stride;
+    if (entry && more) {
+      id = ids[(size_t)next * s.top_stride + tid];
+      weight = top[(size_t)next * s.top_stride + tid];
+    }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int col = (i * THREADS + tid) * V;
@@ -284,15 +336,22 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
         for (int k = 0; k < V; ++k) out[k] = (T)(some ? g * probability((float)v[i][k], l, s) : 0.0f);
         __builtin_nontemporal_store(out, reinterpret_cast<vec *>(dst + col));
       }
-      if (next < s.tokens) fetch(i, next_row);
+      if (more) fetch(i, next_row);
     }
     if (tail >= 0) {
       dst[tail] = (T)(some ? g * probability((float)rest, l, s) : 0.0f);
-      if (next < s.tokens) rest = next_row[tail];
+      if (more) rest = next_row[tail];
     }
-    __syncthreads();
-    if (some) store_entries<T>(dst, e, g, l, s);
-    __syncthreads();  // the lists are done with
+    if (more && id >= 0 && id < s.vocab) z = (float)next_row[id];
+    __syncthreads();  // the entry goes on top of what the row's lanes wrote
+    if (first && some) dst[entry_id] = (T)entry_grad;
+    if (tid == 0) {
+      float sum_loss = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) sum_loss += sh_loss[w];
+      lse[t] = l;
+      loss[t] = bad ? __builtin_nanf("") : s.temperature * s.temperature * sum_loss;
+    }
   }
 }
 
@@ -370,9 +429,9 @@ static int distill_both(float *loss, float *lse, void *dlogits, const void *logi
                         const float *loss_grad, const DistillShape &s, void *ws) {
   const int vecs = s.vocab / Num<T>::V;
 #define CCT_DISTILL_ROW(THREADS, ITEMS, GROUPS)                                                                            \
-  if (vecs <= THREADS * ITEMS) {                                                                                         \
+  if (vecs <= THREADS * ITEMS && s.top <= THREADS) {                                                                      \
     const int grid = min(s.tokens, 256 * GROUPS);                                                                        \
-    distill_row_kernel<T, THREADS, ITEMS><<<grid, THREADS, 5 * s.top * sizeof(float), ctx().stream>>>(                     \
+    distill_row_kernel<T, THREADS, ITEMS><<<grid, THREADS, 0, ctx().stream>>>(                     \
         loss, lse, (T *)dlogits, (const T *)logits, ids, top, loss_grad, s);                                              \
     CCT_LAUNCH_CHECK();                                                                                                   \
     note_kernel("distill_row_kernel<%s, %d, %d> grid=%d", Num<T>::NAME, THREADS, ITEMS, grid);                             \

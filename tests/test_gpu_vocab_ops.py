@@ -552,14 +552,15 @@ class Distill:
             self.lse = m + np.log(np.exp(z - m[:, None]).sum(1))
             tau = np.where(self.ids >= 0, self.tl.astype(np.float64) / T, -np.inf)
             tm = tau.max(1)
-            some = tm > -np.inf
+            tm = np.where(np.isnan(tau).any(1), np.nan, tm)
+            some = ~(tm == -np.inf)
             q = np.where(some[:, None], np.exp(tau - np.where(some, tm, 0)[:, None]), 0.0)
             qs = np.where(some, q.sum(1), 1.0)
             q /= qs[:, None]
             logq = tau - (tm + np.log(qs))[:, None]
             outside = self.ids >= self.vocab
             at = np.where((self.ids >= 0) & ~outside, self.ids, 0)
-            term = np.where(q > 0, q * (logq - z[rows, at] + self.lse[:, None]), 0.0)
+            term = np.where(~(q == 0), q * (logq - z[rows, at] + self.lse[:, None]), 0.0)
             self.loss = np.where(outside.any(1), np.nan, T * T * term.sum(1))
             p = np.exp(z - self.lse[:, None])
             big = np.where(np.isfinite(z), np.abs(z), 0).max(1)
@@ -572,7 +573,7 @@ class Distill:
             size = np.where(np.isfinite(size), size, 0.0)
             self.eloss = T * T * ((eq * size).sum(1) + q.sum(1) * eterm + (self.top / 64 + 8) * U * (q * size).sum(1)) + 1e-30
             g = p.copy()
-            ok = (q > 0) & ~outside
+            ok = ~(q == 0) & (self.ids >= 0) & ~outside
             for t in range(n):
                 np.subtract.at(g[t], at[t][ok[t]], q[t][ok[t]])
             g[~some] = 0.0
@@ -643,6 +644,7 @@ def test_distill_loss_lists_that_are_empty_masked_or_wrong(dtype, vocab):
     d.tl[6] = -3.4e38                                           # the type's lowest values, all alike
     d.tl[7, 3] = 500.0                                          # one entry far above the rest
     d.tl[0, 3] = np.nan                                         # in an absent entry
+    d.ids[11, 1:], d.ids[11, 0], d.tl[11, 0] = -1, 3, np.nan    # nothing but a NaN: so is the token's loss
     d.z[8, 10:200] = float("-inf")                              # a masked vocabulary, the list elsewhere
     d.ids[8] = 250
     d.z[9, :] = float("-inf")
@@ -652,7 +654,8 @@ def test_distill_loss_lists_that_are_empty_masked_or_wrong(dtype, vocab):
     d.ids[10, 0], d.tl[10, 0] = 100, 1.0                        # weight where the student has none: an infinite loss
     d.z64 = d.z.double().cpu().numpy()
     d.upload().reference()
-    assert d.loss[10] == np.inf and np.isnan(d.loss[3]) and (d.loss[:2] == 0).all()
+    assert d.loss[10] == np.inf and np.isnan(d.loss[[3, 11]]).all() and (d.loss[:2] == 0).all()
+    d.ed = np.where(np.isnan(d.ed), 0.0, d.ed)
     for both in (False, True):
         d.run(both)
         d.check()
