@@ -17,7 +17,11 @@ struct EmbShape {
   int tokens, width, vocab, padding;
   float scale;
   size_t table_stride, out_stride;
+  int stream;  // the result goes past the caches
 };
+// Results above this do not stay in the caches anyway (L2: 32 MB); written past them they leave them to the rows that are read
+// (65536 tokens of 2048 bf16: 77 instead of 92 us; the gradient of 131072 rows of 4096: 422 instead of 434 us).
+constexpr size_t EMB_STREAM_BYTES = (size_t)32 << 20;
 
 // ---- forward -----------------------------------------------------------------------------------------------------
 // A workgroup's lanes are laid over (row, 16-byte vector of the row); `cols` vectors of a row belong to one group of
@@ -45,7 +49,10 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_forward_kernel(T *__res
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] = fill;
     }
-    store_vec<T>(dst, f, col, s.width);
+    if (s.stream)
+      store_vec_stream<T>(dst, f, col, s.width);
+    else
+      store_vec<T>(dst, f, col, s.width);
   }
 }
 
@@ -333,7 +340,10 @@ __device__ __forceinline__ void store_row(T *__restrict__ row, float (&acc)[Num<
   if (accumulate) load_vec<T>(old, row, col, s.width);
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = accumulate ? old[i] + acc[i] * s.scale : acc[i] * s.scale;
-  store_vec_stream<T>(row, acc, col, s.width);
+  if (s.stream)
+    store_vec_stream<T>(row, acc, col, s.width);
+  else
+    store_vec<T>(row, acc, col, s.width);
 }
 
 // An id with more than EMB_RUN tokens is summed in pieces of EMB_RUN sorted places.  Piece j covers places
@@ -491,9 +501,11 @@ static int check_embedding(const cct_embedding_args *a, const char *who) {
   return 0;
 }
 
-static EmbShape shape_of(const cct_embedding_args *a) {
+static EmbShape shape_of(const cct_embedding_args *a, int result_rows) {
+  const bool stream = (size_t)result_rows * a->width * dtype_bytes(a->dtype) > EMB_STREAM_BYTES;
   return EmbShape{a->tokens, a->width, a->vocab, a->padding_id, a->scale,
-                  a->table_stride ? a->table_stride : (size_t)a->width, a->out_stride ? a->out_stride : (size_t)a->width};
+                  a->table_stride ? a->table_stride : (size_t)a->width, a->out_stride ? a->out_stride : (size_t)a->width,
+                  stream ? 1 : 0};
 }
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -609,7 +621,7 @@ extern "C" int cct_hip_embedding_forward(void *out, const void *table, const int
   if (args->tokens == 0) return 0;
   CCT_REQUIRE(out && table && ids, "embedding_forward: null array");
   CCT_ENSURE_INIT();
-  const EmbShape s = shape_of(args);
+  const EmbShape s = shape_of(args, args->tokens);
   return args->dtype == CCT_BF16 ? embedding_forward<bf16>(out, table, ids, s) : embedding_forward<float>(out, table, ids, s);
 }
 
@@ -627,7 +639,7 @@ extern "C" int cct_hip_embedding_backward(void *dtable, const void *dout, const 
               "embedding_backward: the workspace holds %zu bytes and starts at %p; it needs %zu, aligned to 16",
               workspace_bytes, workspace, w.total);
   CCT_ENSURE_INIT();
-  const EmbShape s = shape_of(args);
+  const EmbShape s = shape_of(args, args->vocab);
   char *ws = (char *)workspace;
   return args->dtype == CCT_BF16 ? embedding_backward<bf16>(dtable, dout, ids, s, accumulate, ws, w)
                                  : embedding_backward<float>(dtable, dout, ids, s, accumulate, ws, w);

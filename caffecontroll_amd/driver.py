@@ -16,9 +16,8 @@ __all__ = ["HIPDriver", "conv_pmap", "lift_args", "remap_pmap", "embedding_args"
 def _p(x):
     if x is None:
         return None
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
-    return int(x)
+    data_ptr = getattr(x, "data_ptr", None)
+    return int(x) if data_ptr is None else data_ptr()
 
 
 def conv_pmap(b, d, n, k, s, p):
