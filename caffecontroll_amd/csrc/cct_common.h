@@ -42,7 +42,7 @@ struct Tuning {
   int pool_plane = 0;     // 1: plane-tiled pooling kernels at any size
   int gemm_nt = 0;        // 1: non-temporal stores in the GEMM epilogue
   int gemm_tile = -1;     // index of the GEMM tile shape, -1 = model's choice
-  int vocab_tile = 0;     // vocabulary loss: tile of its products, 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 = 64 x 32, 0 = model's choice
+  int vocab_tile = 0;     // vocabulary loss: tile of its products, 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 / 5 = 64 x 32 with two / four stages, 0 = model's choice
   int vocab_keep = 0;     // vocabulary loss: 1 = scores kept where they fit the limit, 2 = never, 0 = model's choice
   int gemm_nodma = 0;     // 1: GEMM operand tiles always staged through registers
 };

@@ -41,17 +41,13 @@ __device__ __forceinline__ void add_values(SoftStat &st, const float (&z)[V], fl
   st.s = s;
 }
 
-// Maximum and sum of one range of one token's scores.
+// Maximum and sum of the scores [begin, end) of a row, by a workgroup; its first wavefront has the result.
 template <class T>
-__global__ __launch_bounds__(DST_THREADS) void distill_stats_kernel(SoftStat *__restrict__ part,
-                                                                    const T *__restrict__ logits, DistillShape s) {
+__device__ __forceinline__ SoftStat range_stats(const T *__restrict__ row, int begin, int end, const DistillShape &s) {
   constexpr int V = Num<T>::V;
   __shared__ SoftStat sh[DST_WAVES];
-  const int t = blockIdx.x / s.splits, cut = blockIdx.x % s.splits;
-  const T *row = logits + (size_t)t * s.logits_stride;
-  const int end = min(s.vocab, (cut + 1) * s.chunk);
   SoftStat st{neg_inf(), 0.0f};
-  for (int col = cut * s.chunk + threadIdx.x * V; col < end; col += DST_THREADS * V) {
+  for (int col = begin + threadIdx.x * V; col < end; col += DST_THREADS * V) {
     float z[V];
     load_vec<T>(z, row, col, s.vocab);
 #pragma unroll
@@ -61,11 +57,19 @@ __global__ __launch_bounds__(DST_THREADS) void distill_stats_kernel(SoftStat *__
   st = wave_join(st, s.scale2);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = st;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  st = sh[0];
 #pragma unroll
-    for (int w = 1; w < DST_WAVES; ++w) st = join(st, sh[w], s.scale2);
-    part[blockIdx.x] = st;
-  }
+  for (int w = 1; w < DST_WAVES; ++w) st = join(st, sh[w], s.scale2);
+  return st;
+}
+
+// One range of one token.
+template <class T>
+__global__ __launch_bounds__(DST_THREADS) void distill_stats_kernel(SoftStat *__restrict__ part,
+                                                                    const T *__restrict__ logits, DistillShape s) {
+  const int t = blockIdx.x / s.splits, cut = blockIdx.x % s.splits;
+  const SoftStat st = range_stats<T>(logits + (size_t)t * s.logits_stride, cut * s.chunk, min(s.vocab, (cut + 1) * s.chunk), s);
+  if (threadIdx.x == 0) part[blockIdx.x] = st;
 }
 
 // softmax(logits / T) of one score; the difference is formed before log2 e is applied
@@ -123,6 +127,20 @@ __device__ __forceinline__ void distill_loss_wave(float *__restrict__ loss, floa
     lse[t] = l;
     loss[t] = te.bad ? __builtin_nanf("") : s.temperature * s.temperature * sum;
   }
+}
+
+// Rows of a single range: statistics and loss in one launch, a workgroup per token.
+template <class T>
+__global__ __launch_bounds__(DST_THREADS) void distill_token_kernel(float *__restrict__ loss, float *__restrict__ lse,
+                                                                    const T *__restrict__ logits,
+                                                                    const int *__restrict__ ids,
+                                                                    const float *__restrict__ top, DistillShape s) {
+  const int t = blockIdx.x;
+  const T *row = logits + (size_t)t * s.logits_stride;
+  const SoftStat st = range_stats<T>(row, 0, s.vocab, s);
+  if (threadIdx.x < 64)
+    distill_loss_wave<T>(loss, lse, st, row, ids + (size_t)t * s.top_stride, top + (size_t)t * s.top_stride, s, t,
+                         threadIdx.x);
 }
 
 template <class T>
@@ -402,6 +420,12 @@ template <class T>
 static int distill_forward(float *loss, float *lse, const void *logits, const int *ids, const float *top,
                            const DistillShape &s, void *ws) {
   hipStream_t st = ctx().stream;
+  if (s.splits == 1) {
+    distill_token_kernel<T><<<s.tokens, DST_THREADS, 0, st>>>(loss, lse, (const T *)logits, ids, top, s);
+    CCT_LAUNCH_CHECK();
+    note_kernel("distill_token_kernel<%s>", Num<T>::NAME);
+    return 0;
+  }
   SoftStat *part = (SoftStat *)ws;
   distill_stats_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 0, st>>>(part, (const T *)logits, s);
   CCT_LAUNCH_CHECK();
@@ -422,8 +446,8 @@ static int distill_backward(void *dlogits, const void *logits, const int *ids, c
   return 0;
 }
 
-// Rows that one workgroup holds in its registers (16 vectors a lane at most), where there are enough of them to fill the
-// chip; few long rows are cut into ranges instead, and longer rows are read twice.
+// Rows that one workgroup holds in its registers (16 vectors a lane at most); longer rows are read twice.  One launch beats the
+// three of the split form for a single row too (a CU alone moves a row of 128 K bf16 scores in 6 us).
 template <class T>
 static int distill_both(float *loss, float *lse, void *dlogits, const void *logits, const int *ids, const float *top,
                         const float *loss_grad, const DistillShape &s, void *ws) {
@@ -437,12 +461,10 @@ static int distill_both(float *loss, float *lse, void *dlogits, const void *logi
     note_kernel("distill_row_kernel<%s, %d, %d> grid=%d", Num<T>::NAME, THREADS, ITEMS, grid);                             \
     return 0;                                                                                                             \
   }
-  if (s.tokens >= 128 || s.splits == 1) {
-    CCT_DISTILL_ROW(256, 4, 8)
-    CCT_DISTILL_ROW(512, 8, 2)
-    CCT_DISTILL_ROW(1024, 8, 1)
-    CCT_DISTILL_ROW(1024, 16, 1)
-  }
+  CCT_DISTILL_ROW(256, 4, 8)
+  CCT_DISTILL_ROW(512, 8, 2)
+  CCT_DISTILL_ROW(1024, 8, 1)
+  CCT_DISTILL_ROW(1024, 16, 1)
 #undef CCT_DISTILL_ROW
   if (int rc = distill_forward<T>(loss, lse, logits, ids, top, s, ws)) return rc;
   return distill_backward<T>(dlogits, logits, ids, top, lse, loss_grad, s);

@@ -478,6 +478,64 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(T *__restri
   }
 }
 
+// Few tokens: one launch without a sort.  Every workgroup reads all ids, keeps those of its rows with their tokens in order,
+// and adds each row's up.  (A row that has all of them is a chain of tokens / 4 loads: 32 at most.)
+constexpr int EMB_FEW = 128;
+template <class T>
+__global__ __launch_bounds__(EMB_THREADS) void embedding_few_kernel(T *__restrict__ dtable, const T *__restrict__ dout,
+                                                                    const int *__restrict__ ids, EmbShape s,
+                                                                    int accumulate, int log_lanes, int rows) {
+  constexpr int V = Num<T>::V;
+  __shared__ int token[EMB_FEW], row_of[EMB_FEW], held;
+  const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes;
+  const int groups = EMB_THREADS >> log_lanes;
+  const int v0 = blockIdx.x * rows, n = min(rows, s.vocab - v0);
+  if (tid < 64) {
+    int count = 0;
+    for (int base = 0; base < s.tokens; base += 64) {
+      const int t = base + tid;
+      const uint32_t key = t < s.tokens ? sort_key(ids[t], s.padding, s.vocab) : (uint32_t)s.vocab;
+      const bool here = key >= (uint32_t)v0 && key < (uint32_t)(v0 + n);
+      const uint64_t all = __ballot(here);
+      if (here) {
+        const int at = count + __popcll(all & ((1ull << tid) - 1ull));
+        token[at] = t;
+        row_of[at] = (int)key - v0;
+      }
+      count += __popcll(all);
+    }
+    if (tid == 0) held = count;
+  }
+  __syncthreads();
+  const int count = held;
+  for (int r = group; r < n; r += groups) {
+    int mine = 0;
+    for (int i = 0; i < count; ++i) mine += row_of[i] == r;
+    if (accumulate && mine == 0) continue;
+    T *row = dtable + (size_t)(v0 + r) * s.table_stride;
+    for (int col = lane * V; col < s.width; col += lanes * V) {
+      float acc[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+      int next = 0;
+      for (int left = mine; left > 0; left -= 4) {  // four rows in flight, added in order
+        float f[4][V];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j >= left) break;
+          while (row_of[next] != r) ++next;
+          load_vec<T>(f[j], dout + (size_t)token[next++] * s.out_stride, col, s.width);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] += j < left ? f[j][i] : 0.0f;
+      }
+      store_row<T>(row, acc, col, s, accumulate);
+    }
+  }
+}
+
 // Lanes that share a row: as many as it has 16-byte vectors, up to 2^most.
 template <class T>
 static int row_lanes_log2(int width, int most) {
@@ -516,7 +574,8 @@ struct EmbWorkspace {
 };
 static EmbWorkspace embedding_layout(const cct_embedding_args *a) {
   EmbWorkspace w;
-  const size_t n = a->tokens, tiles = (n + EMB_TILE - 1) / EMB_TILE;
+  // (none of it is used for EMB_FEW tokens or fewer)
+  const size_t n = a->tokens > EMB_FEW ? a->tokens : 0, tiles = (n + EMB_TILE - 1) / EMB_TILE;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -529,8 +588,8 @@ static EmbWorkspace embedding_layout(const cct_embedding_args *a) {
     w.order[i] = take(i == 0 || radix ? n * 4 : 0);
   }
   w.counts = take(radix ? (tiles + 1) * EMB_BINS * 4 : 0);
-  w.parts = take(a->tokens > EMB_RUN ? (n + EMB_RUN - 1) / EMB_RUN * 2 * a->width * sizeof(float) : 0);
-  w.runs = take(a->tokens > EMB_RUN ? (n + EMB_RUN - 1) / EMB_RUN * sizeof(EmbRun) : 0);
+  w.parts = take((n + EMB_RUN - 1) / EMB_RUN * 2 * a->width * sizeof(float));
+  w.runs = take((n + EMB_RUN - 1) / EMB_RUN * sizeof(EmbRun));
   w.total = at;
   return w;
 }
@@ -589,13 +648,18 @@ template <class T>
 static int embedding_backward(void *dtable, const void *dout, const int *ids, const EmbShape &s, int accumulate, char *ws,
                               const EmbWorkspace &w) {
   hipStream_t st = ctx().stream;
-  uint32_t *keys = nullptr;
-  int *order = nullptr;
-  if (s.tokens > 0)
-    if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
   const int l = row_lanes_log2<T>(s.width, 8), rows = max(EMB_ROWS, EMB_THREADS >> l);
   const int row_blocks = (s.vocab + rows - 1) / rows;
-  const int pieces = s.tokens > EMB_RUN ? (s.tokens + EMB_RUN - 1) / EMB_RUN : 0;
+  if (s.tokens <= EMB_FEW) {
+    embedding_few_kernel<T><<<row_blocks, EMB_THREADS, 0, st>>>((T *)dtable, (const T *)dout, ids, s, accumulate, l, rows);
+    CCT_LAUNCH_CHECK();
+    note_kernel("embedding_few_kernel<%s> rows per workgroup=%d", Num<T>::NAME, rows);
+    return 0;
+  }
+  uint32_t *keys = nullptr;
+  int *order = nullptr;
+  if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
+  const int pieces = (s.tokens + EMB_RUN - 1) / EMB_RUN;
   float *parts = (float *)(ws + w.parts);
   EmbRun *runs = (EmbRun *)(ws + w.runs);
   // the pieces first: they take the longest
@@ -603,7 +667,7 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
                                                                       s, accumulate, l, pieces);
   CCT_LAUNCH_CHECK();
   note_kernel("embedding_sum_kernel<%s> rows per workgroup=%d pieces=%d", Num<T>::NAME, rows, pieces);
-  if (pieces) {
+  {
     const int cols = min((s.width + 255) / 256, 64);
     embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, s,
                                                                                                  accumulate, pieces);

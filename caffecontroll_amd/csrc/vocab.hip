@@ -27,16 +27,17 @@
 namespace cct {
 
 // ---- the product kernel ----------------------------------------------------------------------------------------
-// A workgroup owns a BM x BN tile of C and walks k in steps of 64 bf16 or 32 fp32 elements through two LDS stages that
-// global -> LDS copies fill, 1 KB a wavefront at a time.
+// A workgroup owns a BM x BN tile of C and walks k in steps of 64 bf16 or 32 fp32 elements through two LDS stages (four for
+// the narrow tile, whose workgroups are often alone on a CU and wait for memory) that global -> LDS copies fill, 1 KB a
+// wavefront at a time.
 // Fragments of v_mfma_f32_16x16x32_bf16 and v_mfma_f32_16x16x4_f32: lane l holds 16 bytes of row l % 16, elements
 // along k of chunk l / 16; C element r of lane l is row 4 * (l / 16) + r, column l % 16.  For fp32 the four elements of a
 // chunk feed four MFMAs (the sum over k may run in any order as long as both operands use the same one).
 enum Use { USE_STATS = 0, USE_GRAD = 1, USE_SLAB = 2, USE_OUT = 3 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;  // 16 x 16 blocks of a wavefront
   static constexpr int STAGE = (BM + BN) * 128;               // bytes
@@ -60,7 +61,11 @@ __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, u
       "v"(lane_offset), "s"(rsrc), "s"(offset)
       : "memory");
 }
-__device__ __forceinline__ void copy_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// all but the last N copies of this wavefront have landed
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -277,22 +282,34 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 
   const int steps = (p.K + OpA::KS - 1) / OpA::KS;
   const int s0 = (int)split * p.steps_per_split, s1 = min(steps, s0 + p.steps_per_split);
+  // what lies past this workgroup's part of k counts as past the end: such copies fetch nothing and only keep the count
+  const int K = min(p.K, s1 * OpA::KS);
+  const uint32_t kbytes = min(p.kbytes, (uint32_t)s1 * 128u);
+  constexpr int COPIES = OpA::J + OpB::J;
+  auto copy = [&](int c, int buf, int step) {
+    lds_char *t = (lds_char *)lds + buf * S::STAGE;
+    if (c < OpA::J)
+      opa.copy(t, c, step, K, kbytes, wave);
+    else
+      opb.copy(t + S::BM * 128, c - OpA::J, step, K, kbytes, wave);
+  };
   auto stage = [&](int buf, int step) {
 #pragma unroll
-    for (int j = 0; j < OpA::J; ++j) opa.copy((lds_char *)lds + buf * S::STAGE, j, step, p.K, p.kbytes, wave);
-#pragma unroll
-    for (int j = 0; j < OpB::J; ++j) opb.copy((lds_char *)lds + buf * S::STAGE + S::BM * 128, j, step, p.K, p.kbytes, wave);
+    for (int c = 0; c < COPIES; ++c) copy(c, buf, step);
   };
   if constexpr (std::is_same<T, float>::value) {
     // fp32: a step's MFMAs take eight times as long as its reads; one barrier per step and the compiler's own order (with
     // the phases below: 4 to 6 % slower).  The four MFMAs of a chunk go round the blocks: neighbours in time do not wait for
     // one another's accumulator (1 % against four in a row).
-    if (s0 < s1) stage(0, s0);
+    if (s0 < s1) {
+#pragma unroll
+      for (int i = 0; i + 1 < S::STAGES; ++i) stage(i, s0 + i);
+    }
+    int buf = 0, fill = S::STAGES - 1;
     for (int s = s0; s < s1; ++s) {
-      copy_wait();
+      copy_wait<(S::STAGES - 2) * COPIES>();
       __syncthreads();
-      const int buf = (s - s0) & 1;
-      if (s + 1 < s1) stage(buf ^ 1, s + 1);
+      stage(fill, s + S::STAGES - 1);
       lds_char *ta = (lds_char *)lds + buf * S::STAGE, *tb = ta + S::BM * 128;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
@@ -309,12 +326,14 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
             for (int j = 0; j < NI; ++j)
               acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][e], b[j][e], acc[i][j], 0, 0, 0);
       }
+      fill = buf;
+      buf = buf + 1 == S::STAGES ? 0 : buf + 1;
     }
   } else {
     // A step is cut into phases of MH x NI blocks; while one phase's MFMAs run, the next one's fragments are read.  The last
-    // phase of a step reads the other stage, so the barrier stands before it: every wavefront then has all it needs of
-    // this stage in registers, and the copies of the step after next may overwrite it.  Reads and copies stand between
-    // the MFMAs in the order of the source, so that neither unit gets a burst that holds the other up.
+    // phase of a step reads the next stage, so the barrier stands before it: every wavefront then has all it needs of
+    // this stage in registers, and copies may overwrite it.  Reads and copies stand between the MFMAs in the order of the
+    // source, so that neither unit gets a burst that holds the other up.
     constexpr int MH = MI % 2 == 0 ? MI / 2 : MI, H = MI / MH, PHASES = 2 * H, MFMAS = MH * NI;
     f32x4 a[2][MH], b[2][NI];
     auto read = [&](int item, int to, int buf, int sub, int h) {  // items 0..MH-1: A, then B
@@ -325,48 +344,47 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
         b[sub][item - MH] = OpB::fragment(t + S::BM * 128, fb[item - MH], sub);
     };
     if (s0 < s1) {
-      stage(0, s0);
-      copy_wait();
+#pragma unroll
+      for (int i = 0; i < S::STAGES; ++i) stage(i, s0 + i);
+      copy_wait<(S::STAGES - 1) * COPIES>();
       __syncthreads();
-      if (s0 + 1 < s1) stage(1, s0 + 1);
 #pragma unroll
       for (int i = 0; i < MH + NI; ++i) read(i, 0, 0, 0, 0);
     }
+    int buf = 0;
     for (int s = s0; s < s1; ++s) {
-      const int buf = (s - s0) & 1;
+      const int next = buf + 1 == S::STAGES ? 0 : buf + 1;
 #pragma unroll
       for (int q = 0; q < PHASES; ++q) {
         const bool last = q + 1 == PHASES;
         const int sub = q / H, h = q % H, nsub = last ? 0 : (q + 1) / H, nh = last ? 0 : (q + 1) % H;
         if (last) {
-          copy_wait();
+          copy_wait<(S::STAGES - 2) * COPIES>();
           __syncthreads();
         }
-        const int reads = MH + (nh == 0 ? NI : 0), copies = last ? OpA::J + OpB::J : 0, items = reads + copies;
+        const int reads = MH + (nh == 0 ? NI : 0), copies = last ? COPIES : 0, items = reads + copies;
 #pragma unroll
         for (int m = 0; m < MFMAS; ++m) {
 #pragma unroll
           for (int it = 0; it < items; ++it) {
             if (it * MFMAS / items != m) continue;
-            // the last phase alternates between copies and reads
+            // the last phase alternates between copies and reads (what is read behind the last step is not used)
             const int c = last ? (it < 2 * min(copies, reads) ? ((it & 1) ? -1 : it / 2) : (copies > reads ? it - reads : -1)) : -1;
             const int r = last ? (it < 2 * min(copies, reads) ? it / 2 : it - copies) : it;
-            // past the end both are harmless: the copies fetch nothing, and what is read is not used
-            if (c >= 0 && c < OpA::J)
-              opa.copy((lds_char *)lds + buf * S::STAGE, c, s + 2, p.K, p.kbytes, wave);
-            else if (c >= 0)
-              opb.copy((lds_char *)lds + buf * S::STAGE + S::BM * 128, c - OpA::J, s + 2, p.K, p.kbytes, wave);
+            if (c >= 0)
+              copy(c, buf, s + S::STAGES);
             else
-              read(r, (q + 1) & 1, last ? buf ^ 1 : buf, nsub, nh);
+              read(r, (q + 1) & 1, last ? next : buf, nsub, nh);
           }
           const int i = m / NI, j = m % NI;
           acc[h * MH + i][j] = mfma_bf16(a[q & 1][i], b[sub][j], acc[h * MH + i][j]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      buf = next;
     }
-    copy_wait();  // no copy may land after this workgroup's use of its LDS
   }
+  copy_wait<0>();  // no copy may land after this workgroup's use of its LDS
 
   // this lane's elements: rows mrow + 16 i + r, columns ncol + 16 j
   const int fgroup = lane >> 4, frow = lane & 15;
@@ -500,16 +518,24 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 
 // ---- copies and statistics before the products ---------------------------------------------------------------------
 // dst[r][c] = src[r][c], rows of dst filled up to cpad with zeros: operands whose rows do not start at 16-byte
-// boundaries or are no whole number of 16-byte chunks.
+// boundaries or are no whole number of 16-byte chunks.  Rows [0, rows) of one matrix, then those of another; the lanes of
+// a workgroup are laid over (row, vector).
 template <class T>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, const T *__restrict__ src, size_t ld_src,
-                                                         int cols, int cpad) {
+                                                         int rows, T *__restrict__ dst2, const T *__restrict__ src2,
+                                                         size_t ld_src2, int rows2, int cols, int cpad, int log_lanes) {
   constexpr int V = Num<T>::V;
-  const size_t r = blockIdx.x;
-  for (int c = threadIdx.x * V; c < cpad; c += 256 * V) {
+  const int lanes = 1 << log_lanes;
+  int r = blockIdx.x * (256 >> log_lanes) + (threadIdx.x >> log_lanes);
+  if (r >= rows + rows2) return;
+  const bool second = r >= rows;
+  if (second) r -= rows;
+  const T *from = second ? src2 + (size_t)r * ld_src2 : src + (size_t)r * ld_src;
+  T *to = (second ? dst2 : dst) + (size_t)r * cpad;
+  for (int c = (threadIdx.x & (lanes - 1)) * V; c < cpad; c += lanes * V) {
     float f[V];
-    load_vec<T>(f, src + r * ld_src, c, cols);
-    store_vec<T>(dst + r * cpad, f, c, cpad);
+    load_vec<T>(f, from, c, cols);
+    store_vec<T>(to, f, c, cpad);
   }
 }
 
@@ -742,11 +768,12 @@ __global__ __launch_bounds__(256) void vocab_zero_kernel(T *__restrict__ p, size
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
-typedef Shape<256, 256, 2, 4> ShapeL;
-typedef Shape<256, 256, 4, 2> ShapeLA;  // the same tile with fewer fragments of A per wavefront: A contiguous along its rows
-typedef Shape<128, 128, 2, 2> ShapeM;
-typedef Shape<64, 64, 2, 2> ShapeN;
-typedef Shape<64, 32, 4, 1> ShapeS;
+typedef Shape<256, 256, 2, 4, 2> ShapeL;
+typedef Shape<256, 256, 4, 2, 2> ShapeLA;  // the same tile with fewer fragments of A per wavefront: A contiguous along its rows
+typedef Shape<128, 128, 2, 2, 2> ShapeM;
+typedef Shape<64, 64, 2, 2, 2> ShapeN;
+typedef Shape<64, 32, 4, 1, 2> ShapeS;
+typedef Shape<64, 32, 4, 1, 4> ShapeD;  // few workgroups: deeper prefetch instead of more of them on a CU
 
 static int idiv(int a, int b) { return (a + b - 1) / b; }
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -759,12 +786,13 @@ struct TileCost {
   int bm, bn, occ;
   double alone[2], full[2], finish;  // fp32, bf16
 };
-enum ShapeId { SHAPE_L, SHAPE_M, SHAPE_N, SHAPE_S, SHAPES };
+enum ShapeId { SHAPE_L, SHAPE_M, SHAPE_N, SHAPE_S, SHAPE_D, SHAPES };
 static const TileCost kTiles[SHAPES] = {
     {ShapeL::BM, ShapeL::BN, 1, {7.35, 1.28}, {7.50, 1.62}, 10.0},
-    {ShapeM::BM, ShapeM::BN, 2, {2.06, 0.72}, {3.88, 1.05}, 6.0},
-    {ShapeN::BM, ShapeN::BN, 4, {0.65, 0.50}, {1.97, 0.67}, 3.0},
-    {ShapeS::BM, ShapeS::BN, 6, {0.46, 0.50}, {1.50, 0.71}, 2.0},
+    {ShapeM::BM, ShapeM::BN, 2, {2.06, 0.70}, {3.88, 1.05}, 6.0},
+    {ShapeN::BM, ShapeN::BN, 4, {0.60, 0.44}, {1.97, 0.67}, 3.0},
+    {ShapeS::BM, ShapeS::BN, 6, {0.42, 0.42}, {1.50, 0.71}, 2.0},
+    {ShapeD::BM, ShapeD::BN, 3, {0.36, 0.20}, {0.85, 0.41}, 2.0},
 };
 constexpr double kLaunchUs = 3.0, kBytesPerUs = 5.0e6;  // what a launch costs, and a pass over memory
 
@@ -779,8 +807,8 @@ static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow
   const int pinned = tuning().vocab_tile >= 1 && tuning().vocab_tile <= SHAPES ? tuning().vocab_tile : 0;
   Choice best{SHAPE_M, 1, 1e30};
   for (int s = 0; s < SHAPES; ++s) {
-    if (s == SHAPE_S && !narrow) continue;
-    if (pinned && s != (pinned == SHAPES && !narrow ? SHAPE_N : pinned - 1)) continue;
+    if (s >= SHAPE_S && !narrow) continue;
+    if (pinned && s != (pinned > SHAPE_S && !narrow ? (int)SHAPE_N : pinned - 1)) continue;
     const TileCost &c = kTiles[s];
     const double tiles = (double)idiv(M, c.bm) * idiv(N > 0 ? N : 1, c.bn);
     for (int splits = 1; splits <= 64; splits *= 2) {
@@ -895,7 +923,7 @@ template <class T, class S, int USE, bool KA, bool KB>
 static int launch_product(ProductArgs &p) {
   auto kern = vocab_product_kernel<T, S, USE, KA, KB>;
   static LdsGrant grant;
-  const size_t bytes = 2 * S::STAGE;
+  const size_t bytes = S::STAGES * S::STAGE;
   if (int rc = grant_dynamic_lds((const void *)kern, bytes, grant)) return rc;
   p.tiles_m = idiv(p.M, S::BM);
   p.tiles_n = idiv(p.N, S::BN);
@@ -906,8 +934,8 @@ static int launch_product(ProductArgs &p) {
   p.blocks = (uint32_t)blocks;
   kern<<<p.blocks, S::THREADS, bytes, ctx().stream>>>(p);
   CCT_LAUNCH_CHECK();
-  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d>, %d, %s, %s> splits=%d", Num<T>::NAME, S::BM, S::BN, S::WM,
-              S::WN, USE, KA ? "true" : "false", KB ? "true" : "false", p.splits);
+  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d, %d>, %d, %s, %s> splits=%d", Num<T>::NAME, S::BM, S::BN, S::WM,
+              S::WN, S::STAGES, USE, KA ? "true" : "false", KB ? "true" : "false", p.splits);
   return 0;
 }
 
@@ -920,7 +948,10 @@ static int product(const Choice &c, ProductArgs &p) {
     case SHAPE_N: return launch_product<T, ShapeN, USE, KA, KB>(p);
     default:
       // an operand that is contiguous along its rows needs 64 of them
-      if constexpr (KB) return launch_product<T, ShapeS, USE, KA, KB>(p);
+      if constexpr (KB) {
+        if (c.shape == SHAPE_S) return launch_product<T, ShapeS, USE, KA, KB>(p);
+        return launch_product<T, ShapeD, USE, KA, KB>(p);
+      }
       return launch_product<T, ShapeN, USE, KA, KB>(p);
   }
 }
@@ -958,15 +989,9 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   const size_t packed = p.hp * p.el;
   const int chunk = p.unit / 8;  // elements of 16 bytes
   const bool direct_x = direct_rows(c.x, p.ldx, p.width, p.el), direct_w = direct_rows(c.w, p.ldw, p.width, p.el);
-  const char *x = (const char *)c.x;
-  size_t ldx = p.ldx * p.el;
-  if (!direct_x) {
-    T *xp = (T *)(c.ws + p.xpack);
-    vocab_pack_kernel<T><<<n, 256, 0, st>>>(xp, (const T *)c.x, p.ldx, p.width, p.hp);
-    CCT_LAUNCH_CHECK();
-    x = (const char *)xp;
-    ldx = packed;
-  }
+  const char *x = (const char *)(direct_x ? c.x : c.ws + p.xpack);
+  const size_t ldx = direct_x ? p.ldx * p.el : packed;
+  bool x_packed = direct_x;
   const float *wmax = nullptr;
   if (c.backward) {
     if (c.weight) wmax = (const float *)(c.ws + p.wmax);
@@ -982,15 +1007,20 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     }
     CCT_LAUNCH_CHECK();
   }
-  // the piece's rows of w as an operand
+  // the piece's rows of w as an operand; the first call sees to x too
   const size_t ldw = direct_w ? p.ldw * p.el : packed;
   auto rows_of_w = [&](int v0, int rows, const char **out) -> int {
-    *out = (const char *)c.w + (size_t)v0 * p.ldw * p.el;
-    if (direct_w) return 0;
+    const T *src = (const T *)c.w + (size_t)v0 * p.ldw;
     T *wp = (T *)(c.ws + p.wpack);
-    vocab_pack_kernel<T><<<rows, 256, 0, st>>>(wp, (const T *)*out, p.ldw, p.width, p.hp);
+    *out = (const char *)(direct_w ? src : wp);
+    const int xrows = x_packed ? 0 : n, wrows = direct_w ? 0 : rows;
+    x_packed = true;
+    if (xrows + wrows == 0) return 0;
+    int l = 0;
+    while (l < 8 && (1 << l) * Num<T>::V < p.hp) ++l;
+    vocab_pack_kernel<T><<<idiv(xrows + wrows, 256 >> l), 256, 0, st>>>((T *)(c.ws + p.xpack), (const T *)c.x, p.ldx, xrows, wp,
+                                                                       src, p.ldw, wrows, p.width, p.hp, l);
     CCT_LAUNCH_CHECK();
-    *out = (const char *)wp;
     return 0;
   };
   auto score_args = [&](const char *w, int v0, int rows) {

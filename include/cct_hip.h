@@ -110,7 +110,7 @@ int cct_hip_set_stream(void *hip_stream);
  * x 1000 + column blocks x 100 + column groups x 10 + row blocks, 0 = automatic), "pool_plane", "gemm_nt", "gemm_tile" (-1 = automatic), "gemm_nodma" (1 = GEMM
  * operand tiles always staged through registers), "conv1x1_per_image" (1 x 1 layers, forward and data gradient: 1 = one
  * product per image, 2 = one product over the pixels of all images, 0 = automatic), "vocab_tile" (tile of the
- * vocabulary loss's products: 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 = 64 x 32, 0 = automatic), "vocab_keep"
+ * vocabulary loss's products: 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 / 5 = 64 x 32 with two / four stages, 0 = automatic), "vocab_keep"
  * (1 = its scores are kept where they fit the limit, 2 = never, 0 = automatic; both also change what its workspace must hold).  The
  * environment variables CCT_HIP_<NAME IN CAPITALS> give the initial values; they are read once,
  * when the library initialises, never on a launch path.  No counterpart in the reference. */

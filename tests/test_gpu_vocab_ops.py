@@ -110,7 +110,7 @@ def test_embedding_forward(dtype, tokens, width, vocab, gap):
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("tokens, width, vocab, kind", [
-    (1, 5, 3, "uniform"), (64, 8, 4, "one"), (65, 8, 4, "one"), (129, 33, 9, "one"), (200, 64, 1000, "uniform"),
+    (1, 5, 3, "uniform"), (64, 8, 4, "one"), (128, 1030, 40, "skewed"), (127, 6, 1000, "uniform"), (128, 2060, 7, "one"), (65, 8, 4, "one"), (129, 33, 9, "one"), (200, 64, 1000, "uniform"),
     (640, 12, 3, "uniform"), (1000, 130, 50, "skewed"), (4099, 40, 10007, "skewed"), (8192, 4, 513, "uniform"),
     (8193, 20, 600, "skewed"), (20000, 9, 300000, "uniform"), (30000, 16, 511, "skewed"), (12345, 8, 512, "one"),
     (9000, 3, 40, "padding")])
@@ -325,7 +325,7 @@ def test_vocab_loss_with_the_largest_tiles(dtype, tokens, width, vocab, piece):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
-@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("keep", [1, 2])
 @pytest.mark.parametrize("tokens, width, vocab", [(3, 8, 5), (100, 264, 700), (333, 77, 515), (70, 1048, 1030)])
 def test_vocab_loss_every_tile_with_scores_kept_or_not(dtype, tile, keep, tokens, width, vocab):
