@@ -185,6 +185,57 @@ class HIPDriver {
        "softmax_loss_backward");
   }
 
+  // ---- the vocabulary ends of a model (no counterpart in DeviceDriver.h; include/cct_hip.h says what each computes) ----
+  // Matrices are fp32 or bf16 (args.dtype); workspaces are the caller's, `bytes` long.
+  void embedding_forward(void *out, const void *table, const int *ids, const cct_embedding_args &args) {
+    ok(cct_hip_embedding_forward(out, table, ids, &args), "embedding_forward");
+  }
+  size_t embedding_workspace_bytes(const cct_embedding_args &args) { return cct_hip_embedding_workspace_bytes(&args); }
+  void embedding_backward(void *dtable, const void *dout, const int *ids, const cct_embedding_args &args, bool accumulate,
+                          void *workspace, size_t bytes) {
+    ok(cct_hip_embedding_backward(dtable, dout, ids, &args, accumulate, workspace, bytes), "embedding_backward");
+  }
+  size_t vocab_loss_workspace_bytes(const cct_vocab_loss_args &args, bool training) {
+    return cct_hip_vocab_loss_workspace_bytes(&args, training);
+  }
+  void vocab_loss_forward(float *loss, float *lse, const void *x, const void *w, const void *bias, const int *labels,
+                          const cct_vocab_loss_args &args, void *workspace, size_t bytes) {
+    ok(cct_hip_vocab_loss_forward(loss, lse, x, w, bias, labels, &args, workspace, bytes), "vocab_loss_forward");
+  }
+  void vocab_loss_backward(void *dx, void *dw, void *db, const void *x, const void *w, const void *bias, const int *labels,
+                           const float *lse, const float *loss_grad, const cct_vocab_loss_args &args, void *workspace,
+                           size_t bytes) {
+    ok(cct_hip_vocab_loss_backward(dx, dw, db, x, w, bias, labels, lse, loss_grad, &args, workspace, bytes),
+       "vocab_loss_backward");
+  }
+  void vocab_loss_forward_backward(float *loss, float *lse, void *dx, void *dw, void *db, const void *x, const void *w,
+                                   const void *bias, const int *labels, const float *loss_grad,
+                                   const cct_vocab_loss_args &args, void *workspace, size_t bytes) {
+    ok(cct_hip_vocab_loss_forward_backward(loss, lse, dx, dw, db, x, w, bias, labels, loss_grad, &args, workspace, bytes),
+       "vocab_loss_forward_backward");
+  }
+  size_t distill_loss_workspace_bytes(const cct_distill_loss_args &args) {
+    return cct_hip_distill_loss_workspace_bytes(&args);
+  }
+  void distill_loss_forward(float *loss, float *lse, const void *logits, const int *top_ids, const float *top_logits,
+                            const cct_distill_loss_args &args, void *workspace, size_t bytes) {
+    ok(cct_hip_distill_loss_forward(loss, lse, logits, top_ids, top_logits, &args, workspace, bytes),
+       "distill_loss_forward");
+  }
+  void distill_loss_backward(void *dlogits, const void *logits, const int *top_ids, const float *top_logits,
+                             const float *lse, const float *loss_grad, const cct_distill_loss_args &args, void *workspace,
+                             size_t bytes) {
+    ok(cct_hip_distill_loss_backward(dlogits, logits, top_ids, top_logits, lse, loss_grad, &args, workspace, bytes),
+       "distill_loss_backward");
+  }
+  void distill_loss_forward_backward(float *loss, float *lse, void *dlogits, const void *logits, const int *top_ids,
+                                     const float *top_logits, const float *loss_grad, const cct_distill_loss_args &args,
+                                     void *workspace, size_t bytes) {
+    ok(cct_hip_distill_loss_forward_backward(loss, lse, dlogits, logits, top_ids, top_logits, loss_grad, &args, workspace,
+                                             bytes),
+       "distill_loss_forward_backward");
+  }
+
   // ---- single precision BLAS-shaped members (DeviceDriver.h:197-215) ----
   void math_saxpy(const float alpha, DeviceMemoryPointer *X, DeviceMemoryPointer *Y) const {
     ok(cct_hip_math_saxpy(X->size_in_byte / sizeof(float), alpha, (const float *)X->ptr, (float *)Y->ptr),
