@@ -69,10 +69,40 @@ __device__ __forceinline__ uint32_t sort_key(int id, int padding, int vocab) {
 constexpr int EMB_RANK_MAX = 8192;
 constexpr int EMB_RANK_LANES = 16;
 constexpr int EMB_RANK_TOKENS = EMB_THREADS / EMB_RANK_LANES;
+// Workgroups behind those that rank clear the table, `rows` rows each: the two have nothing to do with one another.
+template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_rank_kernel(uint32_t *__restrict__ keys, int *__restrict__ order,
-                                                                     const int *__restrict__ ids, int tokens,
-                                                                     int padding, int vocab) {
+                                                                     const int *__restrict__ ids, T *__restrict__ dtable,
+                                                                     EmbShape s, int rank_blocks, int rows,
+                                                                     int log_lanes) {
   extern __shared__ __align__(16) uint32_t all[];
+  if ((int)blockIdx.x >= rank_blocks) {
+    constexpr int V = Num<T>::V;
+    const int lanes = 1 << log_lanes, groups = EMB_THREADS >> log_lanes;
+    const int v0 = ((int)blockIdx.x - rank_blocks) * rows, v1 = min(v0 + rows, s.vocab);
+    float zero[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+    if (s.table_stride == (size_t)s.width) {  // dense rows: one stretch, whose stores are aligned whatever the width is
+      const size_t end = (size_t)v1 * s.width;
+      for (size_t i = (size_t)v0 * s.width + threadIdx.x * V; i < end; i += EMB_THREADS * V) {
+        if (s.stream)
+          store_vec_stream<T>(dtable + i, zero, 0, (int)min(end - i, (size_t)V));
+        else
+          store_vec<T>(dtable + i, zero, 0, (int)min(end - i, (size_t)V));
+      }
+      return;
+    }
+    for (int v = v0 + (int)(threadIdx.x >> log_lanes); v < v1; v += groups)
+      for (int col = (threadIdx.x & (lanes - 1)) * V; col < s.width; col += lanes * V) {
+        if (s.stream)
+          store_vec_stream<T>(dtable + (size_t)v * s.table_stride, zero, col, s.width);
+        else
+          store_vec<T>(dtable + (size_t)v * s.table_stride, zero, col, s.width);
+      }
+    return;
+  }
+  const int tokens = s.tokens, padding = s.padding, vocab = s.vocab;
   const int lane = threadIdx.x % EMB_RANK_LANES, t0 = blockIdx.x * EMB_RANK_TOKENS;
   const int t = t0 + threadIdx.x / EMB_RANK_LANES;
   const int pad = (tokens + 63) & ~63;
@@ -358,6 +388,37 @@ struct EmbRun {
   int id;
 };
 
+// Piece `piece` of the ids that are summed in pieces, by a workgroup; bounds: four words of LDS.
+template <class T>
+__device__ __forceinline__ void sum_piece(float *__restrict__ parts, EmbRun *__restrict__ runs, const T *__restrict__ dout,
+                                          const uint32_t *__restrict__ keys, const int *__restrict__ order, int piece,
+                                          int *bounds, const EmbShape &s) {
+  constexpr int V = Num<T>::V;
+  const int tid = threadIdx.x, a = piece * EMB_RUN, b = min(a + EMB_RUN, s.tokens);
+  // wavefronts 0 and 1: the id at the piece's first place; 2 and 3: the one at its last
+  const uint32_t key = keys[tid < 128 ? a : b - 1];
+  const int at = wave_lower_bound(keys, s.tokens, key + ((tid >> 6) & 1), tid & 63);
+  if ((tid & 63) == 0) bounds[tid >> 6] = at;
+  __syncthreads();
+  if (tid == 128) {
+    const bool begins = key < (uint32_t)s.vocab && bounds[3] - bounds[2] > EMB_RUN && bounds[2] >= a;
+    runs[piece] = begins ? EmbRun{bounds[2], bounds[3], (int)key} : EmbRun{0, 0, 0};
+  }
+  for (int slot = 0; slot < 2; ++slot) {
+    const int r0 = bounds[2 * slot], r1 = bounds[2 * slot + 1];
+    if (r1 - r0 <= EMB_RUN || keys[r0] >= (uint32_t)s.vocab || (slot == 1 && r0 <= a)) continue;
+    const int p0 = max(r0, a), p1 = min(r1, b);
+    float *dst = parts + ((size_t)piece * 2 + slot) * s.width;
+    for (int col = tid * V; col < s.width; col += EMB_THREADS * V) {
+      float acc[1][V];
+      sum_rows<T, 1>(acc, dout, order, p0, p1, col, 0, s);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (col + i < s.width) dst[col + i] = acc[0][i];
+    }
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(T *__restrict__ dtable, float *__restrict__ parts,
                                                                     EmbRun *__restrict__ runs,
@@ -402,27 +463,45 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(T *__restric
     }
     return;
   }
-  const int piece = blockIdx.x, a = piece * EMB_RUN, b = min(a + EMB_RUN, s.tokens);
-  // wavefronts 0 and 1: the id at the piece's first place; 2 and 3: the one at its last
-  const uint32_t key = keys[tid < 128 ? a : b - 1];
-  const int at = wave_lower_bound(keys, s.tokens, key + ((tid >> 6) & 1), tid & 63);
-  if ((tid & 63) == 0) bounds[tid >> 6] = at;
-  __syncthreads();
-  if (tid == 128) {
-    const bool begins = key < (uint32_t)s.vocab && bounds[3] - bounds[2] > EMB_RUN && bounds[2] >= a;
-    runs[piece] = begins ? EmbRun{bounds[2], bounds[3], (int)key} : EmbRun{0, 0, 0};
+  sum_piece<T>(parts, runs, dout, keys, order, blockIdx.x, bounds, s);
+}
+
+// The same from the tokens' side, for a table whose other rows have been cleared beside the sort: a group of lanes takes
+// EMB_RUN_PLACES sorted places and sums the ids that begin there.  No row is looked up, and rows without tokens cost this launch
+// nothing (4099 tokens, 10007 rows of 1001 fp32: 34 us with the kernel above in its place).
+constexpr int EMB_RUN_PLACES = 2;
+template <class T>
+__global__ __launch_bounds__(EMB_THREADS) void embedding_runs_kernel(T *__restrict__ dtable, float *__restrict__ parts,
+                                                                     EmbRun *__restrict__ runs,
+                                                                     const T *__restrict__ dout,
+                                                                     const uint32_t *__restrict__ keys,
+                                                                     const int *__restrict__ order, EmbShape s,
+                                                                     int accumulate, int log_lanes, int pieces) {
+  constexpr int V = Num<T>::V;
+  constexpr int MOST = EMB_THREADS * EMB_RUN_PLACES + EMB_RUN + 1;
+  __shared__ uint32_t key_sh[MOST + 1];  // [0]: the place before the first
+  __shared__ int place_sh[MOST];
+  if ((int)blockIdx.x < pieces) return sum_piece<T>(parts, runs, dout, keys, order, blockIdx.x, place_sh, s);
+  const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes;
+  const int places = (EMB_THREADS >> log_lanes) * EMB_RUN_PLACES, first = ((int)blockIdx.x - pieces) * places;
+  for (int i = tid; i <= places + EMB_RUN; i += EMB_THREADS) {
+    const int p = first + i;
+    key_sh[i + 1] = p < s.tokens ? keys[p] : 0xFFFFFFFFu;
+    place_sh[i] = p < s.tokens ? order[p] : 0;
   }
-  for (int slot = 0; slot < 2; ++slot) {
-    const int r0 = bounds[2 * slot], r1 = bounds[2 * slot + 1];
-    if (r1 - r0 <= EMB_RUN || keys[r0] >= (uint32_t)s.vocab || (slot == 1 && r0 <= a)) continue;
-    const int p0 = max(r0, a), p1 = min(r1, b);
-    float *dst = parts + ((size_t)piece * 2 + slot) * s.width;
-    for (int col = tid * V; col < s.width; col += EMB_THREADS * V) {
+  if (tid == 0) key_sh[0] = first > 0 ? keys[first - 1] : 0xFFFFFFFFu;
+  __syncthreads();
+  for (int q = 0; q < EMB_RUN_PLACES; ++q) {
+    const int at = group * EMB_RUN_PLACES + q;
+    const uint32_t key = key_sh[at + 1];
+    if (key >= (uint32_t)s.vocab || key_sh[at] == key) continue;  // (what lies past the tokens is above every id)
+    int length = 1;
+    while (length <= EMB_RUN && key_sh[at + 1 + length] == key) ++length;
+    if (length > EMB_RUN) continue;  // in pieces
+    for (int col = lane * V; col < s.width; col += lanes * V) {
       float acc[1][V];
-      sum_rows<T, 1>(acc, dout, order, p0, p1, col, 0, s);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (col + i < s.width) dst[col + i] = acc[0][i];
+      sum_rows<T, 1>(acc, dout, place_sh, at, at + length, col, 0, s);
+      store_row<T>(dtable + (size_t)key * s.table_stride, acc[0], col, s, accumulate);
     }
   }
 }
@@ -612,15 +691,6 @@ static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const Em
   hipStream_t st = ctx().stream;
   uint32_t *k[2] = {(uint32_t *)(ws + w.keys[0]), (uint32_t *)(ws + w.keys[1])};
   int *o[2] = {(int *)(ws + w.order[0]), (int *)(ws + w.order[1])};
-  if (s.tokens <= EMB_RANK_MAX) {
-    const int blocks = (s.tokens + EMB_RANK_TOKENS - 1) / EMB_RANK_TOKENS;
-    const size_t lds = ((size_t)s.tokens + 63) / 64 * 64 * sizeof(uint32_t);
-    embedding_rank_kernel<<<blocks, EMB_THREADS, lds, st>>>(k[0], o[0], ids, s.tokens, s.padding, s.vocab);
-    CCT_LAUNCH_CHECK();
-    *keys = k[0];
-    *order = o[0];
-    return 0;
-  }
   const unsigned tiles = (s.tokens + EMB_TILE - 1) / EMB_TILE;
   uint32_t *counts = (uint32_t *)(ws + w.counts);
   int from = -1;  // the first pass reads the ids
@@ -656,17 +726,36 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
     note_kernel("embedding_few_kernel<%s> rows per workgroup=%d", Num<T>::NAME, rows);
     return 0;
   }
-  uint32_t *keys = nullptr;
-  int *order = nullptr;
-  if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
   const int pieces = (s.tokens + EMB_RUN - 1) / EMB_RUN;
   float *parts = (float *)(ws + w.parts);
   EmbRun *runs = (EmbRun *)(ws + w.runs);
-  // the pieces first: they take the longest
-  embedding_sum_kernel<T><<<pieces + row_blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
-                                                                      s, accumulate, l, pieces);
-  CCT_LAUNCH_CHECK();
-  note_kernel("embedding_sum_kernel<%s> rows per workgroup=%d pieces=%d", Num<T>::NAME, rows, pieces);
+  if (s.tokens <= EMB_RANK_MAX) {
+    uint32_t *keys = (uint32_t *)(ws + w.keys[0]);
+    int *order = (int *)(ws + w.order[0]);
+    const int rank_blocks = (s.tokens + EMB_RANK_TOKENS - 1) / EMB_RANK_TOKENS;
+    // a workgroup clears 32 KB or more
+    const size_t row_bytes = (size_t)s.width * sizeof(T);
+    const int clear_rows = max(EMB_THREADS >> l, ((int)((32768 + row_bytes - 1) / row_bytes) + 7) & ~7);  // (whole vectors)
+    const int clear_blocks = accumulate ? 0 : (s.vocab + clear_rows - 1) / clear_rows;
+    const size_t lds = ((size_t)s.tokens + 63) / 64 * 64 * sizeof(uint32_t);
+    embedding_rank_kernel<T><<<rank_blocks + clear_blocks, EMB_THREADS, lds, st>>>(keys, order, ids, (T *)dtable, s,
+                                                                                  rank_blocks, clear_rows, l);
+    CCT_LAUNCH_CHECK();
+    const int places = (EMB_THREADS >> l) * EMB_RUN_PLACES, blocks = (s.tokens + places - 1) / places;
+    embedding_runs_kernel<T><<<pieces + blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
+                                                                     s, accumulate, l, pieces);
+    CCT_LAUNCH_CHECK();
+    note_kernel("embedding_runs_kernel<%s> pieces=%d", Num<T>::NAME, pieces);
+  } else {
+    uint32_t *keys = nullptr;
+    int *order = nullptr;
+    if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
+    // the pieces first: they take the longest
+    embedding_sum_kernel<T><<<pieces + row_blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
+                                                                        s, accumulate, l, pieces);
+    CCT_LAUNCH_CHECK();
+    note_kernel("embedding_sum_kernel<%s> rows per workgroup=%d pieces=%d", Num<T>::NAME, rows, pieces);
+  }
   {
     const int cols = min((s.width + 255) / 256, 64);
     embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, s,
