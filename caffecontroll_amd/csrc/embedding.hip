@@ -20,7 +20,7 @@ struct EmbShape {
   int stream;  // the result goes past the caches
 };
 // Results above this do not stay in the caches anyway (L2: 32 MB); written past them they leave them to the rows that are read
-// (65536 tokens of 2048 bf16: 77 instead of 92 us; the gradient of 131072 rows of 4096: 422 instead of 434 us).
+// (65536 tokens of 2048 bf16: 77 instead of 92 us; the gradient of 131072 rows of 4096: 3 % less).
 constexpr size_t EMB_STREAM_BYTES = (size_t)32 << 20;
 
 // ---- forward -----------------------------------------------------------------------------------------------------
@@ -62,6 +62,31 @@ __device__ __forceinline__ uint32_t sort_key(int id, int padding, int vocab) {
   return id == padding || (unsigned)id >= (unsigned)vocab ? (uint32_t)vocab : (uint32_t)id;
 }
 
+// The table cleared by workgroups of 4 KB each, in address order (6.8 TB/s; with 32 KB a workgroup 5.1 TB/s for 1 GB), whose
+// stores are aligned whatever the width is; or by one row each where rows have gaps between them.
+static unsigned clear_blocks_of(const EmbShape &s, int vec) {
+  const size_t dense = ((size_t)s.vocab * s.width + EMB_THREADS * vec - 1) / (EMB_THREADS * vec);
+  return s.table_stride == (size_t)s.width && dense < (1u << 23) ? (unsigned)dense : (unsigned)s.vocab;
+}
+template <class T>
+__device__ __forceinline__ void clear_block(T *__restrict__ dtable, const EmbShape &s, uint32_t block, uint32_t blocks) {
+  constexpr int V = Num<T>::V;
+  float zero[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+  const bool rows = blocks == (uint32_t)s.vocab;
+  const size_t i = rows ? (size_t)block * s.table_stride : ((size_t)block * EMB_THREADS + threadIdx.x) * V;
+  const size_t end = rows ? i + s.width : (size_t)s.vocab * s.width;
+  const size_t step = EMB_THREADS * V;
+  for (size_t at = rows ? i + threadIdx.x * V : i; at < end; at += step) {
+    if (s.stream)
+      store_vec_stream<T>(dtable + at, zero, 0, (int)min(end - at, (size_t)V));
+    else
+      store_vec<T>(dtable + at, zero, 0, (int)min(end - at, (size_t)V));
+    if (!rows) break;
+  }
+}
+
 // Few tokens: a token's place is the number of tokens that come before it, counted directly.  All keys lie in LDS; 16 lanes
 // share a token and take four keys at a time.  Of a workgroup's 16 tokens, those before the first of them come earlier
 // with an equal key too, those behind the last one do not, so but for one stretch of 16 every key costs one comparison.
@@ -69,39 +94,13 @@ __device__ __forceinline__ uint32_t sort_key(int id, int padding, int vocab) {
 constexpr int EMB_RANK_MAX = 8192;
 constexpr int EMB_RANK_LANES = 16;
 constexpr int EMB_RANK_TOKENS = EMB_THREADS / EMB_RANK_LANES;
-// Workgroups behind those that rank clear the table, `rows` rows each: the two have nothing to do with one another.
+// Workgroups behind those that rank clear the table: the two have nothing to do with one another.
 template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_rank_kernel(uint32_t *__restrict__ keys, int *__restrict__ order,
                                                                      const int *__restrict__ ids, T *__restrict__ dtable,
-                                                                     EmbShape s, int rank_blocks, int rows,
-                                                                     int log_lanes) {
+                                                                     EmbShape s, int rank_blocks) {
   extern __shared__ __align__(16) uint32_t all[];
-  if ((int)blockIdx.x >= rank_blocks) {
-    constexpr int V = Num<T>::V;
-    const int lanes = 1 << log_lanes, groups = EMB_THREADS >> log_lanes;
-    const int v0 = ((int)blockIdx.x - rank_blocks) * rows, v1 = min(v0 + rows, s.vocab);
-    float zero[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) zero[i] = 0.0f;
-    if (s.table_stride == (size_t)s.width) {  // dense rows: one stretch, whose stores are aligned whatever the width is
-      const size_t end = (size_t)v1 * s.width;
-      for (size_t i = (size_t)v0 * s.width + threadIdx.x * V; i < end; i += EMB_THREADS * V) {
-        if (s.stream)
-          store_vec_stream<T>(dtable + i, zero, 0, (int)min(end - i, (size_t)V));
-        else
-          store_vec<T>(dtable + i, zero, 0, (int)min(end - i, (size_t)V));
-      }
-      return;
-    }
-    for (int v = v0 + (int)(threadIdx.x >> log_lanes); v < v1; v += groups)
-      for (int col = (threadIdx.x & (lanes - 1)) * V; col < s.width; col += lanes * V) {
-        if (s.stream)
-          store_vec_stream<T>(dtable + (size_t)v * s.table_stride, zero, col, s.width);
-        else
-          store_vec<T>(dtable + (size_t)v * s.table_stride, zero, col, s.width);
-      }
-    return;
-  }
+  if ((int)blockIdx.x >= rank_blocks) return clear_block<T>(dtable, s, blockIdx.x - rank_blocks, gridDim.x - rank_blocks);
   const int tokens = s.tokens, padding = s.padding, vocab = s.vocab;
   const int lane = threadIdx.x % EMB_RANK_LANES, t0 = blockIdx.x * EMB_RANK_TOKENS;
   const int t = t0 + threadIdx.x / EMB_RANK_LANES;
@@ -162,11 +161,15 @@ __device__ __forceinline__ uint32_t pass_key(const uint32_t *__restrict__ keys, 
   return keys ? keys[i] : sort_key(ids[i], padding, vocab);
 }
 
+// Workgroups behind the tiles' clear the table.
+template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_count_kernel(uint32_t *__restrict__ counts,
                                                                       const uint32_t *__restrict__ keys,
-                                                                      const int *__restrict__ ids, int tokens,
-                                                                      int padding, int vocab, int shift) {
+                                                                      const int *__restrict__ ids, T *__restrict__ dtable,
+                                                                      EmbShape s, int shift, int tiles) {
   __shared__ uint32_t bins[EMB_BINS];
+  if ((int)blockIdx.x >= tiles) return clear_block<T>(dtable, s, blockIdx.x - tiles, gridDim.x - tiles);
+  const int tokens = s.tokens, padding = s.padding, vocab = s.vocab;
   for (int i = threadIdx.x; i < EMB_BINS; i += EMB_THREADS) bins[i] = 0;
   __syncthreads();
   for (int i = 0; i < EMB_ITEMS; ++i) {
@@ -509,18 +512,22 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_runs_kernel(T *__restri
 // The pieces of a long id, added in order: workgroups of the EMB_JOIN pieces among which it begins, 256 columns each, their
 // four wavefronts taking every fourth piece.  (One workgroup per piece and 256 columns are mostly workgroups that find
 // nothing: 36 us for 65536 tokens of width 4096.)
-constexpr int EMB_JOIN = 8;
+constexpr int EMB_JOIN = 16;
+constexpr int EMB_JOIN_WAVES = 4;
 template <class T>
-__global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(T *__restrict__ dtable,
+__global__ __launch_bounds__(EMB_JOIN_WAVES * 64) void embedding_join_kernel(T *__restrict__ dtable,
                                                                      const float *__restrict__ parts,
                                                                      const EmbRun *__restrict__ runs, EmbShape s,
                                                                      int accumulate, int pieces) {
-  __shared__ f32x4 sums[3][64];
+  __shared__ f32x4 sums[EMB_JOIN_WAVES][64];
   const int tid = threadIdx.x, lane = tid & 63, group = tid >> 6;
-  const int first = blockIdx.x * EMB_JOIN, last = min(first + EMB_JOIN, pieces);
-  for (int piece = first; piece < last; ++piece) {
-    const EmbRun run = runs[piece];
-    if (run.first == run.last) continue;
+  const int first = blockIdx.x * EMB_JOIN, slot = first + (lane & (EMB_JOIN - 1));
+  const EmbRun mine = slot < pieces ? runs[slot] : EmbRun{0, 0, 0};  // all of them with one load
+  uint64_t found = __ballot(lane < EMB_JOIN && mine.first != mine.last);
+  while (found) {
+    const int which = __builtin_ctzll(found), piece = first + which;
+    found &= found - 1;
+    const EmbRun run{__shfl(mine.first, which, 64), __shfl(mine.last, which, 64), __shfl(mine.id, which, 64)};
     const int end = (run.last - 1) / EMB_RUN;
     for (int c0 = blockIdx.y * 256; c0 < s.width; c0 += gridDim.y * 256) {
       const int col = c0 + lane * 4;
@@ -532,22 +539,23 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_join_kernel(T *__restri
       };
       int j = piece + group;
       if (j <= end) add(j);
-      j += 4;
+      j += EMB_JOIN_WAVES;
       if (col + 4 <= s.width)
-        for (; j + 28 <= end; j += 32) {  // eight loads in flight, added in order
+        for (; j + 7 * EMB_JOIN_WAVES <= end; j += 8 * EMB_JOIN_WAVES) {  // eight loads in flight, added in order
           Num<float>::vec v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            v[k] = *reinterpret_cast<const Num<float>::vec *>(parts + (size_t)(j + 4 * k) * 2 * s.width + col);
+            v[k] = *reinterpret_cast<const Num<float>::vec *>(parts + (size_t)(j + EMB_JOIN_WAVES * k) * 2 * s.width + col);
 #pragma unroll
           for (int k = 0; k < 8; ++k) acc += f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
         }
-      for (; j <= end; j += 4) add(j);
+      for (; j <= end; j += EMB_JOIN_WAVES) add(j);
       __syncthreads();
-      if (group > 0) sums[group - 1][lane] = acc;
+      if (group > 0) sums[group][lane] = acc;
       __syncthreads();
       if (group == 0) {
-        acc = ((acc + sums[0][lane]) + sums[1][lane]) + sums[2][lane];
+#pragma unroll
+        for (int w = 1; w < EMB_JOIN_WAVES; ++w) acc += sums[w][lane];
         T *dst = dtable + (size_t)run.id * s.table_stride + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -687,7 +695,9 @@ static int embedding_forward(void *out, const void *table, const int *ids, const
   return 0;
 }
 
-static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const EmbShape &s, uint32_t **keys, int **order) {
+template <class T>
+static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const EmbShape &s, T *dtable, unsigned clear_blocks,
+                       uint32_t **keys, int **order) {
   hipStream_t st = ctx().stream;
   uint32_t *k[2] = {(uint32_t *)(ws + w.keys[0]), (uint32_t *)(ws + w.keys[1])};
   int *o[2] = {(int *)(ws + w.order[0]), (int *)(ws + w.order[1])};
@@ -698,7 +708,9 @@ static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const Em
     const int to = from == 0 ? 1 : 0;
     const uint32_t *kin = from < 0 ? nullptr : k[from];
     const int *oin = from < 0 ? nullptr : o[from];
-    embedding_count_kernel<<<tiles, EMB_THREADS, 0, st>>>(counts, kin, ids, s.tokens, s.padding, s.vocab, shift);
+    // the table is cleared beside the first pass's count
+    embedding_count_kernel<T><<<tiles + (from < 0 ? clear_blocks : 0u), EMB_THREADS, 0, st>>>(
+        counts, kin, ids, dtable, s, shift, (int)tiles);
     CCT_LAUNCH_CHECK();
     if (tiles > EMB_TILES_MAX) {
       embedding_scan_kernel<<<1, EMB_BINS, 0, st>>>(counts, tiles);
@@ -729,27 +741,30 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
   const int pieces = (s.tokens + EMB_RUN - 1) / EMB_RUN;
   float *parts = (float *)(ws + w.parts);
   EmbRun *runs = (EmbRun *)(ws + w.runs);
-  if (s.tokens <= EMB_RANK_MAX) {
-    uint32_t *keys = (uint32_t *)(ws + w.keys[0]);
-    int *order = (int *)(ws + w.order[0]);
+  const bool ranked = s.tokens <= EMB_RANK_MAX;
+  // Visiting only the rows with tokens writes those twice; looking every row's tokens up costs those that have none.
+  // 131072 rows of 4096 bf16, 65536 tokens as text has them (a fifth of the rows): 367 and 421 us; all of them different (half
+  // of the rows): 394 and 369 us.  With more tokens than half the rows the second way is taken.
+  const bool visit = ranked || s.tokens <= s.vocab / 2;
+  const unsigned clear_blocks = accumulate || !visit ? 0u : clear_blocks_of(s, Num<T>::V);
+  uint32_t *keys = (uint32_t *)(ws + w.keys[0]);
+  int *order = (int *)(ws + w.order[0]);
+  if (ranked) {
     const int rank_blocks = (s.tokens + EMB_RANK_TOKENS - 1) / EMB_RANK_TOKENS;
-    // a workgroup clears 32 KB or more
-    const size_t row_bytes = (size_t)s.width * sizeof(T);
-    const int clear_rows = max(EMB_THREADS >> l, ((int)((32768 + row_bytes - 1) / row_bytes) + 7) & ~7);  // (whole vectors)
-    const int clear_blocks = accumulate ? 0 : (s.vocab + clear_rows - 1) / clear_rows;
     const size_t lds = ((size_t)s.tokens + 63) / 64 * 64 * sizeof(uint32_t);
     embedding_rank_kernel<T><<<rank_blocks + clear_blocks, EMB_THREADS, lds, st>>>(keys, order, ids, (T *)dtable, s,
-                                                                                  rank_blocks, clear_rows, l);
+                                                                                  rank_blocks);
     CCT_LAUNCH_CHECK();
+  } else if (int rc = sort_tokens<T>(ws, w, ids, s, (T *)dtable, clear_blocks, &keys, &order)) {
+    return rc;
+  }
+  if (visit) {
     const int places = (EMB_THREADS >> l) * EMB_RUN_PLACES, blocks = (s.tokens + places - 1) / places;
     embedding_runs_kernel<T><<<pieces + blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
                                                                      s, accumulate, l, pieces);
     CCT_LAUNCH_CHECK();
     note_kernel("embedding_runs_kernel<%s> pieces=%d", Num<T>::NAME, pieces);
   } else {
-    uint32_t *keys = nullptr;
-    int *order = nullptr;
-    if (int rc = sort_tokens(ws, w, ids, s, &keys, &order)) return rc;
     // the pieces first: they take the longest
     embedding_sum_kernel<T><<<pieces + row_blocks, EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, (const T *)dout, keys, order,
                                                                         s, accumulate, l, pieces);
@@ -758,7 +773,7 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
   }
   {
     const int cols = min((s.width + 255) / 256, 64);
-    embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_THREADS, 0, st>>>((T *)dtable, parts, runs, s,
+    embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_JOIN_WAVES * 64, 0, st>>>((T *)dtable, parts, runs, s,
                                                                                                  accumulate, pieces);
     CCT_LAUNCH_CHECK();
   }
