@@ -839,10 +839,14 @@ constexpr size_t kPieceBytes = (size_t)384 << 20;  // automatic piece: G and w's
 // a tile's rows are addressed with 32-bit byte offsets: 256 rows of a piece's columns in fp32 are 2^30 bytes
 constexpr int kPieceMax = 1 << 20;
 
+// rows that the product kernel can take as they are, if they start at a multiple of 16 bytes
+static bool whole_chunks(size_t ld, int width, size_t el) { return (ld * el & 15) == 0 && ((size_t)width * el & 15) == 0; }
+
 struct VocabPlan {
   int tokens, width, vocab, dtype;
   size_t el, ldx, ldw;
   int unit;            // elements of a 128-byte step
+  bool packed;         // rows of x or w are no whole 16-byte chunks: those operands are copied
   int piece, pieces;   // rows of w at a time
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, kept, dx, dw;
@@ -866,18 +870,24 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.np = (idiv(p.tokens, p.unit) + 1) * p.unit;
   const size_t n = p.tokens;
   const int vmax = idiv(p.vocab, 256) * 256;
+  p.packed = !whole_chunks(p.ldx, p.width, p.el) || !whole_chunks(p.ldw, p.width, p.el);
+  // a piece's tiles, with the smallest tile, are fewer than 2^32 lanes in a launch
+  size_t most = ((size_t)1 << 34) / (n > (size_t)p.hp ? n : (size_t)p.hp) & ~(size_t)255;
+  if (most < 256) most = 256;
+  if (most > (size_t)kPieceMax) most = kPieceMax;
   if (a->piece > 0) {
-    p.piece = (int)min((((size_t)a->piece + 255) / 256) * 256, (size_t)kPieceMax);
+    p.piece = (int)min((((size_t)a->piece + 255) / 256) * 256, most);
   } else {
     // a power of two, so that the tiles of a piece fill whole rounds of the chip
     const size_t row = (n + p.hp) * p.el, want = kPieceBytes / row;
     size_t rows = 1024;
     while (rows * 2 <= want && rows < (size_t)vmax) rows *= 2;
-    p.piece = (int)min(rows, (size_t)kPieceMax);
+    p.piece = (int)min(rows, most);
   }
   if (p.piece > vmax) p.piece = vmax;
-  // kept scores: all of the vocabulary at once
-  const bool may_keep = vmax <= kPieceMax && (a->piece <= 0 || p.piece == vmax);
+  // kept scores: all of the vocabulary at once, and so its packed copy
+  const bool may_keep = (size_t)vmax <= most && (a->piece <= 0 || p.piece == vmax) &&
+                        (!p.packed || (size_t)vmax * p.hp * p.el <= kPieceBytes);
   p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
   p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, true, true);
   const double score_bytes = (double)n * vmax * 4;
@@ -911,15 +921,16 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   };
   p.part = take((size_t)p.stats_tiles * n * sizeof(SoftStat));
   p.label_score = take(n * 4);
-  p.xpack = take(n * p.hp * p.el);
-  p.wpack = take((size_t)p.piece * p.hp * p.el);
+  p.xpack = take(p.packed ? n * p.hp * p.el : 0);
+  p.wpack = take(p.packed ? (size_t)p.piece * p.hp * p.el : 0);
   const size_t score_space = (size_t)p.kept.splits * n * p.vp * 4;
   p.scores = take(p.keep_forward ? score_space : 0);
   p.total_forward = at;
   if (!p.keep_forward) p.scores = take(keep_any ? score_space : 0);
   p.xl = take((p.el == 2 ? (size_t)p.width * p.np : n * p.hp) * p.el);
   p.wmax = take(4);
-  p.g = take(n * p.vp * p.el);
+  const bool g_in_scores = p.el == 4 && p.keep_backward[0] && p.keep_backward[1] && p.keep_both[0] && p.keep_both[1];
+  p.g = take(g_in_scores ? 0 : n * p.vp * p.el);
   p.slabs = take((size_t)p.dx.splits * n * p.hp * 4);
   p.db = take((size_t)idiv(p.tokens, 32) * p.vp * 4);
   p.total = at;
@@ -976,11 +987,6 @@ struct VocabCall {
   bool forward, backward;
 };
 
-// operand rows as the product kernel needs them: 16-byte aligned, whole 16-byte chunks
-static bool direct_rows(const void *p, size_t ld, int width, size_t el) {
-  return ((uintptr_t)p & 15) == 0 && (ld * el & 15) == 0 && ((size_t)width * el & 15) == 0;
-}
-
 template <class T>
 static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   hipStream_t st = ctx().stream;
@@ -995,7 +1001,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   if (keep && p.el == 4) g = (T *)scores;  // fp32 G takes the scores' place
   const size_t packed = p.hp * p.el;
   const int chunk = p.unit / 8;  // elements of 16 bytes
-  const bool direct_x = direct_rows(c.x, p.ldx, p.width, p.el), direct_w = direct_rows(c.w, p.ldw, p.width, p.el);
+  const bool direct_x = whole_chunks(p.ldx, p.width, p.el), direct_w = whole_chunks(p.ldw, p.width, p.el);
   const char *x = (const char *)(direct_x ? c.x : c.ws + p.xpack);
   const size_t ldx = direct_x ? p.ldx * p.el : packed;
   bool x_packed = direct_x;
@@ -1163,6 +1169,13 @@ static int check_vocab_workspace(const VocabPlan &p, const void *ws, size_t byte
   return 0;
 }
 
+static int check_vocab_rows(const VocabPlan &p, const void *x, const void *w, const char *who) {
+  CCT_REQUIRE(!(whole_chunks(p.ldx, p.width, p.el) && ((uintptr_t)x & 15)) &&
+                  !(whole_chunks(p.ldw, p.width, p.el) && ((uintptr_t)w & 15)),
+              "%s: x at %p, w at %p: rows of whole 16-byte chunks have to start at a multiple of 16 bytes", who, x, w);
+  return 0;
+}
+
 static int vocab_dispatch(const VocabPlan &p, const VocabCall &c) {
   CCT_ENSURE_INIT();
   return p.dtype == CCT_BF16 ? vocab_run<bf16>(p, c) : vocab_run<float>(p, c);
@@ -1202,6 +1215,7 @@ extern "C" int cct_hip_vocab_loss_forward(float *loss, float *lse, const void *x
   CCT_REQUIRE(loss && lse && x && w && labels, "%s: null array", who);
   const VocabPlan p = vocab_plan(args);
   if (int rc = check_vocab_workspace(p, workspace, workspace_bytes, false, who)) return rc;
+  if (int rc = check_vocab_rows(p, x, w, who)) return rc;
   VocabCall c{};
   c.loss = loss;
   c.lse = lse;
@@ -1225,6 +1239,7 @@ extern "C" int cct_hip_vocab_loss_backward(void *dx, void *dw, void *db, const v
   if (args->tokens == 0) return vocab_zero_gradients(p, dw, db);
   CCT_REQUIRE(x && w && labels && lse, "%s: null array", who);
   if (int rc = check_vocab_workspace(p, workspace, workspace_bytes, true, who)) return rc;
+  if (int rc = check_vocab_rows(p, x, w, who)) return rc;
   VocabCall c{};
   c.lse_in = lse;
   c.dx = dx;
@@ -1252,6 +1267,7 @@ extern "C" int cct_hip_vocab_loss_forward_backward(float *loss, float *lse, void
   if (args->tokens == 0) return vocab_zero_gradients(p, dw, db);
   CCT_REQUIRE(loss && lse && x && w && labels, "%s: null array", who);
   if (int rc = check_vocab_workspace(p, workspace, workspace_bytes, true, who)) return rc;
+  if (int rc = check_vocab_rows(p, x, w, who)) return rc;
   VocabCall c{};
   c.loss = loss;
   c.lse = lse;

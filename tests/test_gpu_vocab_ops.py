@@ -359,6 +359,45 @@ def test_vocab_loss_with_strides_leaves_the_gaps_alone(dtype):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+def test_operators_on_columns_of_wider_matrices(dtype):
+    """Rows that start at an element's alignment: every matrix is a view from the second column on."""
+    import torch
+    from caffecontroll_amd.driver import embedding_args, vocab_loss_args
+    drv, v = driver(), Vocab(dtype, 90, 77, 700, bias=True).reference()
+
+    def view(t, fill):
+        whole = torch.full((t.shape[0], t.shape[1] + 19), fill, dtype=t.dtype, device="cuda")
+        whole[:, 1:1 + t.shape[1]] = t
+        return whole, whole[:, 1:1 + t.shape[1]]
+
+    (xw, x), (ww, w) = view(v.x, float("nan")), view(v.w, float("nan"))
+    (dxw, dx), (dww, dw) = view(torch.zeros_like(v.x), 7.0), view(torch.zeros_like(v.w), 7.0)
+    v.outputs()
+    v.o_dx, v.o_dw = dx, dw
+    a = vocab_loss_args(90, 77, 700, code(dtype), x_stride=96, w_stride=96)
+    n = drv.vocab_loss_workspace_bytes(a)
+    drv.vocab_loss_forward_backward(v.o_loss, v.o_lse, dx, dw, v.o_db, x, w, v.b, ints(v.labels), up(v.gs)[0], a,
+                                    space(n).ptr, n)
+    v.check_loss()
+    v.check_gradients()
+    for t in (dxw, dww):
+        assert (t[:, 0] == 7.0).all() and (t[:, 78:] == 7.0).all()
+    ids = np.random.default_rng(3).integers(0, 700, 90)
+    ea = embedding_args(90, 77, 700, code(dtype), 2.0, -1, 96, 96)
+    outw, out = view(torch.zeros_like(v.x), 7.0)
+    drv.embedding_forward(out, w, ints(ids), ea)
+    near(values(out), 2.0 * v.w64[ids], 0.0)                    # a power of two: exact
+    drv.embedding_backward(dw, out, ints(ids), ea, None, 0)
+    want = np.zeros((700, 77))
+    np.add.at(want, ids, 2.0 * values(out))
+    size = np.zeros((700, 77))
+    np.add.at(size, ids, 2.0 * np.abs(values(out)))
+    near(values(dw), want, (90 * U + HALF[dtype]) * size)
+    for t in (outw, dww):
+        assert (t[:, 0] == 7.0).all() and (t[:, 78:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_vocab_loss_labels_outside_the_vocabulary_and_ignored_tokens(dtype):
     import torch
     v = Vocab(dtype, 40, 64, 500, bias=True, ignore=-100)

@@ -94,6 +94,16 @@ def test_vocab_loss_refuses_arrays_and_workspaces(drv):
     refused(drv.vocab_loss_forward_backward, A, A, A, A, None, A, A, None, A, None, a, None, need, match="workspace")
 
 
+def test_vocab_loss_refuses_rows_of_whole_chunks_that_start_between_them(drv):
+    for dtype, width, off in ((BF16, 8, 2), (F32, 4, 4), (BF16, 64, 8)):
+        a = vocab_loss_args(10, width, 300, dtype)
+        n = drv.vocab_loss_workspace_bytes(a)
+        for x, w in ((A + off, A), (A, A + off)):
+            refused(drv.vocab_loss_forward, A, A, x, w, None, A, a, A, n, match="multiple of 16")
+            refused(drv.vocab_loss_backward, A, A, None, x, w, None, A, A, None, a, A, n, match="multiple of 16")
+            refused(drv.vocab_loss_forward_backward, A, A, A, A, None, x, w, None, A, None, a, A, n, match="multiple of 16")
+
+
 def test_vocab_loss_workspace_stays_bounded():
     """The workspace goes by tokens and piece, not by tokens * vocab; pieces smaller than the automatic ones need less."""
     d = HIPDriver.__new__(HIPDriver)
