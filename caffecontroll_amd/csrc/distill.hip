@@ -239,8 +239,8 @@ __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, c
 // Loss and gradient of whole rows, each read once: a workgroup keeps its row in registers from the statistics to the
 // gradient, and fetches its next row into the registers that the gradient has left.  ITEMS vectors a lane; one entry of the
 // list a lane (top <= THREADS).  The statistics are taken vector by vector as they arrive, with a running maximum: the
-// exponentials (two per score, 16 us of a 128 K row's 26 us of traffic) then run beside the loads and stores, where a pass for the
-// maximum first had them wait for the whole row (4096 rows of 131072 bf16 scores: 490 us, 4.4 TB/s, against 585).
+// exponentials (two per score, 16 us of a 128 K row's 26 us of traffic) then run beside the loads and stores, where a pass for
+// the maximum first had them wait for the whole row (4096 rows of 131072 bf16 scores: 490 us, 4.4 TB/s, against 585).
 template <class T, int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict__ loss, float *__restrict__ lse, T *dlogits,
                                                               const T *logits, const int *__restrict__ ids,

@@ -471,8 +471,8 @@ __global__ __launch_bounds__(EMB_THREADS) void embedding_sum_kernel(T *__restric
 }
 
 // The same from the tokens' side, for a table whose other rows have been cleared beside the sort: a group of lanes takes
-// EMB_RUN_PLACES sorted places and sums the ids that begin there.  No row is looked up, and rows without tokens cost this launch
-// nothing (4099 tokens, 10007 rows of 1001 fp32: 34 us with the kernel above in its place).
+// EMB_RUN_PLACES sorted places and sums the ids that begin there.  No row is looked up, and rows without tokens cost this
+// launch nothing (4099 tokens, 10007 rows of 1001 fp32: 34 us with the kernel above in its place).
 constexpr int EMB_RUN_PLACES = 2;
 template <class T>
 __global__ __launch_bounds__(EMB_THREADS) void embedding_runs_kernel(T *__restrict__ dtable, float *__restrict__ parts,
@@ -775,8 +775,8 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, co
   }
   {
     const int cols = min((s.width + 255) / 256, 64);
-    embedding_join_kernel<T><<<dim3((pieces + EMB_JOIN - 1) / EMB_JOIN, cols), EMB_JOIN_WAVES * 64, 0, st>>>((T *)dtable, parts, runs, s,
-                                                                                                 accumulate, pieces);
+    const dim3 grid((pieces + EMB_JOIN - 1) / EMB_JOIN, cols);
+    embedding_join_kernel<T><<<grid, EMB_JOIN_WAVES * 64, 0, st>>>((T *)dtable, parts, runs, s, accumulate, pieces);
     CCT_LAUNCH_CHECK();
   }
   return 0;

@@ -53,7 +53,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 // 16 bytes a lane from global memory into LDS: lane l's land at dst + 16 l; an offset past the descriptor's 2^31 bytes fetches
 // nothing and writes zeros.  The instruction itself instead of its builtin: the compiler would wait for all copies
 // in flight before every ds_read_b64_tr_b16, whose address it cannot tell from theirs (a product with such an operand: 1.43
-// instead of 0.96 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 (the
+// instead of 0.83 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 (the
 // LDS address) is used by nothing else in these kernels.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, uint32_t offset, lds_char *dst) {
@@ -372,8 +372,9 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
           for (int it = 0; it < items; ++it) {
             if (it * MFMAS / items != m) continue;
             // the last phase alternates between copies and reads (what is read behind the last step is not used)
-            const int c = last ? (it < 2 * min(copies, reads) ? ((it & 1) ? -1 : it / 2) : (copies > reads ? it - reads : -1)) : -1;
-            const int r = last ? (it < 2 * min(copies, reads) ? it / 2 : it - copies) : it;
+            const bool paired = it < 2 * min(copies, reads);
+            const int c = !last ? -1 : paired ? ((it & 1) ? -1 : it / 2) : copies > reads ? it - reads : -1;
+            const int r = !last ? it : paired ? it / 2 : it - copies;
             if (c >= 0)
               copy(c, buf, s + S::STAGES);
             else
@@ -646,6 +647,202 @@ __global__ __launch_bounds__(256) void vocab_loss_kernel(float *__restrict__ los
     store_loss(loss, lse, t, log_sum(sh[0][x], 1.0f), labels[t], label_score[t], vocab, ignore);
 }
 
+// The loss of at most 64 tokens where w's rows would have to be packed first: one walk over w, its rows as they lie, bound by
+// reading them.  A wave takes 16 rows: lane l reads 16 bytes of row l & 15 and has with them its operand of a matrix
+// instruction, against the tokens' x, which lie in LDS in the order of that operand: all of them, or panel by panel of the
+// width with up to four times 16 rows a wave for each.  With few rows `split` waves share them, each a range of the width, and
+// the first one adds the sums up in order.  A lane keeps the running statistics of its token.  The chunk that holds a row's
+// end is the row's last 16 bytes, where those that the chunk before has too count as zero: no load has a branch
+// around it.  bf16, 2 tokens: 118050 rows of 119 in 13.6 us (30.7 with packing and the tiles above), 131071 rows of 4095 in 222
+// us, 4.8 TB/s (585); 64 tokens: 298 us (665).  fp32, 131071 rows of 4095: 2 tokens 367 us (1218), 64 tokens 722 us (1390).
+constexpr int kFewTokens = 64, kFewWaves = 8;
+// 16 bytes of a row of any alignment.  bf16 rows of odd lengths start between dwords, and 16 rows' 16-byte loads at such
+// addresses take twice the time of dword-aligned ones: those five dwords are read that hold the elements, and shifted.
+struct RowBytes {
+  uint32_t d[5], odd;
+};
+template <class T>
+__device__ __forceinline__ RowBytes row_load(const T *p) {
+  typedef u32x4 __attribute__((aligned(4))) u32x4_dword;
+  RowBytes b;
+  b.odd = sizeof(T) == 2 ? (uint32_t)(uintptr_t)p & 2 : 0;
+  const uint32_t *q = (const uint32_t *)((const char *)p - b.odd);
+  const u32x4 v = *(const u32x4_dword *)q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b.d[i] = v[i];
+  b.d[4] = sizeof(T) == 2 ? q[b.odd ? 4 : 3] : 0;  // none past the elements' own dwords
+  return b;
+}
+template <class T>
+__device__ __forceinline__ auto row_value(const RowBytes &b) {
+  typedef T vecT __attribute__((ext_vector_type(Num<T>::V)));
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = sizeof(T) == 2 ? __builtin_amdgcn_alignbit(b.d[i + 1], b.d[i], b.odd * 8) : b.d[i];
+  return __builtin_bit_cast(vecT, v);
+}
+constexpr int kFewLds = 144 << 10, kFewPanel = 64 << 10;  // x in LDS: all of it, or by panels
+constexpr int kFewRows = 4;                               // tiles of a wave for each staging of a panel
+struct FewShape {
+  int split;        // waves that share rows
+  int panel, rows;  // steps of the width in LDS, tiles of a wave where that is less than all of them
+};
+template <class T, int NT, bool PANELS>
+__global__ __launch_bounds__(kFewWaves * 64) void vocab_few_kernel(SoftStat *__restrict__ part,
+                                                                   float *__restrict__ label_score,
+                                                                   const T *__restrict__ x, const T *__restrict__ w,
+                                                                   const T *__restrict__ bias,
+                                                                   const int *__restrict__ labels, size_t ldx, size_t ldw,
+                                                                   int tokens, int width, int vocab, FewShape shape) {
+  constexpr int V = Num<T>::V, K = 4 * V, R = PANELS ? kFewRows : 1;
+  typedef T vecT __attribute__((ext_vector_type(V)));
+  extern __shared__ __align__(16) char lds[];
+  const int steps = (width + K - 1) / K, split = PANELS ? 1 : shape.split;
+  vecT *xs = (vecT *)lds;                                         // [step of the panel][16 tokens][lane]
+  f32x4 *sums = (f32x4 *)(xs + (size_t)shape.panel * NT * 64);    // [wave][16 tokens][lane], where waves share rows
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const auto stage = [&](int first, int count) {
+    for (int i = tid; i < count * NT * 64; i += kFewWaves * 64) {
+      const int l = i & 63, t = (i >> 6) % NT * 16 + (l & 15), col = (first + (i >> 6) / NT) * K + (l >> 4) * V;
+      const int from = min(col, width - V);
+      const vecT raw = row_value<T>(row_load(x + (size_t)min(t, tokens - 1) * ldx + from));
+      vecT v;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = t < tokens && from + e >= col ? raw[e] : (T)0.0f;
+      xs[i] = v;
+    }
+  };
+  if (!PANELS) {
+    stage(0, steps);
+    __syncthreads();
+  }
+  const int group = wave / split, share = wave % split;
+  const int rows = PANELS ? shape.rows : 1, stride = kFewWaves / split * rows;  // tiles of a wave, of a workgroup
+  const int per = (steps + split - 1) / split;
+  const int tiles = (vocab + 15) / 16;
+  SoftStat st[NT];
+  int label[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    st[n] = SoftStat{neg_inf(), 0.0f};
+    label[n] = n * 16 + (lane & 15) < tokens ? labels[n * 16 + (lane & 15)] : -1;
+  }
+  for (int first = (int)blockIdx.x * stride; first < tiles; first += (int)gridDim.x * stride) {
+    const int tile0 = first + group * rows;
+    f32x4 sum[R][NT];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sum[i][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p0 = 0; p0 < steps; p0 += shape.panel) {
+      if (PANELS) {
+        __syncthreads();  // the panel before has been used
+        stage(p0, min(shape.panel, steps - p0));
+        __syncthreads();
+      }
+      const int k0 = PANELS ? p0 : share * per, k1 = min(steps, PANELS ? p0 + shape.panel : k0 + per);
+      const int whole = min(k1, steps - 1);  // steps before the one that holds the rows' end
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i >= rows) break;
+        const T *row = w + (size_t)min((tile0 + i) * 16 + (lane & 15), vocab - 1) * ldw;
+        const auto multiply = [&](vecT a, int k) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const vecT b = xs[((k - (PANELS ? p0 : 0)) * NT + n) * 64 + lane];
+            if constexpr (sizeof(T) == 2) {
+              sum[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, sum[i][n], 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int e = 0; e < V; ++e)
+                sum[i][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], sum[i][n], 0, 0, 0);
+            }
+          }
+        };
+        const T *at = row + (lane >> 4) * V;
+        constexpr int AHEAD = 8;
+        int k = k0;
+        for (; k + AHEAD <= whole; k += AHEAD) {
+          RowBytes a[AHEAD];
+#pragma unroll
+          for (int j = 0; j < AHEAD; ++j) a[j] = row_load(at + (k + j) * K);
+          __builtin_amdgcn_sched_barrier(0);  // all of them are in flight before the first is used
+#pragma unroll
+          for (int j = 0; j < AHEAD; ++j) multiply(row_value<T>(a[j]), k + j);
+        }
+        for (; k < whole; ++k) multiply(row_value<T>(row_load(at + k * K)), k);
+        if (k0 < k1 && k1 == steps) {
+          const int col = (steps - 1) * K + (lane >> 4) * V, from = min(col, width - V);
+          const vecT raw = row_value<T>(row_load(row + from));
+          vecT a;
+#pragma unroll
+          for (int e = 0; e < V; ++e) a[e] = from + e >= col ? raw[e] : (T)0.0f;
+          multiply(a, steps - 1);
+        }
+      }
+    }
+    if (split > 1) {
+      __syncthreads();  // the sums of the rows before have been read
+      if (share != 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sums[(wave * NT + n) * 64 + lane] = sum[0][n];
+      }
+      __syncthreads();
+      if (share != 0) continue;
+      for (int o = 1; o < split; ++o) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const f32x4 other = sums[((wave + o) * NT + n) * 64 + lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[0][n][r] += other[r];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (i >= rows) break;
+      const int v = (tile0 + i) * 16 + (lane >> 4) * 4;
+      float add[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) add[r] = bias && v + r < vocab ? (float)bias[v + r] : 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float score[4], m = st[n].m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          score[r] = v + r < vocab ? sum[i][n][r] + add[r] : neg_inf();
+          m = fmaxf(m, score[r]);
+        }
+        const unsigned of = (unsigned)label[n] - (unsigned)v;
+        if (of < 4u && label[n] < vocab) {
+          float s = score[0];
+#pragma unroll
+          for (int r = 1; r < 4; ++r) s = of == (unsigned)r ? score[r] : s;
+          label_score[n * 16 + (lane & 15)] = s;
+        }
+        const float base = m == neg_inf() ? 0.0f : m;
+        float s = st[n].s * (st[n].m == m ? 1.0f : exp2_fast((st[n].m - base) * kLog2e));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += exp2_fast((score[r] - base) * kLog2e);
+        st[n] = SoftStat{m, s};
+      }
+    }
+  }
+  __shared__ SoftStat sh[kFewWaves][NT * 16];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    st[n] = shfl_xor_join(st[n], 16, kLog2e);
+    st[n] = shfl_xor_join(st[n], 32, kLog2e);
+    if (lane < 16) sh[wave][n * 16 + lane] = st[n];
+  }
+  __syncthreads();
+  if (tid < tokens) {
+    SoftStat all = sh[0][tid];
+    for (int i = split; i < kFewWaves; i += split) all = join(all, sh[i][tid], kLog2e);
+    part[(size_t)blockIdx.x * tokens + tid] = all;
+  }
+}
+
 // Kept scores of one token: the parts that the product was cut into are added up in order, then
 // lse and loss (forward), then G (backward) in T; fp32 G takes the place of the scores, and so does bf16's unrounded G where
 // db needs its column sums.  A workgroup per token; the second walk over the row finds it in a cache.  HBM: 120 us for 2048
@@ -826,7 +1023,8 @@ static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow
       const double step = rounds * c.full[d] + (per_cu > 0 ? (last > c.alone[d] ? last : c.alone[d]) : 0.0);
       // (parts are written by the product and read by what joins them)
       const double work = step * idiv(steps, splits), bytes = ((double)M + N) * K * (d ? 2 : 4);
-      const double us = (work * kBytesPerUs > bytes ? work : bytes / kBytesPerUs) + kLaunchUs + c.finish * (rounds + (per_cu > 0 ? 1 : 0)) +
+      const double us = (work * kBytesPerUs > bytes ? work : bytes / kBytesPerUs) + kLaunchUs +
+                        c.finish * (rounds + (per_cu > 0 ? 1 : 0)) +
                         (may_split ? 2.0 * splits * M * (double)N * 4.0 / kBytesPerUs : 0.0);
       if (us < best.us) best = Choice{(ShapeId)s, splits, us};
     }
@@ -847,12 +1045,15 @@ struct VocabPlan {
   size_t el, ldx, ldw;
   int unit;            // elements of a 128-byte step
   bool packed;         // rows of x or w are no whole 16-byte chunks: those operands are copied
-  int piece, pieces;   // rows of w at a time
+  int piece;           // rows of w at a time
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, kept, dx, dw;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
   int stats_tiles;
+  int few_blocks;      // workgroups of a few tokens' forward pass (0: it takes the tiles)
+  FewShape few;
+  size_t few_lds;
   size_t part, label_score, xpack, wpack, scores, xl, wmax, g, slabs, db, total_forward, total;
 };
 
@@ -906,7 +1107,6 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     keep_any = keep_any || p.keep_forward || p.keep_backward[db] || p.keep_both[db];
   }
   if (keep_any) p.piece = vmax;
-  p.pieces = idiv(p.vocab, p.piece);
   p.vp = p.piece + p.unit;
   p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
   p.stats_tiles = 0;
@@ -919,13 +1119,31 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     at += align256(bytes);
     return here;
   };
-  p.part = take((size_t)p.stats_tiles * n * sizeof(SoftStat));
+  // a few tokens' forward pass: 16 rows a wave or shared by up to eight, so that about 2048 waves have work; as many
+  // workgroups as the chip holds at once.  x by panels from 16384 rows on: fewer leave compute units without a workgroup (64
+  // tokens of 1001 fp32: 45 us up to there, the tiles 23 us with 4001 rows and 47 us with 16001)
+  const int few_n = n <= 16 ? 1 : n <= 32 ? 2 : 4, few_steps = idiv(p.width, 64 / (int)p.el), few_tiles = idiv(p.vocab, 16);
+  FewShape &f = p.few;
+  f = FewShape{1, few_steps, 1};
+  while (f.split < kFewWaves && few_tiles * f.split < 2048 && few_steps >= 8 * f.split) f.split *= 2;
+  p.few_lds = (size_t)few_steps * few_n * 1024 + (f.split > 1 ? kFewWaves * few_n * 1024 : 0);
+  if (p.few_lds > (size_t)kFewLds) {
+    f = FewShape{1, kFewPanel / (few_n * 1024), max(1, min(kFewRows, few_tiles / (kFewWaves * 512)))};
+    p.few_lds = kFewPanel;
+  }
+  p.few_blocks = 0;
+  if (!whole_chunks(p.ldw, p.width, p.el) && p.tokens <= kFewTokens && p.width * p.el >= 16 && !tuning().vocab_tile &&
+      tuning().vocab_keep != 1 && (f.panel == few_steps || few_tiles >= 1024))
+    p.few_blocks = min(idiv(few_tiles, kFewWaves / f.split * f.rows),
+                       p.few_lds <= 36 << 10 ? 1024 : p.few_lds <= 72 << 10 ? 512 : 256);
+  p.part = take((size_t)max(p.stats_tiles, p.few_blocks) * n * sizeof(SoftStat));
   p.label_score = take(n * 4);
+  const size_t few_forward = at;
   p.xpack = take(p.packed ? n * p.hp * p.el : 0);
   p.wpack = take(p.packed ? (size_t)p.piece * p.hp * p.el : 0);
   const size_t score_space = (size_t)p.kept.splits * n * p.vp * 4;
   p.scores = take(p.keep_forward ? score_space : 0);
-  p.total_forward = at;
+  p.total_forward = p.few_blocks ? few_forward : at;
   if (!p.keep_forward) p.scores = take(keep_any ? score_space : 0);
   p.xl = take((p.el == 2 ? (size_t)p.width * p.np : n * p.hp) * p.el);
   p.wmax = take(4);
@@ -987,10 +1205,32 @@ struct VocabCall {
   bool forward, backward;
 };
 
+template <class T, int NT>
+static int vocab_few(const VocabPlan &p, const VocabCall &c) {
+  SoftStat *part = (SoftStat *)(c.ws + p.part);
+  float *label_score = (float *)(c.ws + p.label_score);
+  const bool panels = p.few.panel < idiv(p.width, 4 * Num<T>::V);
+  auto kern = panels ? vocab_few_kernel<T, NT, true> : vocab_few_kernel<T, NT, false>;
+  static LdsGrant grants[2];
+  if (int rc = grant_dynamic_lds((const void *)kern, kFewLds, grants[panels])) return rc;
+  kern<<<p.few_blocks, kFewWaves * 64, p.few_lds, ctx().stream>>>(part, label_score, (const T *)c.x, (const T *)c.w,
+                                                                 (const T *)c.bias, c.labels, p.ldx, p.ldw, p.tokens,
+                                                                 p.width, p.vocab, p.few);
+  CCT_LAUNCH_CHECK();
+  note_kernel("vocab_few_kernel<%s, %d, %s> split=%d rows=%d", Num<T>::NAME, NT, panels ? "true" : "false", p.few.split,
+              p.few.rows);
+  vocab_loss_kernel<1><<<p.tokens, 256, 0, ctx().stream>>>(c.loss, c.lse, part, label_score, c.labels, p.tokens,
+                                                          p.few_blocks, p.vocab, c.ignore);
+  CCT_LAUNCH_CHECK();
+  return 0;
+}
+
 template <class T>
 static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   hipStream_t st = ctx().stream;
   const int n = p.tokens;
+  if (!c.backward && p.few_blocks)
+    return n <= 16 ? vocab_few<T, 1>(p, c) : n <= 32 ? vocab_few<T, 2>(p, c) : vocab_few<T, 4>(p, c);
   const int db = c.db ? 1 : 0;
   const bool keep = c.forward && c.backward ? p.keep_both[db] : c.forward ? p.keep_forward : p.keep_backward[db];
   SoftStat *part = (SoftStat *)(c.ws + p.part);

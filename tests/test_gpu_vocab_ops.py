@@ -313,6 +313,60 @@ def test_vocab_loss(dtype, tokens, width, vocab):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("tokens", [1, 2, 15, 16, 17, 33, 64, 65])
+@pytest.mark.parametrize("width, vocab, gap", [(1, 2, 0), (7, 5, 1), (119, 4099, 0), (128, 1023, 3), (130, 3, 8), (257, 70001, 0),
+                                               (520, 1500, 1), (1030, 801, 5), (4096, 66, 0), (9000, 130, 0)])
+def test_vocab_loss_of_a_few_tokens(dtype, tokens, width, vocab, gap):
+    """The loss alone, of as few tokens as have a kernel of their own and of one more: whole and ragged rows, one to many
+    sets of rows for each wave, waves that share rows, x of more than the shared memory's share."""
+    v = Vocab(dtype, tokens, width, vocab, bias=(tokens + vocab) % 2 == 0, gap=gap, peaked=tokens == 15).reference()
+    for piece in (0, 256):
+        v.outputs()
+        v.forward(piece)
+        v.check_loss()
+    half = vocab // 2
+    if v.b is not None:                                            # masked entries leave the others as they were
+        v.b[half + 1:] = float("-inf")
+        v.b64 = v.b.double().cpu().numpy()
+        v.labels = np.minimum(v.labels, half)
+        v.reference()
+        v.outputs()
+        v.forward()
+        v.check_loss()
+
+
+@pytest.mark.parametrize("dtype, tokens, width, vocab", [("f32", 2, 2311, 16400), ("f32", 20, 1201, 33001), ("bf16", 33, 1211, 66003),
+                                                         ("bf16", 64, 1155, 16385), ("f32", 64, 579, 131100)])
+def test_vocab_loss_of_a_few_tokens_by_panels_of_the_width(dtype, tokens, width, vocab):
+    """x of more than the shared memory's share, with rows enough that each panel is staged for more than one set of them."""
+    v = Vocab(dtype, tokens, width, vocab, bias=tokens != 20).reference()
+    v.outputs()
+    v.forward()
+    name = driver().lib.cct_hip_last_kernel().decode()
+    assert name.startswith("vocab_few_kernel<") and ", true>" in name and name.endswith("rows=%d" % max(1, vocab // 65536)), name
+    v.check_loss()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_vocab_loss_of_a_few_tokens_with_scores_that_do_not_exist(dtype):
+    """A fully masked vocabulary, a NaN in one token's states, a label outside: each stays with its own token."""
+    v = Vocab(dtype, 4, 40, 600, bias=True, ignore=-100)
+    v.labels[:] = [5, 600, 7, -100]
+    v.reference()
+    v.x[2, 3] = float("nan")
+    v.outputs()
+    v.forward()
+    lse, loss = values(v.o_lse), values(v.o_loss)
+    near(lse[[0, 1, 3]], v.lse[[0, 1, 3]], v.else_[[0, 1, 3]])
+    near(loss[[0]], v.loss[[0]], v.eloss[[0]])
+    assert np.isnan(lse[2]) and np.isnan(loss[[1, 2]]).all() and loss[3] == 0
+    v.b[:] = float("-inf")
+    v.outputs()
+    v.forward()
+    assert (values(v.o_lse)[[0, 1, 3]] == -np.inf).all() and np.isnan(values(v.o_loss)[[0, 1, 2]]).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("tokens, width, vocab, piece", [(4500, 72, 4600, 0), (2100, 520, 2300, 512), (700, 2304, 900, 0)])
 def test_vocab_loss_with_the_largest_tiles(dtype, tokens, width, vocab, piece):
     """Enough rows and columns for the 256 x 256 tiles, in every use of the product."""
