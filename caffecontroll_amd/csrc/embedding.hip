@@ -17,7 +17,8 @@ struct EmbShape {
   int tokens, width, vocab, padding;
   float scale;
   size_t table_stride, out_stride;
-  int stream;  // the result goes past the caches
+  int stream;      // the result goes past the caches
+  int clear_rows;  // the table is cleared row by row
 };
 // Results above this do not stay in the caches anyway (L2: 32 MB); written past them they leave them to the rows that are read
 // (65536 tokens of 2048 bf16: 77 instead of 92 us; the gradient of 131072 rows of 4096: 3 % less).
@@ -64,10 +65,12 @@ __device__ __forceinline__ uint32_t sort_key(int id, int padding, int vocab) {
 }
 
 // The table cleared by workgroups of 4 KB each, in address order (6.8 TB/s; with 32 KB a workgroup 5.1 TB/s for 1 GB), whose
-// stores are aligned whatever the width is; or by one row each where rows have gaps between them.
-static unsigned clear_blocks_of(const EmbShape &s, int vec) {
+// stores are aligned whatever the width is; or by rows, where they have gaps between them or the table is too long for that.
+constexpr size_t EMB_CLEAR_BLOCKS = (size_t)1 << 23;  // a launch has fewer than 2^32 lanes
+static unsigned clear_blocks_of(EmbShape &s, int vec) {
   const size_t dense = ((size_t)s.vocab * s.width + EMB_THREADS * vec - 1) / (EMB_THREADS * vec);
-  return s.table_stride == (size_t)s.width && dense < (1u << 23) ? (unsigned)dense : (unsigned)s.vocab;
+  s.clear_rows = s.table_stride != (size_t)s.width || dense > EMB_CLEAR_BLOCKS;
+  return (unsigned)(s.clear_rows ? min((size_t)s.vocab, EMB_CLEAR_BLOCKS) : dense);
 }
 template <class T>
 __device__ __forceinline__ void clear_block(T *__restrict__ dtable, const EmbShape &s, uint32_t block, uint32_t blocks) {
@@ -75,17 +78,20 @@ __device__ __forceinline__ void clear_block(T *__restrict__ dtable, const EmbSha
   float zero[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) zero[i] = 0.0f;
-  const bool rows = blocks == (uint32_t)s.vocab;
-  const size_t i = rows ? (size_t)block * s.table_stride : ((size_t)block * EMB_THREADS + threadIdx.x) * V;
-  const size_t end = rows ? i + s.width : (size_t)s.vocab * s.width;
-  const size_t step = EMB_THREADS * V;
-  for (size_t at = rows ? i + threadIdx.x * V : i; at < end; at += step) {
+  const auto clear = [&](T *at, int left) {
     if (s.stream)
-      store_vec_stream<T>(dtable + at, zero, 0, (int)min(end - at, (size_t)V));
+      store_vec_stream<T>(at, zero, 0, left);
     else
-      store_vec<T>(dtable + at, zero, 0, (int)min(end - at, (size_t)V));
-    if (!rows) break;
+      store_vec<T>(at, zero, 0, left);
+  };
+  if (!s.clear_rows) {
+    const size_t at = ((size_t)block * EMB_THREADS + threadIdx.x) * V, end = (size_t)s.vocab * s.width;
+    if (at < end) clear(dtable + at, (int)min(end - at, (size_t)V));
+    return;
   }
+  for (uint32_t v = block; v < (uint32_t)s.vocab; v += blocks)
+    for (int col = threadIdx.x * V; col < s.width; col += EMB_THREADS * V)
+      clear(dtable + (size_t)v * s.table_stride + col, s.width - col);
 }
 
 // Few tokens: a token's place is the number of tokens that come before it, counted directly.  All keys lie in LDS; 16 lanes
@@ -652,7 +658,7 @@ static EmbShape shape_of(const cct_embedding_args *a, int result_rows) {
   const bool stream = (size_t)result_rows * a->width * dtype_bytes(a->dtype) > EMB_STREAM_BYTES;
   return EmbShape{a->tokens, a->width, a->vocab, a->padding_id, a->scale,
                   a->table_stride ? a->table_stride : (size_t)a->width, a->out_stride ? a->out_stride : (size_t)a->width,
-                  stream ? 1 : 0};
+                  stream ? 1 : 0, 0};
 }
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -729,7 +735,7 @@ static int sort_tokens(char *ws, const EmbWorkspace &w, const int *ids, const Em
 }
 
 template <class T>
-static int embedding_backward(void *dtable, const void *dout, const int *ids, const EmbShape &s, int accumulate, char *ws,
+static int embedding_backward(void *dtable, const void *dout, const int *ids, EmbShape s, int accumulate, char *ws,
                               const EmbWorkspace &w) {
   hipStream_t st = ctx().stream;
   const int l = row_lanes_log2<T>(s.width, 8), rows = max(EMB_ROWS, EMB_THREADS >> l);

@@ -155,6 +155,25 @@ def test_embedding_backward(dtype, accumulate, tokens, width, vocab, kind):
         assert (got[:, :width][count == 0] == o64[count == 0]).all()
 
 
+@pytest.mark.parametrize("tokens", [100, 200, 9000])
+def test_embedding_backward_clears_more_rows_with_gaps_than_a_launch_has_workgroups(tokens):
+    import torch
+    from caffecontroll_amd.driver import embedding_args
+    drv, rng, vocab = driver(), np.random.default_rng(tokens), (1 << 24) + 77
+    ids = rng.permutation(vocab - 1)[:tokens]
+    ids[0] = vocab - 1
+    dout, d64 = up(rng.standard_normal((tokens, 1)))
+    table = blank((vocab, 2), fill=3.0)
+    args = embedding_args(tokens, 1, vocab, table_stride=2)
+    n = drv.embedding_workspace_bytes(args)
+    drv.embedding_backward(table, dout, ints(ids), args, space(n).ptr, n)
+    assert bool((table[:, 1] == 3.0).all())
+    at = torch.from_numpy(ids).cuda()
+    np.testing.assert_array_equal(values(table[at, 0]), d64[:, 0])     # one token a row, a scale of 1: exact
+    table[at, 0] = 0.0
+    assert int(torch.count_nonzero(table[:, 0])) == 0
+
+
 def test_embedding_backward_is_the_same_every_time_and_clears_without_tokens():
     import torch
     from caffecontroll_amd.driver import embedding_args
