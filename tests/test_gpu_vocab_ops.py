@@ -398,6 +398,23 @@ def test_vocab_loss_with_the_largest_tiles(dtype, tokens, width, vocab, piece):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("tokens, width, vocab, piece, gap", [(1023, 520, 17011, 0, 0), (600, 300, 30011, 0, 4), (257, 520, 34011, 30000, 0)])
+def test_vocab_loss_with_the_rows_past_whole_rounds_of_tiles(dtype, tokens, width, vocab, piece, gap):
+    """More tiles than the chip holds at once: the last rows take another tile, in the loss, in G with its column sums
+    and in dw."""
+    v = Vocab(dtype, tokens, width, vocab, bias=True, gap=gap).reference()
+    with tuning("vocab_keep", 2):
+        v.outputs()
+        v.forward(piece)
+        v.check_loss()
+        v.backward(piece)
+        v.check_gradients()
+        if gap:
+            import torch
+            assert bool(torch.isnan(v.o_dw[:, width:]).all()) and bool(torch.isnan(v.o_dx[:, width:]).all())
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("keep", [1, 2])
 @pytest.mark.parametrize("tokens, width, vocab", [(3, 8, 5), (100, 264, 700), (333, 77, 515), (70, 1048, 1030)])
