@@ -394,6 +394,51 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int fgroup = lane >> 4, frow = lane & 15;
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
+  // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from the
+  // accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A wavefront
+  // takes its own part of the stages, as many rows at a time as it holds; the 16-byte chunks lie swizzled by the row.  (fp32
+  // stores have 16 bytes a lane as it is: no gain.)
+  const auto store_rows = [&](bf16 *C, size_t ld, int cols) {
+    typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    typedef Num<bf16>::vec chunk_any;
+    constexpr int ROW = MI * 16, CR = ROW / 8, ROWBYTES = ROW * 2;
+    constexpr int AREA = S::STAGES * S::STAGE / S::WAVES, FIT = AREA / (16 * ROWBYTES), JP = FIT < NI ? FIT : NI;
+    static_assert(JP >= 1 && NI % JP == 0 && 64 % CR == 0, "a wavefront's rows have to fit its part of the stages");
+    const auto swizzle = [](int row) { return CR >= 16 ? row & 15 : (row & 15) / (16 / CR); };
+    lds_char *area = (lds_char *)lds + wave * AREA;
+    const int c = lane % CR, m = m0 + wm * ROW + c * 8, left = cols - m;
+#pragma unroll
+    for (int j0 = 0; j0 < NI; j0 += JP) {
+#pragma unroll
+      for (int j = j0; j < j0 + JP; ++j)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int chunk = (2 * i + fgroup / 2) ^ swizzle(frow);
+          bf16x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (bf16)acc[i][j][r];
+          const int at = ((j - j0) * 16 + frow) * ROWBYTES + chunk * 16 + fgroup % 2 * 8;
+          *(__attribute__((address_space(3))) bf16x4 *)(area + at) = v;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+      for (int r = lane / CR; r < JP * 16; r += 64 / CR) {
+        const int n = n0 + (wn * NI + j0) * 16 + r;
+        const bf16x8 v = *(__attribute__((address_space(3))) bf16x8 *)(area + r * ROWBYTES + (c ^ swizzle(r)) * 16);
+        if (n >= p.N || left <= 0) continue;
+        bf16 *to = C + (size_t)n * ld + m;
+        if (left >= 8) {
+          *(chunk_any *)to = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) to[e] = v[e];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  };
+
   if constexpr (USE == USE_STATS || USE == USE_GRAD) {
     __syncthreads();  // the stages are done with
     if (p.bias) {
@@ -471,8 +516,12 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
           g[r] = grad_entry(acc[i][j][r], tg, at == i * 16 + r);
           acc[i][j][r] = g[r];
         }
-        if (t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g, 4);
+        if (sizeof(T) == 4 && t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g, 4);
       }
+    }
+    if constexpr (sizeof(T) == 2) {
+      store_rows((T *)p.g, p.ldg, p.mpad);
+      __syncthreads();
     }
     if (p.db_part) {
 #pragma unroll
@@ -499,22 +548,35 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   if constexpr (USE == USE_SLAB || USE == USE_OUT) {
     typedef typename std::conditional<USE == USE_SLAB, float, T>::type Out;
     const float scale = USE == USE_OUT && p.wmax ? *p.wmax : 1.0f;
+    if constexpr (USE == USE_OUT) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = ncol + j * 16;
-      if (n >= p.N) continue;
-      Out *row = (Out *)p.C + (USE == USE_SLAB ? ((size_t)split * p.N + n) * p.ldc : (size_t)n * p.ldc);
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int m = mrow + i * 16, left = p.M - m;
-        if (left <= 0) continue;
-        float f[4];
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          f[r] = USE == USE_OUT ? acc[i][j][r] * scale : acc[i][j][r];
-          if (USE == USE_SLAB && p.accumulate && r < left) f[r] += (float)row[m + r];
+          for (int r = 0; r < 4; ++r) acc[i][j][r] *= scale;
+    }
+    if constexpr (sizeof(Out) == 2) {
+      __syncthreads();  // the stages are done with
+      store_rows((Out *)p.C, p.ldc, p.M);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int n = ncol + j * 16;
+        if (n >= p.N) continue;
+        Out *row = (Out *)p.C + (USE == USE_SLAB ? ((size_t)split * p.N + n) * p.ldc : (size_t)n * p.ldc);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int m = mrow + i * 16, left = p.M - m;
+          if (left <= 0) continue;
+          float f[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f[r] = acc[i][j][r];
+            if (USE == USE_SLAB && p.accumulate && r < left) f[r] += (float)row[m + r];
+          }
+          store4<Out>(row + m, f, left);
         }
-        store4<Out>(row + m, f, left);
       }
     }
   }
@@ -1005,19 +1067,25 @@ struct Choice {
   int splits;
   double us;
 };
-static double shape_us(int shape, int splits, int M, int N, int K, int dtype, bool may_split) {
+enum ProductKind { REDUCED, PARTS, ROWS };  // scores that stay inside, fp32 parts along k, rows of dw
+static double shape_us(int shape, int splits, int M, int N, int K, int dtype, ProductKind kind) {
   const int d = dtype == CCT_BF16 ? 1 : 0, steps = idiv(K, d ? 64 : 32);
   const TileCost &c = kTiles[shape];
   const double w = (double)idiv(M, c.bm) * idiv(N > 0 ? N : 1, c.bn) * splits, round = 256.0 * c.occ;
   const double rounds = (double)(long)(w / round), per_cu = (double)(long)((w - rounds * round + 255.0) / 256.0);
   const double last = per_cu * c.full[d] / c.occ;
   const double step = rounds * c.full[d] + (per_cu > 0 ? (last > c.alone[d] ? last : c.alone[d]) : 0.0);
-  // (parts are written by the product and read by what joins them)
-  const double work = step * idiv(steps, splits), bytes = ((double)M + N) * K * (d ? 2 : 4);
-  return (work * kBytesPerUs > bytes ? work : bytes / kBytesPerUs) + kLaunchUs + c.finish * (rounds + (per_cu > 0 ? 1 : 0)) +
-         (may_split ? 2.0 * splits * M * (double)N * 4.0 / kBytesPerUs : 0.0);
+  const double el = d ? 2 : 4, in_us = ((double)M + N) * K * el / kBytesPerUs, out = (double)M * N;
+  const double work = step * idiv(steps, splits), ends = c.finish * (rounds + (per_cu > 0 ? 1 : 0));
+  const double us = kLaunchUs + (work > in_us ? work : in_us) + ends;
+  // parts are written by the product and read by what joins them
+  if (kind == PARTS) return us + 2.0 * splits * out * 4.0 / kBytesPerUs;
+  // rows are written while others are computed, or bound the launch
+  const double rows_us = kLaunchUs + in_us + out * el / kBytesPerUs;
+  return kind == ROWS && rows_us > us ? rows_us : us;
 }
-static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow) {
+static Choice choose(int M, int N, int K, int dtype, ProductKind kind) {
+  const bool narrow = kind != ROWS;  // an operand that is contiguous along its rows needs 64 of them
   const int steps = idiv(K, dtype == CCT_BF16 ? 64 : 32);
   const int pinned = tuning().vocab_tile >= 1 && tuning().vocab_tile <= SHAPES ? tuning().vocab_tile : 0;
   Choice best{SHAPE_M, 1, 1e30};
@@ -1025,8 +1093,8 @@ static Choice choose(int M, int N, int K, int dtype, bool may_split, bool narrow
     if (s >= SHAPE_S && !narrow) continue;
     if (pinned && s != (pinned > SHAPE_S && !narrow ? (int)SHAPE_N : pinned - 1)) continue;
     for (int splits = 1; splits <= 64; splits *= 2) {
-      if (splits > 1 && (!may_split || steps < 4 * splits)) break;
-      const double us = shape_us(s, splits, M, N, K, dtype, may_split);
+      if (splits > 1 && (kind != PARTS || steps < 4 * splits)) break;
+      const double us = shape_us(s, splits, M, N, K, dtype, kind);
       if (us < best.us) best = Choice{(ShapeId)s, splits, us};
     }
   }
@@ -1048,10 +1116,10 @@ static Cut cut_rows(const Choice &c, int rows, int other, int K, int dtype, bool
   const long blocks = (rows + block - 1) / block, rounds = blocks * per / round, main = rounds * round / per * block;
   if (main == 0 || main >= rows) return whole;
   const auto us = [&](int n) {
-    return across ? shape_us(c.shape, 1, other, n, K, dtype, false) : shape_us(c.shape, 1, n, other, K, dtype, false);
+    return across ? shape_us(c.shape, 1, other, n, K, dtype, ROWS) : shape_us(c.shape, 1, n, other, K, dtype, REDUCED);
   };
   const int left = rows - (int)main;
-  const Choice rest = across ? choose(other, left, K, dtype, false, false) : choose(left, other, K, dtype, false, true);
+  const Choice rest = across ? choose(other, left, K, dtype, ROWS) : choose(left, other, K, dtype, REDUCED);
   return us((int)main) + rest.us < us(rows) ? Cut{(int)main, rest} : whole;
 }
 
@@ -1112,8 +1180,8 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   // kept scores: all of the vocabulary at once, and so its packed copy
   const bool may_keep = (size_t)vmax <= most && (a->piece <= 0 || p.piece == vmax) &&
                         (!p.packed || (size_t)vmax * p.hp * p.el <= kPieceBytes);
-  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
-  p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, true, true);
+  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, PARTS);
   const double score_bytes = (double)n * vmax * 4;
   const double stats_us = p.stats.us * idiv(p.vocab, p.piece) + kLaunchUs;
   // (the choice's own cost has the scores written and read once; G is written on top, in place of the scores in fp32)
@@ -1131,15 +1199,15 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   }
   if (keep_any) p.piece = vmax;
   p.vp = p.piece + p.unit;
-  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, false, true);
+  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
   p.stats_tiles = 0;
   for (int v = 0; v < p.vocab; v += p.piece) {
     const int rows = min(p.piece, p.vocab - v);
     const Cut cut = cut_rows(p.stats, rows, p.tokens, p.width, p.dtype, false);
     p.stats_tiles += idiv(cut.main, kTiles[p.stats.shape].bm) + idiv(rows - cut.main, kTiles[cut.rest.shape].bm);
   }
-  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, true, true);
-  p.dw = choose(p.width, p.piece, p.tokens, p.dtype, false, false);
+  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, PARTS);
+  p.dw = choose(p.width, p.piece, p.tokens, p.dtype, ROWS);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
