@@ -192,6 +192,9 @@ struct ProductArgs {
   void *C;
   size_t ldc;
   int accumulate;
+  // OUT: rows are whole cache lines, written past the caches (512 tokens, 32000 rows of 2048 bf16: 80 -> 74 us; rows of 776,
+  // whose lines are written in parts: 37 -> 44)
+  int stream;
 };
 
 __device__ __forceinline__ f32x4 mfma_bf16(const f32x4 &a, const f32x4 &b, const f32x4 &c) {
@@ -394,10 +397,10 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int fgroup = lane >> 4, frow = lane & 15;
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
-  // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from the
-  // accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A wavefront
-  // takes its own part of the stages, as many rows at a time as it holds; the 16-byte chunks lie swizzled by the row.  (fp32
-  // stores have 16 bytes a lane as it is: no gain.)
+  // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from
+  // the accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A
+  // wavefront takes its own part of the stages, as many rows at a time as it holds; the 16-byte chunks lie swizzled by the
+  // row.  (fp32 stores have 16 bytes a lane as it is: no gain.)
   const auto store_rows = [&](bf16 *C, size_t ld, int cols) {
     typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
     typedef Num<bf16>::vec chunk_any;
@@ -428,7 +431,10 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
         if (n >= p.N || left <= 0) continue;
         bf16 *to = C + (size_t)n * ld + m;
         if (left >= 8) {
-          *(chunk_any *)to = v;
+          if (USE == USE_OUT && p.stream)
+            __builtin_nontemporal_store((chunk_any)v, (chunk_any *)to);
+          else
+            *(chunk_any *)to = v;
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -654,12 +660,16 @@ __global__ __launch_bounds__(256) void vocab_xt_kernel(T *__restrict__ xt, const
   }
   const int t0 = (int)(blockIdx.x % tiles_t) * 64, c0 = (int)(blockIdx.x / tiles_t) * 64;
   const int lane = threadIdx.x & 63, y = threadIdx.x >> 6;
+  int label[16];
+  T v[16];
+  const int c = min(c0 + lane, width - 1);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int t = t0 + y + i * 4, c = c0 + lane;
-    const bool in = t < tokens && c < width && labels[t] != ignore;
-    tile[y + i * 4][lane] = in ? x[(size_t)t * ldx + c] : (T)0.0f;
-  }
+  for (int i = 0; i < 16; ++i) label[i] = labels[min(t0 + y + i * 4, tokens - 1)];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = x[(size_t)min(t0 + y + i * 4, tokens - 1) * ldx + c];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    tile[y + i * 4][lane] = t0 + y + i * 4 < tokens && c0 + lane < width && label[i] != ignore ? v[i] : (T)0.0f;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -905,79 +915,144 @@ __global__ __launch_bounds__(kFewWaves * 64) void vocab_few_kernel(SoftStat *__r
   }
 }
 
-// Kept scores of one token: the parts that the product was cut into are added up in order, then
-// lse and loss (forward), then G (backward) in T; fp32 G takes the place of the scores, and so does bf16's unrounded G where
-// db needs its column sums.  A workgroup per token; the second walk over the row finds it in a cache.  HBM: 120 us for 2048
-// tokens and 32768 rows of fp32 (537 MB, 4.5 TB/s).
+// Kept scores of a token: the parts that the product was cut into are added up in order, then lse and loss (forward),
+// then G (backward) in T; fp32 G takes the place of the scores, and so does bf16's unrounded G where db needs its column
+// sums.  ld is a multiple of four and rows start at 16-byte boundaries.
+constexpr int kRowThreads = 512;
+struct RowArgs {
+  float *scores;
+  const void *bias;
+  const int *labels;
+  const float *weight, *wmax;
+  int tokens, vocab, splits, ignore, mpad, keep_g;
+  size_t ld;
+};
 template <class T>
-__global__ __launch_bounds__(512) void vocab_row_kernel(float *__restrict__ loss, float *__restrict__ lse_out,
-                                                        const float *__restrict__ lse_in, T *__restrict__ g,
-                                                        float *__restrict__ scores, const T *__restrict__ bias,
-                                                        const int *__restrict__ labels, const float *__restrict__ weight,
-                                                        const float *__restrict__ wmax, int tokens, int vocab, int splits,
-                                                        size_t ld, int ignore, int mpad, int keep_g) {
-  __shared__ SoftStat sh[8];
-  __shared__ float lse_sh;
-  const int t = blockIdx.x, tid = threadIdx.x;
-  float *row = scores + (size_t)t * ld;
-  const size_t part = (size_t)tokens * ld;
-  const int label = labels[t];
-  auto add_bias = [&](f32x4 &v, int c) {
+__device__ __forceinline__ void add_bias(f32x4 &v, const RowArgs &p, int c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < vocab) v[i] += (float)bias[c + i];
-  };
+  for (int i = 0; i < 4; ++i)
+    if (c + i < p.vocab) v[i] += (float)((const T *)p.bias)[c + i];
+}
+// The sums over [begin, end) of a row, and if asked for their statistics, by a workgroup: its first lane has them.
+template <class T>
+__device__ __forceinline__ SoftStat row_stats(float *__restrict__ row, const RowArgs &p, int begin, int end, bool stats) {
+  __shared__ SoftStat sh[kRowThreads / 64];
+  const int tid = threadIdx.x;
+  const size_t part = (size_t)p.tokens * p.ld;
   SoftStat st{neg_inf(), 0.0f};
-  // ld is a multiple of four and rows start at 16-byte boundaries
-  for (int c = tid * 4; c < vocab && (loss || splits > 1); c += 512 * 4) {
+  for (int c = begin + tid * 4; c < end; c += kRowThreads * 4) {
     f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
-    if (splits > 1) {
-      for (int i = 1; i < splits; ++i) v += *reinterpret_cast<const f32x4 *>(row + i * part + c);
+    if (p.splits > 1) {
+      for (int i = 1; i < p.splits; ++i) v += *reinterpret_cast<const f32x4 *>(row + i * part + c);
       *reinterpret_cast<f32x4 *>(row + c) = v;
     }
-    if (bias) add_bias(v, c);
-    if (loss) {
-      float m = st.m;
+    if (!stats) continue;
+    if (p.bias) add_bias<T>(v, p, c);
+    float m = st.m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = c + i < vocab ? v[i] : neg_inf();
-        m = fmaxf(m, v[i]);
-      }
-      const float base = m == neg_inf() ? 0.0f : m;
-      float s = st.s * (st.m == m ? 1.0f : exp2_fast((st.m - base) * kLog2e));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s += exp2_fast((v[i] - base) * kLog2e);
-      st = SoftStat{m, s};
+    for (int i = 0; i < 4; ++i) {
+      v[i] = c + i < p.vocab ? v[i] : neg_inf();
+      m = fmaxf(m, v[i]);
     }
+    const float base = m == neg_inf() ? 0.0f : m;
+    float s = st.s * (st.m == m ? 1.0f : exp2_fast((st.m - base) * kLog2e));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += exp2_fast((v[i] - base) * kLog2e);
+    st = SoftStat{m, s};
   }
-  if (loss) {
+  if (stats) {
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) st = shfl_xor_join(st, m, kLog2e);
     if ((tid & 63) == 0) sh[tid >> 6] = st;
-    __syncthreads();  // (also: this row's sums are written)
+    __syncthreads();  // (also: these sums are written)
     if (tid == 0) {
 #pragma unroll
-      for (int i = 1; i < 8; ++i) st = join(st, sh[i], kLog2e);
-      const float l = log_sum(st, 1.0f);
-      lse_sh = l;
-      const bool in = (unsigned)label < (unsigned)vocab;
-      store_loss(loss, lse_out, t, l, label, in ? row[label] + (bias ? (float)bias[label] : 0.0f) : 0.0f, vocab, ignore);
+      for (int i = 1; i < kRowThreads / 64; ++i) st = join(st, sh[i], kLog2e);
     }
-  } else if (tid == 0) {
-    lse_sh = lse_in[t];
   }
-  if (!g) return;
-  __syncthreads();
-  TokenGrad tg = token_grad(0, 1, labels + t, ignore, &lse_sh, weight ? weight + t : nullptr, wmax);
-  for (int c = tid * 4; c < mpad; c += 512 * 4) {
+  return st;
+}
+template <class T>
+__device__ __forceinline__ float row_score(const float *__restrict__ row, const RowArgs &p, int label) {
+  return row[label] + (p.bias ? (float)((const T *)p.bias)[label] : 0.0f);
+}
+// G over [begin, end) of a row
+template <class T>
+__device__ __forceinline__ void row_grad(T *__restrict__ g, float *__restrict__ row, const RowArgs &p, int t, float lse,
+                                         int begin, int end) {
+  const TokenGrad tg = token_grad(0, 1, p.labels + t, p.ignore, &lse, p.weight ? p.weight + t : nullptr, p.wmax);
+  for (int c = begin + threadIdx.x * 4; c < end; c += kRowThreads * 4) {
     float f[4];
     f32x4 v = *reinterpret_cast<const f32x4 *>(row + c);
-    if (bias) add_bias(v, c);
+    if (p.bias) add_bias<T>(v, p, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = c + i < vocab ? grad_entry(v[i], tg, c + i == label) : 0.0f;
-    if (keep_g || std::is_same<T, float>::value) *reinterpret_cast<f32x4 *>(row + c) = f32x4{f[0], f[1], f[2], f[3]};
-    if (!std::is_same<T, float>::value) store4<T>(g + (size_t)t * ld + c, f, 4);
+    for (int i = 0; i < 4; ++i) f[i] = c + i < p.vocab ? grad_entry(v[i], tg, c + i == tg.label) : 0.0f;
+    if (p.keep_g || std::is_same<T, float>::value) *reinterpret_cast<f32x4 *>(row + c) = f32x4{f[0], f[1], f[2], f[3]};
+    if (!std::is_same<T, float>::value) store4<T>(g + (size_t)t * p.ld + c, f, 4);
   }
+}
+
+// A workgroup per token; the second walk over the row finds it in a cache.  HBM: 120 us for 2048 tokens and 32768 rows of
+// fp32 (537 MB, 4.5 TB/s).
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void vocab_row_kernel(float *__restrict__ loss, float *__restrict__ lse_out,
+                                                                const float *__restrict__ lse_in, T *__restrict__ g,
+                                                                RowArgs p) {
+  __shared__ float lse_sh;
+  const int t = blockIdx.x;
+  float *row = p.scores + (size_t)t * p.ld;
+  if (loss || p.splits > 1) {
+    const SoftStat st = row_stats<T>(row, p, 0, p.vocab, loss != nullptr);
+    if (loss && threadIdx.x == 0) {
+      const int label = p.labels[t];
+      lse_sh = log_sum(st, 1.0f);
+      store_loss(loss, lse_out, t, lse_sh, label, (unsigned)label < (unsigned)p.vocab ? row_score<T>(row, p, label) : 0.0f,
+                 p.vocab, p.ignore);
+    }
+  }
+  if (!loss && threadIdx.x == 0) lse_sh = lse_in[t];
+  if (!g) return;
+  __syncthreads();
+  row_grad<T>(g, row, p, t, lse_sh, 0, p.mpad);
+}
+
+// The same for few tokens with long rows, each cut into ranges of `len`: statistics of the ranges, then G, whose workgroups
+// join the ranges for themselves (8 tokens, 50000 rows of bf16: 10 us, with a workgroup a token 38).
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void vocab_range_stats_kernel(SoftStat *__restrict__ part,
+                                                                        float *__restrict__ label_score, RowArgs p, int len) {
+  const int t = blockIdx.y, begin = (int)blockIdx.x * len, end = min(p.vocab, begin + len);
+  float *row = p.scores + (size_t)t * p.ld;
+  const SoftStat st = row_stats<T>(row, p, begin, end, part != nullptr);
+  if (!part || threadIdx.x != 0) return;
+  part[(size_t)blockIdx.x * p.tokens + t] = st;
+  const int label = p.labels[t];
+  if (label >= begin && label < end) label_score[t] = row_score<T>(row, p, label);
+}
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void vocab_range_grad_kernel(float *__restrict__ loss, float *__restrict__ lse_out,
+                                                                       const float *__restrict__ lse_in,
+                                                                       const SoftStat *__restrict__ part,
+                                                                       const float *__restrict__ label_score,
+                                                                       T *__restrict__ g, RowArgs p, int len) {
+  __shared__ float lse_sh;
+  const int t = blockIdx.y, begin = (int)blockIdx.x * len;
+  const int end = blockIdx.x + 1 == gridDim.x ? p.mpad : begin + len;
+  if (loss) {
+    if (threadIdx.x < 64) {
+      SoftStat st = threadIdx.x < gridDim.x ? part[(size_t)threadIdx.x * p.tokens + t] : SoftStat{neg_inf(), 0.0f};
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) st = shfl_xor_join(st, m, kLog2e);
+      if (threadIdx.x == 0) {
+        lse_sh = log_sum(st, 1.0f);
+        if (blockIdx.x == 0) store_loss(loss, lse_out, t, lse_sh, p.labels[t], label_score[t], p.vocab, p.ignore);
+      }
+    }
+  } else if (threadIdx.x == 0) {
+    lse_sh = lse_in[t];
+  }
+  __syncthreads();
+  row_grad<T>(g, p.scores + (size_t)t * p.ld, p, t, lse_sh, begin, end);
 }
 
 // db = *wmax times the column sums of kept G: 64 columns a workgroup, its 16 wavefronts taking every 16th token each (576
@@ -1142,6 +1217,7 @@ struct VocabPlan {
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
   int stats_tiles;
+  int ranges, range;   // a token's kept scores are cut into so many ranges of so many
   int few_blocks;      // workgroups of a few tokens' forward pass (0: it takes the tiles)
   FewShape few;
   size_t few_lds;
@@ -1231,7 +1307,12 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
       tuning().vocab_keep != 1 && (f.panel == few_steps || few_tiles >= 1024))
     p.few_blocks = min(idiv(few_tiles, kFewWaves / f.split * f.rows),
                        p.few_lds <= 36 << 10 ? 1024 : p.few_lds <= 72 << 10 ? 512 : 256);
-  p.part = take((size_t)max(p.stats_tiles, p.few_blocks) * n * sizeof(SoftStat));
+  // ranges of a token's kept scores: about 1024 workgroups, of 4096 scores or more, where a token would have four or more
+  p.ranges = min(min(1024 / max(p.tokens, 1), p.vocab / 4096), 64);
+  if (p.ranges < 4) p.ranges = 1;
+  p.range = idiv(idiv(p.vocab, p.ranges), 64) * 64;
+  p.ranges = idiv(p.vocab, p.range);
+  p.part = take((size_t)max(max(p.stats_tiles, p.few_blocks), p.ranges) * n * sizeof(SoftStat));
   p.label_score = take(n * 4);
   const size_t few_forward = at;
   p.xpack = take(p.packed ? n * p.hp * p.el : 0);
@@ -1394,9 +1475,23 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     a.C = scores;
     a.ldc = p.vp;
     if (int rc = product<T, USE_SLAB, true, true>(p.kept, a)) return rc;
-    vocab_row_kernel<T><<<n, 512, 0, st>>>(c.forward ? c.loss : nullptr, c.lse, c.lse_in, c.backward ? g : nullptr, scores,
-                                          (const T *)c.bias, c.labels, c.weight, wmax, n, p.vocab, p.kept.splits, p.vp,
-                                          c.ignore, idiv(p.vocab, chunk) * chunk, c.db ? 1 : 0);
+    RowArgs r{scores, c.bias, c.labels, c.weight, wmax, n, p.vocab, p.kept.splits, c.ignore, idiv(p.vocab, chunk) * chunk,
+              c.db ? 1 : 0, (size_t)p.vp};
+    if (p.ranges > 1) {
+      const dim3 grid(p.ranges, n);
+      if (c.forward || r.splits > 1) {
+        vocab_range_stats_kernel<T><<<grid, kRowThreads, 0, st>>>(c.forward ? part : nullptr, label_score, r, p.range);
+        CCT_LAUNCH_CHECK();
+      }
+      if (c.backward)
+        vocab_range_grad_kernel<T><<<grid, kRowThreads, 0, st>>>(c.forward ? c.loss : nullptr, c.lse, c.lse_in, part,
+                                                                label_score, g, r, p.range);
+      else
+        vocab_loss_kernel<1><<<n, 256, 0, st>>>(c.loss, c.lse, part, label_score, c.labels, n, p.ranges, p.vocab, c.ignore);
+    } else {
+      vocab_row_kernel<T><<<n, kRowThreads, 0, st>>>(c.forward ? c.loss : nullptr, c.lse, c.lse_in, c.backward ? g : nullptr,
+                                                    r);
+    }
     CCT_LAUNCH_CHECK();
     if (c.db) {
       vocab_colsum_kernel<T><<<idiv(p.vocab, 64), 1024, 0, st>>>((T *)c.db, scores, p.vp, wmax, n, p.vocab);
@@ -1483,6 +1578,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
         a.wmax = wmax;
         a.C = (T *)c.dw + (size_t)(v0 + r0) * p.ldw;
         a.ldc = p.ldw;
+        a.stream = ((p.ldw * p.el | (uintptr_t)a.C) & 127) == 0;
         if (int rc = product<T, USE_OUT, kXt, false>(r0 == 0 ? p.dw : cut.rest, a)) return rc;
       }
     }

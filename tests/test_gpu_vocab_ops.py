@@ -415,6 +415,26 @@ def test_vocab_loss_with_the_rows_past_whole_rounds_of_tiles(dtype, tokens, widt
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("tokens, width, vocab", [(1, 33, 270001), (3, 2900, 17001), (100, 40, 33000), (256, 64, 16384)])
+def test_vocab_loss_with_kept_scores_cut_into_ranges(dtype, bias, tokens, width, vocab):
+    """Long rows of few tokens, with one part along the width and with several; labels in the first and the last range."""
+    v = Vocab(dtype, tokens, width, vocab, bias=bias, peaked=tokens == 100)
+    v.labels[0], v.labels[-1] = vocab - 1, min(5, vocab - 1) if tokens > 1 else vocab - 1
+    v.reference()
+    with tuning("vocab_keep", 1):
+        v.outputs()
+        v.forward()
+        v.check_loss()
+        v.backward()
+        v.check_gradients()
+        v.outputs()
+        v.both()
+        v.check_loss()
+        v.check_gradients()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("keep", [1, 2])
 @pytest.mark.parametrize("tokens, width, vocab", [(3, 8, 5), (100, 264, 700), (333, 77, 515), (70, 1048, 1030)])
