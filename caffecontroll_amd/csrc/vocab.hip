@@ -1055,41 +1055,48 @@ __global__ __launch_bounds__(kRowThreads) void vocab_range_grad_kernel(float *__
   row_grad<T>(g, p.scores + (size_t)t * p.ld, p, t, lse_sh, begin, end);
 }
 
-// db = *wmax times the column sums of kept G: 64 columns a workgroup, its 16 wavefronts taking every 16th token each (576
-// tokens, 6400 rows: 5 us).
+// What is left behind the products, in one launch.  db = *wmax times the column sums of kept G: 64 columns a workgroup, its 16
+// wavefronts taking every 16th token each.  dx[t] = *wmax times the sum of the slabs, in order, four columns a lane.  HBM
+// (8192 x 4096 from one slab: 37 us, 5.4 TB/s) and the launch, which is why the two share it (256 tokens of 4096, 1000 rows of
+// fp32: 82 us a step with two launches, 80 with one).
+constexpr int kFinishThreads = 1024;
+struct FinishArgs {
+  const float *slabs, *g, *wmax;
+  int tokens, width, splits, db_blocks, rows, dx_lanes;
+  size_t ldx, ld, ldg;
+};
 template <class T>
-__global__ __launch_bounds__(1024) void vocab_colsum_kernel(T *__restrict__ db, const float *__restrict__ g, size_t ldg,
-                                                            const float *__restrict__ wmax, int tokens, int rows) {
+__global__ __launch_bounds__(kFinishThreads) void vocab_finish_kernel(T *__restrict__ dx, T *__restrict__ db, FinishArgs p) {
   __shared__ float sh[16][64];
-  const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, m = blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (m < rows) {
+  const float weight = p.wmax ? *p.wmax : 1.0f;
+  if ((int)blockIdx.x < p.db_blocks) {
+    const int lane = threadIdx.x & 63, y = threadIdx.x >> 6, m = blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (m < p.rows) {
 #pragma unroll 8
-    for (int t = y; t < tokens; t += 16) s += g[(size_t)t * ldg + m];
-  }
-  sh[y][lane] = s;
-  __syncthreads();
-  if (y == 0 && m < rows) {
+      for (int t = y; t < p.tokens; t += 16) s += p.g[(size_t)t * p.ldg + m];
+    }
+    sh[y][lane] = s;
+    __syncthreads();
+    if (y == 0 && m < p.rows) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += sh[i][lane];
-    db[m] = (T)(wmax ? s * *wmax : s);
+      for (int i = 1; i < 16; ++i) s += sh[i][lane];
+      db[m] = (T)(s * weight);
+    }
+    return;
   }
-}
-
-// dx[t] = *wmax times the sum of the slabs, in order (8192 x 4096 from one slab: 37 us, 5.4 TB/s).
-template <class T>
-__global__ __launch_bounds__(256) void vocab_dx_kernel(T *__restrict__ dx, const float *__restrict__ slabs,
-                                                       const float *__restrict__ wmax, int tokens, int width, size_t ldx,
-                                                       size_t ld, int splits) {
-  const int t = blockIdx.x;
-  const float weight = wmax ? *wmax : 1.0f;
-  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
-  if (c >= width) return;
-  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+  if ((int)threadIdx.x >= p.dx_lanes) return;
+  const unsigned vecs = (unsigned)(p.width + 3) / 4;
+  const size_t all = (size_t)p.tokens * vecs, stride = (size_t)(gridDim.x - p.db_blocks) * p.dx_lanes;
+  for (size_t i = (size_t)(blockIdx.x - p.db_blocks) * p.dx_lanes + threadIdx.x; i < all; i += stride) {
+    const size_t t = all >> 32 ? i / vecs : (unsigned)i / vecs;
+    const int c = (int)(i - t * vecs) * 4;
+    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4 *>(slabs + ((size_t)i * tokens + t) * ld + c);
-  const float f[4] = {s[0] * weight, s[1] * weight, s[2] * weight, s[3] * weight};
-  store4<T>(dx + (size_t)t * ldx + c, f, width - c);
+    for (int k = 0; k < p.splits; ++k) s += *reinterpret_cast<const f32x4 *>(p.slabs + ((size_t)k * p.tokens + t) * p.ld + c);
+    const float f[4] = {s[0] * weight, s[1] * weight, s[2] * weight, s[3] * weight};
+    store4<T>(dx + t * p.ldx + c, f, p.width - c);
+  }
 }
 
 template <class T>
@@ -1493,10 +1500,6 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
                                                     r);
     }
     CCT_LAUNCH_CHECK();
-    if (c.db) {
-      vocab_colsum_kernel<T><<<idiv(p.vocab, 64), 1024, 0, st>>>((T *)c.db, scores, p.vp, wmax, n, p.vocab);
-      CCT_LAUNCH_CHECK();
-    }
   } else if (c.forward) {
     int tiles = 0;
     for (int v0 = 0; v0 < p.vocab; v0 += p.piece) {
@@ -1583,9 +1586,16 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
       }
     }
   }
-  if (c.dx) {
-    vocab_dx_kernel<T><<<dim3(n, idiv(p.width, 1024)), 256, 0, st>>>((T *)c.dx, slabs, wmax, n, p.width, p.ldx, p.hp,
-                                                                    p.dx.splits);
+  const int db_blocks = keep && c.db ? idiv(p.vocab, 64) : 0;
+  // fewer lanes of a workgroup take part where that puts more of them to work (320 tokens of 200: 32 instead of 34 us with dx)
+  const size_t dx_vecs = c.dx ? (size_t)n * idiv(p.width, 4) : 0;
+  int dx_lanes = kFinishThreads;
+  while (dx_lanes > 64 && dx_vecs / dx_lanes < 512) dx_lanes /= 2;
+  const unsigned dx_blocks = (unsigned)min((dx_vecs + dx_lanes - 1) / dx_lanes, (size_t)1 << 21);
+  if (db_blocks + dx_blocks > 0) {
+    const FinishArgs f{slabs, scores, wmax, n, p.width, p.dx.splits, db_blocks, p.vocab, dx_lanes, p.ldx, (size_t)p.hp,
+                       (size_t)p.vp};
+    vocab_finish_kernel<T><<<db_blocks + dx_blocks, kFinishThreads, 0, st>>>((T *)c.dx, (T *)c.db, f);
     CCT_LAUNCH_CHECK();
   }
   return 0;
