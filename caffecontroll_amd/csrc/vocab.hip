@@ -1149,7 +1149,8 @@ struct Choice {
   int splits;
   double us;
 };
-enum ProductKind { REDUCED, PARTS, ROWS };  // scores that stay inside, fp32 parts along k, rows of dw
+// scores that stay inside; kept scores, fp32 parts along k; dx, the same with w read across its rows; rows of dw
+enum ProductKind { REDUCED, PARTS, TURNED, ROWS };
 static double shape_us(int shape, int splits, int M, int N, int K, int dtype, ProductKind kind) {
   const int d = dtype == CCT_BF16 ? 1 : 0, steps = idiv(K, d ? 64 : 32);
   const TileCost &c = kTiles[shape];
@@ -1157,11 +1158,15 @@ static double shape_us(int shape, int splits, int M, int N, int K, int dtype, Pr
   const double rounds = (double)(long)(w / round), per_cu = (double)(long)((w - rounds * round + 255.0) / 256.0);
   const double last = per_cu * c.full[d] / c.occ;
   const double step = rounds * c.full[d] + (per_cu > 0 ? (last > c.alone[d] ? last : c.alone[d]) : 0.0);
-  const double el = d ? 2 : 4, in_us = ((double)M + N) * K * el / kBytesPerUs, out = (double)M * N;
+  const double el = d ? 2 : 4, out = (double)M * N;
+  // across rows narrow tiles take pieces of 128 bytes, and tiles along n fetch them again, mostly from a cache (dx of 131072
+  // rows of 4096 bf16: 64 tokens 332 us with 64 x 32 and 264 with 128 x 128, 128 tokens 400 us with 64 x 64)
+  const double again = 1.0 + 0.2 * (idiv(N > 0 ? N : 1, c.bn) - 1), rate = c.bm >= 128 ? 4.1e6 : 3.5e6;
+  const double in_us = kind == TURNED ? ((double)M * again + N) * K * el / rate : ((double)M + N) * K * el / kBytesPerUs;
   const double work = step * idiv(steps, splits), ends = c.finish * (rounds + (per_cu > 0 ? 1 : 0));
   const double us = kLaunchUs + (work > in_us ? work : in_us) + ends;
   // parts are written by the product and read by what joins them
-  if (kind == PARTS) return us + 2.0 * splits * out * 4.0 / kBytesPerUs;
+  if (kind == PARTS || kind == TURNED) return us + 2.0 * splits * out * 4.0 / kBytesPerUs;
   // rows are written while others are computed, or bound the launch
   const double rows_us = kLaunchUs + in_us + out * el / kBytesPerUs;
   return kind == ROWS && rows_us > us ? rows_us : us;
@@ -1175,7 +1180,7 @@ static Choice choose(int M, int N, int K, int dtype, ProductKind kind) {
     if (s >= SHAPE_S && !narrow) continue;
     if (pinned && s != (pinned > SHAPE_S && !narrow ? (int)SHAPE_N : pinned - 1)) continue;
     for (int splits = 1; splits <= 64; splits *= 2) {
-      if (splits > 1 && (kind != PARTS || steps < 4 * splits)) break;
+      if (splits > 1 && ((kind != PARTS && kind != TURNED) || steps < 4 * splits)) break;
       const double us = shape_us(s, splits, M, N, K, dtype, kind);
       if (us < best.us) best = Choice{(ShapeId)s, splits, us};
     }
@@ -1202,7 +1207,8 @@ static Cut cut_rows(const Choice &c, int rows, int other, int K, int dtype, bool
   };
   const int left = rows - (int)main;
   const Choice rest = across ? choose(other, left, K, dtype, ROWS) : choose(left, other, K, dtype, REDUCED);
-  return us((int)main) + rest.us < us(rows) ? Cut{(int)main, rest} : whole;
+  // (2538 tokens of 824, 44875 rows, 6.9 rounds of tiles: no gain by this estimate, a step of 944 us instead of 890)
+  return us((int)main) + rest.us < 0.92 * us(rows) ? Cut{(int)main, rest} : whole;
 }
 
 constexpr size_t kKeepBytes = (size_t)512 << 20;   // fp32 scores that may be kept
@@ -1218,9 +1224,9 @@ struct VocabPlan {
   size_t el, ldx, ldw;
   int unit;            // elements of a 128-byte step
   bool packed;         // rows of x or w are no whole 16-byte chunks: those operands are copied
-  int piece;           // rows of w at a time
+  int piece, loss_piece;  // rows of w at a time; for the loss alone, which keeps nothing of them
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
-  Choice stats, kept, dx, dw;
+  Choice stats, grad, kept, dx, dw;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
   int stats_tiles;
@@ -1253,20 +1259,24 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   if (a->piece > 0) {
     p.piece = (int)min((((size_t)a->piece + 255) / 256) * 256, most);
   } else {
-    // a power of two, so that the tiles of a piece fill whole rounds of the chip
+    // all of the vocabulary, or a power of two, so that the tiles of a piece fill whole rounds of the chip
     const size_t row = (n + p.hp) * p.el, want = kPieceBytes / row;
     size_t rows = 1024;
     while (rows * 2 <= want && rows < (size_t)vmax) rows *= 2;
+    if ((size_t)vmax <= want) rows = vmax;
     p.piece = (int)min(rows, most);
   }
   if (p.piece > vmax) p.piece = vmax;
   // kept scores: all of the vocabulary at once, and so its packed copy
   const bool may_keep = (size_t)vmax <= most && (a->piece <= 0 || p.piece == vmax) &&
                         (!p.packed || (size_t)vmax * p.hp * p.el <= kPieceBytes);
-  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.loss_piece = a->piece > 0 || p.packed ? p.piece : (int)min((size_t)vmax, most);
+  p.stats = choose(min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.grad = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
   p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, PARTS);
   const double score_bytes = (double)n * vmax * 4;
-  const double stats_us = p.stats.us * idiv(p.vocab, p.piece) + kLaunchUs;
+  const double stats_us = p.stats.us * idiv(p.vocab, p.loss_piece) + kLaunchUs;
+  const double grad_scores_us = p.grad.us * idiv(p.vocab, p.piece) + kLaunchUs;
   // (the choice's own cost has the scores written and read once; G is written on top, in place of the scores in fp32)
   const double join_us = kLaunchUs, grad_us = (double)n * vmax * p.el / kBytesPerUs;
   const bool fits = may_keep && score_bytes * p.kept.splits <= (double)kKeepBytes;
@@ -1275,21 +1285,22 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   for (int db = 0; db < 2; ++db) {
     // the column sums read the kept G (in bf16 it is written in fp32 for them), those of a GRAD product come with it
     const double db_us = db ? kLaunchUs + score_bytes * (p.el == 4 ? 1 : 2) / kBytesPerUs : 0.0;
-    p.keep_backward[db] = fits && p.kept.us + join_us + grad_us + db_us < stats_us;
-    p.keep_both[db] = fits && p.kept.us + join_us + grad_us + db_us < 2 * stats_us;
+    p.keep_backward[db] = fits && p.kept.us + join_us + grad_us + db_us < grad_scores_us;
+    p.keep_both[db] = fits && p.kept.us + join_us + grad_us + db_us < stats_us + grad_scores_us;
     if (tuning().vocab_keep) p.keep_forward = p.keep_backward[db] = p.keep_both[db] = fits && tuning().vocab_keep == 1;
     keep_any = keep_any || p.keep_forward || p.keep_backward[db] || p.keep_both[db];
   }
-  if (keep_any) p.piece = vmax;
+  if (keep_any) p.piece = p.loss_piece = vmax;
   p.vp = p.piece + p.unit;
-  p.stats = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.stats = choose(min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.grad = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
   p.stats_tiles = 0;
-  for (int v = 0; v < p.vocab; v += p.piece) {
-    const int rows = min(p.piece, p.vocab - v);
+  for (int v = 0; v < p.vocab; v += p.loss_piece) {
+    const int rows = min(p.loss_piece, p.vocab - v);
     const Cut cut = cut_rows(p.stats, rows, p.tokens, p.width, p.dtype, false);
     p.stats_tiles += idiv(cut.main, kTiles[p.stats.shape].bm) + idiv(rows - cut.main, kTiles[cut.rest.shape].bm);
   }
-  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, PARTS);
+  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, TURNED);
   p.dw = choose(p.width, p.piece, p.tokens, p.dtype, ROWS);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -1502,8 +1513,8 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     CCT_LAUNCH_CHECK();
   } else if (c.forward) {
     int tiles = 0;
-    for (int v0 = 0; v0 < p.vocab; v0 += p.piece) {
-      const int rows = min(p.piece, p.vocab - v0);
+    for (int v0 = 0; v0 < p.vocab; v0 += p.loss_piece) {
+      const int rows = min(p.loss_piece, p.vocab - v0);
       if (int rc = rows_of_w(v0, rows, &w)) return rc;
       const Cut cut = cut_rows(p.stats, rows, n, p.width, p.dtype, false);
       for (int r0 = 0; r0 < rows; r0 = r0 == 0 ? cut.main : rows) {
@@ -1528,7 +1539,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     const int rows = min(p.piece, p.vocab - v0), mpad = idiv(rows, chunk) * chunk;
     if (!keep) {
       if (int rc = rows_of_w(v0, rows, &w)) return rc;
-      const Cut cut = cut_rows(p.stats, rows, n, p.width, p.dtype, false);
+      const Cut cut = cut_rows(p.grad, rows, n, p.width, p.dtype, false);
       for (int r0 = 0; r0 < rows; r0 = r0 == 0 ? cut.main : rows) {
         const int some = r0 == 0 ? cut.main : rows - r0;
         ProductArgs a = score_args(w + r0 * ldw, v0 + r0, some);
@@ -1540,7 +1551,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
         a.mpad = r0 + some == rows ? mpad - r0 : some;
         a.db_part = c.db ? db_part : nullptr;
         a.db_ld = p.vp;
-        if (int rc = product<T, USE_GRAD, true, true>(r0 == 0 ? p.stats : cut.rest, a)) return rc;
+        if (int rc = product<T, USE_GRAD, true, true>(r0 == 0 ? p.grad : cut.rest, a)) return rc;
         if (c.db) {
           vocab_db_kernel<T><<<idiv(some, 256), 256, 0, st>>>((T *)c.db + v0 + r0, db_part, wmax, some, p.vp, a.tiles_n);
           CCT_LAUNCH_CHECK();
