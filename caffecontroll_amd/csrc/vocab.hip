@@ -397,6 +397,9 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int fgroup = lane >> 4, frow = lane & 15;
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
+  // The epilogues' exponents are score * log2 e - base * log2 e in one instruction, whose second product is rounded once for all
+  // rows, where the base is far enough from the type's limits for it.
+  constexpr float kScaledMax = 2e38f;
   // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from
   // the accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A
   // wavefront takes its own part of the stages, as many rows at a time as it holds; the 16-byte chunks lie swizzled by the
@@ -477,21 +480,33 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
       const int label = t < p.N ? p.labels[t] : -1;
       // the label among this lane's rows: 16 i + r, or out of their range
       const int at = label >= p.v0 && label < p.v0 + p.M ? label - p.v0 - mrow : -1;
-      float score = 0.0f;
+      const bool here = at >= 0 && at < MI * 16 && (at & 15) < 4;
       SoftStat st{neg_inf(), 0.0f};
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          score = at == i * 16 + r ? acc[i][j][r] : score;
-          st.m = fmaxf(st.m, acc[i][j][r]);
-        }
-      if (at >= 0 && at < MI * 16 && (at & 15) < 4) p.label_score[t] = score;
+        for (int r = 0; r < 4; ++r) st.m = fmaxf(st.m, acc[i][j][r]);
+      if (__any(here)) {  // few of a wavefront's tokens have their label among its rows
+        float score = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) score = at == i * 16 + r ? acc[i][j][r] : score;
+        if (here) p.label_score[t] = score;
+      }
       const float base = st.m == neg_inf() ? 0.0f : st.m;
+      if (__any(fabsf(base) > kScaledMax)) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st.s += exp2_fast((acc[i][j][r] - base) * kLog2e);
+          for (int r = 0; r < 4; ++r) st.s += exp2_fast((acc[i][j][r] - base) * kLog2e);
+      } else {
+        const float scaled = base * kLog2e;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st.s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -scaled));
+      }
       st = shfl_xor_join(st, 16, kLog2e);
       st = shfl_xor_join(st, 32, kLog2e);
       if (fgroup == 0) sh[wm * S::BN + (wn * NI + j) * 16 + frow] = st;
@@ -513,13 +528,31 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
       const int t = ncol + j * 16;
       const TokenGrad tg = token_grad(t, p.N, p.labels, p.ignore, p.lse, p.weight, p.wmax);
       const int at = tg.label >= p.v0 && tg.label < p.v0 + p.M ? tg.label - p.v0 - mrow : -1;
+      if (__any(fabsf(tg.lse) > kScaledMax)) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast((acc[i][j][r] - tg.lse) * kLog2e);
+      } else {
+        const float scaled = tg.lse * kLog2e;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -scaled));
+      }
+      if (__any(at >= 0 && at < MI * 16 && (at & 15) < 4)) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] -= at == i * 16 + r ? 1.0f : 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = mrow + i * 16;
         float g[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          g[r] = grad_entry(acc[i][j][r], tg, at == i * 16 + r);
+          g[r] = tg.live ? tg.weight * acc[i][j][r] : 0.0f;
           acc[i][j][r] = g[r];
         }
         if (sizeof(T) == 4 && t < p.N && m < p.mpad) store4<T>((T *)p.g + (size_t)t * p.ldg + m, g, 4);
