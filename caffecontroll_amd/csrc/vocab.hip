@@ -17,6 +17,8 @@
 //          k = vocabulary), and scores that are kept;
 //   OUT    m = width, n = vocabulary, k = token: dw of the piece, stored once in its own type.
 //
+// The loss of few tokens over rows of odd lengths has a kernel of its own, a walk over w.
+//
 // Bound: matrix-core rate.  2 tokens*width*vocab operations for the loss, 4 more for the gradients and 2 for the scores
 // again where they were not kept.
 #include <type_traits>
@@ -397,8 +399,8 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int fgroup = lane >> 4, frow = lane & 15;
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
-  // The epilogues' exponents are score * log2 e - base * log2 e in one instruction, whose second product is rounded once for all
-  // rows, where the base is far enough from the type's limits for it.
+  // The epilogues' exponents are score * log2 e - base * log2 e in one instruction, whose second product is rounded once for
+  // all rows, where the base is far enough from the type's limits for it.
   constexpr float kScaledMax = 2e38f;
   // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from
   // the accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A
@@ -662,7 +664,7 @@ __device__ __forceinline__ void largest_weight(float *__restrict__ wmax, float *
 // x as dw's operand, zero for ignored tokens, so that whatever their x holds stays out of the product.  bf16: transposed,
 // xt[c][t] = x[t][c] for t < tpad (zero past the end), since a transposed read of both operands from LDS is slower than
 // of one.  fp32: xl[t][c] for c < cpad.  With weights, one workgroup more takes the largest of them.  HBM, and a few
-// microseconds beside the products: 91 us for 8192 x 4096 bf16 transposed, 11 us for 2048 x 1024 fp32.
+// microseconds beside the products: 53 us for 8192 x 4096 bf16 transposed, 11 us for 2048 x 1024 fp32.
 template <class T>
 __global__ __launch_bounds__(256) void vocab_live_kernel(T *__restrict__ xl, const T *__restrict__ x, size_t ldx, int tokens,
                                                          int width, int cpad, const int *__restrict__ labels, int ignore,
@@ -719,7 +721,7 @@ __device__ __forceinline__ void store_loss(float *__restrict__ loss, float *__re
 }
 
 // The tiles' statistics of each token: 16 tokens per workgroup, 16 lanes each taking every 16th tile (many tokens), or one
-// token per workgroup (few tokens, so that the launch is not one workgroup's walk over the tiles: 11 instead of 4 us for 16
+// token per workgroup (few tokens, so that the launch is not one workgroup's walk over the tiles: 4 instead of 11 us for 16
 // tokens and 500 tiles).  8192 tokens, 512 tiles: 8 us, 4.2 TB/s.
 template <int TOK>
 __global__ __launch_bounds__(256) void vocab_loss_kernel(float *__restrict__ loss, float *__restrict__ lse,
