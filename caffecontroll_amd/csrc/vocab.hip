@@ -1184,8 +1184,9 @@ struct Choice {
   int splits;
   double us;
 };
-// scores that stay inside; kept scores, fp32 parts along k; dx, the same with w read across its rows; rows of dw
-enum ProductKind { REDUCED, PARTS, TURNED, ROWS };
+// scores that stay inside; kept scores, fp32 parts along k; dx, the same with w read across its rows; dx written at once; rows
+// of dw
+enum ProductKind { REDUCED, PARTS, TURNED, TURNED_ROWS, ROWS };
 static double shape_us(int shape, int splits, int M, int N, int K, int dtype, ProductKind kind) {
   const int d = dtype == CCT_BF16 ? 1 : 0, steps = idiv(K, d ? 64 : 32);
   const TileCost &c = kTiles[shape];
@@ -1197,14 +1198,15 @@ static double shape_us(int shape, int splits, int M, int N, int K, int dtype, Pr
   // across rows narrow tiles take pieces of 128 bytes, and tiles along n fetch them again, mostly from a cache (dx of 131072
   // rows of 4096 bf16: 64 tokens 332 us with 64 x 32 and 264 with 128 x 128, 128 tokens 400 us with 64 x 64)
   const double again = 1.0 + 0.2 * (idiv(N > 0 ? N : 1, c.bn) - 1), rate = c.bm >= 128 ? 4.1e6 : 3.5e6;
-  const double in_us = kind == TURNED ? ((double)M * again + N) * K * el / rate : ((double)M + N) * K * el / kBytesPerUs;
+  const bool turned = kind == TURNED || kind == TURNED_ROWS;
+  const double in_us = turned ? ((double)M * again + N) * K * el / rate : ((double)M + N) * K * el / kBytesPerUs;
   const double work = step * idiv(steps, splits), ends = c.finish * (rounds + (per_cu > 0 ? 1 : 0));
   const double us = kLaunchUs + (work > in_us ? work : in_us) + ends;
   // parts are written by the product and read by what joins them
   if (kind == PARTS || kind == TURNED) return us + 2.0 * splits * out * 4.0 / kBytesPerUs;
   // rows are written while others are computed, or bound the launch
   const double rows_us = kLaunchUs + in_us + out * el / kBytesPerUs;
-  return kind == ROWS && rows_us > us ? rows_us : us;
+  return (kind == ROWS || kind == TURNED_ROWS) && rows_us > us ? rows_us : us;
 }
 static Choice choose(int M, int N, int K, int dtype, ProductKind kind) {
   const bool narrow = kind != ROWS;  // an operand that is contiguous along its rows needs 64 of them
@@ -1262,6 +1264,7 @@ struct VocabPlan {
   int piece, loss_piece;  // rows of w at a time; for the loss alone, which keeps nothing of them
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, grad, kept, dx, dw;
+  bool dx_at_once;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
   int stats_tiles;
@@ -1336,6 +1339,12 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     p.stats_tiles += idiv(cut.main, kTiles[p.stats.shape].bm) + idiv(rows - cut.main, kTiles[cut.rest.shape].bm);
   }
   p.dx = choose(p.width, p.tokens, p.piece, p.dtype, TURNED);
+  // one piece and one part: dx at once, without a launch that joins (bf16, 8 tokens of 64, 500 rows: 19.6 us a step, 24.6 with
+  // it; 4000 tokens of 4096, 20011 rows: 1682 and 1731).  In fp32 the estimate for few workgroups is too good by a sixth (576
+  // tokens of 1408, 6400 rows: 318 us a step at once, 286 in parts).
+  const Choice at_once = choose(p.width, p.tokens, p.piece, p.dtype, TURNED_ROWS);
+  p.dx_at_once = p.piece >= p.vocab && at_once.us < (p.el == 4 ? 0.85 : 1.0) * (p.dx.us + kLaunchUs);
+  if (p.dx_at_once) p.dx = at_once;
   p.dw = choose(p.width, p.piece, p.tokens, p.dtype, ROWS);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -1378,7 +1387,7 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   p.wmax = take(4);
   const bool g_in_scores = p.el == 4 && p.keep_backward[0] && p.keep_backward[1] && p.keep_both[0] && p.keep_both[1];
   p.g = take(g_in_scores ? 0 : n * p.vp * p.el);
-  p.slabs = take((size_t)p.dx.splits * n * p.hp * 4);
+  p.slabs = take(p.dx_at_once ? 0 : (size_t)p.dx.splits * n * p.hp * 4);
   p.db = take((size_t)idiv(p.tokens, 32) * p.vp * 4);
   p.total = at;
   return p;
@@ -1604,10 +1613,17 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
       a.N = n;
       a.K = rows;
       a.kbytes = (uint32_t)(mpad * p.el);
-      a.C = slabs;
-      a.ldc = p.hp;
-      a.accumulate = v0 > 0;
-      if (int rc = product<T, USE_SLAB, false, true>(p.dx, a)) return rc;
+      if (p.dx_at_once) {
+        a.wmax = wmax;
+        a.C = c.dx;
+        a.ldc = p.ldx;
+        if (int rc = product<T, USE_OUT, false, true>(p.dx, a)) return rc;
+      } else {
+        a.C = slabs;
+        a.ldc = p.hp;
+        a.accumulate = v0 > 0;
+        if (int rc = product<T, USE_SLAB, false, true>(p.dx, a)) return rc;
+      }
     }
     if (c.dw) {
       const Cut cut = cut_rows(p.dw, rows, p.width, n, p.dtype, true);
@@ -1634,7 +1650,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
   }
   const int db_blocks = keep && c.db ? idiv(p.vocab, 64) : 0;
   // fewer lanes of a workgroup take part where that puts more of them to work (320 tokens of 200: 32 instead of 34 us with dx)
-  const size_t dx_vecs = c.dx ? (size_t)n * idiv(p.width, 4) : 0;
+  const size_t dx_vecs = c.dx && !p.dx_at_once ? (size_t)n * idiv(p.width, 4) : 0;
   int dx_lanes = kFinishThreads;
   while (dx_lanes > 64 && dx_vecs / dx_lanes < 512) dx_lanes /= 2;
   const unsigned dx_blocks = (unsigned)min((dx_vecs + dx_lanes - 1) / dx_lanes, (size_t)1 << 21);
