@@ -213,6 +213,11 @@ def test_every_call_in_a_replayed_graph(tokens, width, vocab, top):
             np.testing.assert_array_equal(got, w)
 
 
+@pytest.mark.parametrize("tokens, width, vocab, top", [(12, 99, 40001, 5), (1023, 520, 17011, 4)])
+def test_every_call_in_a_replayed_graph_few_tokens_and_rows_past_whole_rounds(tokens, width, vocab, top):
+    test_every_call_in_a_replayed_graph(tokens, width, vocab, top)
+
+
 def test_two_graphs_and_eager_calls_between_them():
     import torch
     a, outs_a, _ka = bf16_calls(2, 130, 72, 1100, 9)
@@ -300,6 +305,30 @@ def test_vocab_loss_weights_past_four_gib():
     assert rel_err(host(dw[vocab - 64:].double()), host(g.T @ x.double())) <= 2 * 2.0 ** -8
     rest = (1.0 / total)[:, None] * x.double()
     assert rel_err(host(dw[5].double()), host(rest.sum(0))) <= 2 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("tokens, width", [(8, 4095), (80, 4096)])
+def test_vocab_loss_alone_past_four_gib(tokens, width):
+    """The loss of few tokens over rows of an odd length, and the loss of more as one piece of 565000 rows."""
+    import torch
+    from caffecontroll_amd.driver import BF16, vocab_loss_args
+    drv, vocab = driver(), 565000
+    w = torch.zeros((vocab, width), dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(tokens, width, device="cuda").to(torch.bfloat16)
+    tail = (torch.randn(64, width, device="cuda") / 16).to(torch.bfloat16)
+    w[vocab - 64:] = tail
+    labels = torch.arange(vocab - tokens, vocab, device="cuda", dtype=torch.int32).clamp_(min=vocab - 64)
+    a = vocab_loss_args(tokens, width, vocab, BF16)
+    n = drv.vocab_loss_workspace_bytes(a, training=False)
+    loss, lse = torch.empty(tokens, device="cuda"), torch.empty(tokens, device="cuda")
+    drv.vocab_loss_forward(loss, lse, x, w, None, labels, a, workspace(n), n)
+    s = x.double() @ tail.double().T
+    want_lse = torch.log(torch.exp(s).sum(1) + (vocab - 64))
+    at = s.gather(1, (labels.long() - (vocab - 64))[:, None])[:, 0]
+    # width terms of a fp32 sum, as above; lse and the label's score each
+    size = 2.5e-4 * float((x.double().abs() @ tail.double().abs().T).max())
+    assert float((lse.double() - want_lse).abs().max()) <= size
+    assert float((loss.double() - (want_lse - at)).abs().max()) <= 2 * size
 
 
 def test_distill_scores_past_four_gib():
