@@ -1,7 +1,7 @@
 // Vocabulary loss: the softmax loss of an inner-product layer with a large vocabulary of outputs, without its scores.
 //
 //   l[t][v] = x[t] . w[v] + bias[v]      lse[t] = log sum_v exp l[t][v]      loss[t] = lse[t] - l[t][label[t]]
-//   G[t][v] = r[t] * (exp(l[t][v] - lse[t]) - [v == label[t]]),  r[t] = loss_grad[t] / c,  c = max |loss_grad|
+//   G[t][v] = r[t] * (exp(l[t][v] - lse[t]) - [v == label[t]]),  r[t] = loss_grad[t] / c,  c = max finite |loss_grad|
 //   dx[t] = c * sum_v G[t][v] w[v]       dw[v] = c * sum_t G[t][v] x[t]      db[v] = c * sum_t G[t][v]
 //
 // G is what bf16 products take as an operand, so it is rounded once.  The weights enter it relative to the largest of
@@ -184,7 +184,7 @@ struct ProductArgs {
   SoftStat *part;            // STATS: [tile of the whole vocabulary][token]
   int part_row;              // first tile of the piece
   float *label_score;        // STATS: [token]
-  const float *lse, *weight, *wmax;  // GRAD; weight: loss_grad or null, wmax: its largest magnitude
+  const float *lse, *weight, *wmax;  // GRAD; weight: loss_grad or null, wmax: its largest finite magnitude
   void *g;                   // GRAD: [token][ldg]
   size_t ldg;                // elements
   int mpad;                  // GRAD: columns of g, whole 16-byte chunks (those past M are zero)
@@ -217,8 +217,7 @@ __device__ __forceinline__ TokenGrad token_grad(int t, int tokens, const int *__
     g.label = labels[t];
     g.live = g.label != ignore;
     g.lse = lse[t];
-    const float c = weight ? *wmax : 1.0f;
-    g.weight = !weight ? 1.0f : c > 0.0f ? weight[t] / c : 0.0f;
+    g.weight = weight ? weight[t] / *wmax : 1.0f;
   }
   return g;
 }
@@ -646,19 +645,23 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(T *__restrict__ dst, co
   }
 }
 
-// The largest magnitude among the weights of the tokens that are not ignored, by one workgroup.
+// The largest magnitude among the finite weights of the tokens that are not ignored, by one workgroup; 1 where none is above
+// zero.  It divides every token's weight and multiplies every result, so a weight that is NaN or infinite has no say in it:
+// such a weight stays what it is, in its own token's G.
 __device__ __forceinline__ void largest_weight(float *__restrict__ wmax, float *sh, const float *__restrict__ weight,
                                                const int *__restrict__ labels, int tokens, int ignore) {
   float m = 0.0f;
-  for (int t = threadIdx.x; t < tokens; t += 256)
-    if (labels[t] != ignore) m = fmaxf(m, fabsf(weight[t]));
+  for (int t = threadIdx.x; t < tokens; t += 256) {
+    const float w = fabsf(weight[t]);
+    if (labels[t] != ignore && w < __builtin_inff()) m = fmaxf(m, w);
+  }
   sh[threadIdx.x] = m;
   __syncthreads();
   for (int d = 128; d > 0; d >>= 1) {
     if ((int)threadIdx.x < d) sh[threadIdx.x] = fmaxf(sh[threadIdx.x], sh[threadIdx.x + d]);
     __syncthreads();
   }
-  if (threadIdx.x == 0) *wmax = sh[0];
+  if (threadIdx.x == 0) *wmax = sh[0] > 0.0f ? sh[0] : 1.0f;
 }
 
 // x as dw's operand, zero for ignored tokens, so that whatever their x holds stays out of the product.  bf16: transposed,

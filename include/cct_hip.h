@@ -555,6 +555,7 @@ int cct_hip_embedding_backward(void *dtable, const void *dout, const int *ids, c
  * gradient is that of the lse alone, as in cct_hip_softmax_loss_backward.  A bias of -inf masks its row of the vocabulary.
  * Gradients for G[t][v] = loss_grad[t] * (exp(l[t][v] - lse[t]) - [v == labels[t]]), loss_grad NULL = all ones:
  *   dx = G w,  dw = G^T x,  db = column sums of G;  any of the three may be NULL.
+ * A loss_grad that is NaN or infinite reaches its own token's row of dx, and dw and db.
  * Rows of x and w may have any width and stride; where both are whole numbers of 16 bytes, x and w start at a multiple
  * of 16 bytes and are read as they are, other rows are copied into the workspace first (but for the loss of a few
  * tokens).  Outputs do not overlap inputs.
