@@ -18,8 +18,6 @@ static std::mutex g_mu;
 static thread_local char g_err[512] = "";
 
 Context &ctx() { return g_ctx; }
-Tuning &tuning() { return g_tuning; }
-
 static void read_tuning_from_env() {
   auto geti = [](const char *name, int dflt) {
     const char *e = getenv(name);
@@ -40,6 +38,12 @@ static void read_tuning_from_env() {
   g_tuning.gemm_nodma = geti("CCT_HIP_GEMM_NODMA", 0);
   g_tuning.vocab_tile = geti("CCT_HIP_VOCAB_TILE", 0);
   g_tuning.vocab_keep = geti("CCT_HIP_VOCAB_KEEP", 0);
+}
+
+// Workspace sizes depend on the knobs and can be asked for before a device is selected.
+Tuning &tuning() {
+  std::call_once(g_tuning_once, read_tuning_from_env);
+  return g_tuning;
 }
 
 // per host thread, like the error text: a launch on one thread never rewrites what another thread reads
@@ -76,7 +80,7 @@ int set_error(int code, const char *fmt, ...) {
 }
 
 static int init_locked(int device_id) {
-  std::call_once(g_tuning_once, read_tuning_from_env);
+  tuning();
   int count = 0;
   CCT_HIP_CHECK(hipGetDeviceCount(&count));
   CCT_REQUIRE(device_id >= 0 && device_id < count, "device %d not present (%d devices)", device_id,
@@ -166,7 +170,6 @@ int cct_hip_init(int device_id) {
 
 int cct_hip_set_tuning(const char *name, int value) {
   CCT_REQUIRE(name != nullptr, "set_tuning: null name");
-  std::call_once(g_tuning_once, read_tuning_from_env);
   Tuning &t = tuning();
   struct { const char *name; int *field; } const table[] = {
       {"direct_tile", &t.direct_tile}, {"direct_waves", &t.direct_waves}, {"direct_tb", &t.direct_tb},

@@ -26,7 +26,7 @@ struct Context {
 };
 
 // Tuning overrides, for experiments and for tests that pin a kernel instance.  Read ONCE from the
-// environment when the library initialises (CCT_HIP_DIRECT_TILE, _DIRECT_WAVES, _DIRECT_TB,
+// environment before their first use (CCT_HIP_DIRECT_TILE, _DIRECT_WAVES, _DIRECT_TB,
 // _DIRECT_NOSPEC, _DIRECT_SPLITS, _DIRECT_ALDS, _DIRECT_WGRAD_ROWS, _STRIDED_WGRAD, _POOL_PLANE, _GEMM_NT, _GEMM_TILE, _GEMM_NODMA, _VOCAB_TILE, _VOCAB_KEEP), changed afterwards only through
 // cct_hip_set_tuning(); the launch paths read this struct, never the environment.
 struct Tuning {

@@ -1211,10 +1211,10 @@ static double shape_us(int shape, int splits, int M, int N, int K, int dtype, Pr
   const double rows_us = kLaunchUs + in_us + out * el / kBytesPerUs;
   return (kind == ROWS || kind == TURNED_ROWS) && rows_us > us ? rows_us : us;
 }
-static Choice choose(int M, int N, int K, int dtype, ProductKind kind) {
+static Choice choose(int tile, int M, int N, int K, int dtype, ProductKind kind) {
   const bool narrow = kind != ROWS;  // an operand that is contiguous along its rows needs 64 of them
   const int steps = idiv(K, dtype == CCT_BF16 ? 64 : 32);
-  const int pinned = tuning().vocab_tile >= 1 && tuning().vocab_tile <= SHAPES ? tuning().vocab_tile : 0;
+  const int pinned = tile >= 1 && tile <= SHAPES ? tile : 0;  // the tuning override
   Choice best{SHAPE_M, 1, 1e30};
   for (int s = 0; s < SHAPES; ++s) {
     if (s >= SHAPE_S && !narrow) continue;
@@ -1235,9 +1235,9 @@ struct Cut {
   int main;  // rows of the first launch: all of them, where there is no second one
   Choice rest;
 };
-static Cut cut_rows(const Choice &c, int rows, int other, int K, int dtype, bool across) {
+static Cut cut_rows(int tile, const Choice &c, int rows, int other, int K, int dtype, bool across) {
   const Cut whole{rows, c};
-  if (other == 0 || tuning().vocab_tile) return whole;
+  if (other == 0 || tile) return whole;
   const TileCost &t = kTiles[c.shape];
   const long per = idiv(other, across ? t.bm : t.bn), block = across ? t.bn : t.bm, round = 256l * t.occ;
   const long blocks = (rows + block - 1) / block, rounds = blocks * per / round, main = rounds * round / per * block;
@@ -1246,7 +1246,7 @@ static Cut cut_rows(const Choice &c, int rows, int other, int K, int dtype, bool
     return across ? shape_us(c.shape, 1, other, n, K, dtype, ROWS) : shape_us(c.shape, 1, n, other, K, dtype, REDUCED);
   };
   const int left = rows - (int)main;
-  const Choice rest = across ? choose(other, left, K, dtype, ROWS) : choose(left, other, K, dtype, REDUCED);
+  const Choice rest = across ? choose(tile, other, left, K, dtype, ROWS) : choose(tile, left, other, K, dtype, REDUCED);
   // (2538 tokens of 824, 44875 rows, 6.9 rounds of tiles: no gain by this estimate, a step of 944 us instead of 890)
   return us((int)main) + rest.us < 0.92 * us(rows) ? Cut{(int)main, rest} : whole;
 }
@@ -1267,6 +1267,7 @@ struct VocabPlan {
   int piece, loss_piece;  // rows of w at a time; for the loss alone, which keeps nothing of them
   int hp, np, vp;      // row lengths of packed operands, x's transpose and G: width, tokens, piece, in whole steps
   Choice stats, grad, kept, dx, dw;
+  Cut stats_cut[2], grad_cut[2], dw_cut[2];  // [1]: of the last piece, whose rows may be fewer
   bool dx_at_once;
   // whether a call keeps the scores (which takes a single piece) or reduces them tile by tile
   bool keep_forward, keep_backward[2], keep_both[2];  // [1]: db is asked for
@@ -1278,8 +1279,11 @@ struct VocabPlan {
   size_t part, label_score, xpack, wpack, scores, xl, wmax, g, slabs, db, total_forward, total;
 };
 
+// All that a call's launches and its workspace have to agree on: the tuning overrides are read here, once, whatever another
+// thread sets in the meantime.
 static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   VocabPlan p;
+  const int tile = tuning().vocab_tile, keep = tuning().vocab_keep;
   p.tokens = a->tokens;
   p.width = a->width;
   p.vocab = a->vocab;
@@ -1312,9 +1316,9 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
   const bool may_keep = (size_t)vmax <= most && (a->piece <= 0 || p.piece == vmax) &&
                         (!p.packed || (size_t)vmax * p.hp * p.el <= kPieceBytes);
   p.loss_piece = a->piece > 0 || p.packed ? p.piece : (int)min((size_t)vmax, most);
-  p.stats = choose(min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
-  p.grad = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
-  p.kept = choose(p.vocab, p.tokens, p.width, p.dtype, PARTS);
+  p.stats = choose(tile, min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.grad = choose(tile, min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.kept = choose(tile, p.vocab, p.tokens, p.width, p.dtype, PARTS);
   const double score_bytes = (double)n * vmax * 4;
   const double stats_us = p.stats.us * idiv(p.vocab, p.loss_piece) + kLaunchUs;
   const double grad_scores_us = p.grad.us * idiv(p.vocab, p.piece) + kLaunchUs;
@@ -1328,27 +1332,32 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     const double db_us = db ? kLaunchUs + score_bytes * (p.el == 4 ? 1 : 2) / kBytesPerUs : 0.0;
     p.keep_backward[db] = fits && p.kept.us + join_us + grad_us + db_us < grad_scores_us;
     p.keep_both[db] = fits && p.kept.us + join_us + grad_us + db_us < stats_us + grad_scores_us;
-    if (tuning().vocab_keep) p.keep_forward = p.keep_backward[db] = p.keep_both[db] = fits && tuning().vocab_keep == 1;
+    if (keep) p.keep_forward = p.keep_backward[db] = p.keep_both[db] = fits && keep == 1;
     keep_any = keep_any || p.keep_forward || p.keep_backward[db] || p.keep_both[db];
   }
   if (keep_any) p.piece = p.loss_piece = vmax;
   p.vp = p.piece + p.unit;
-  p.stats = choose(min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
-  p.grad = choose(min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
-  p.stats_tiles = 0;
-  for (int v = 0; v < p.vocab; v += p.loss_piece) {
-    const int rows = min(p.loss_piece, p.vocab - v);
-    const Cut cut = cut_rows(p.stats, rows, p.tokens, p.width, p.dtype, false);
-    p.stats_tiles += idiv(cut.main, kTiles[p.stats.shape].bm) + idiv(rows - cut.main, kTiles[cut.rest.shape].bm);
-  }
-  p.dx = choose(p.width, p.tokens, p.piece, p.dtype, TURNED);
+  p.stats = choose(tile, min(p.loss_piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.grad = choose(tile, min(p.piece, p.vocab), p.tokens, p.width, p.dtype, REDUCED);
+  p.dx = choose(tile, p.width, p.tokens, p.piece, p.dtype, TURNED);
   // one piece and one part: dx at once, without a launch that joins (bf16, 8 tokens of 64, 500 rows: 19.6 us a step, 24.6 with
   // it; 4000 tokens of 4096, 20011 rows: 1682 and 1731).  In fp32 the estimate for few workgroups is too good by a sixth (576
   // tokens of 1408, 6400 rows: 318 us a step at once, 286 in parts).
-  const Choice at_once = choose(p.width, p.tokens, p.piece, p.dtype, TURNED_ROWS);
+  const Choice at_once = choose(tile, p.width, p.tokens, p.piece, p.dtype, TURNED_ROWS);
   p.dx_at_once = p.piece >= p.vocab && at_once.us < (p.el == 4 ? 0.85 : 1.0) * (p.dx.us + kLaunchUs);
   if (p.dx_at_once) p.dx = at_once;
-  p.dw = choose(p.width, p.piece, p.tokens, p.dtype, ROWS);
+  p.dw = choose(tile, p.width, p.piece, p.tokens, p.dtype, ROWS);
+  p.stats_tiles = 0;
+  for (int last = 0; last < 2; ++last) {
+    const auto rows_of = [&](int piece) { return last ? p.vocab - (idiv(p.vocab, piece) - 1) * piece : min(piece, p.vocab); };
+    const int loss_rows = rows_of(p.loss_piece), rows = rows_of(p.piece);
+    p.stats_cut[last] = cut_rows(tile, p.stats, loss_rows, p.tokens, p.width, p.dtype, false);
+    p.grad_cut[last] = cut_rows(tile, p.grad, rows, p.tokens, p.width, p.dtype, false);
+    p.dw_cut[last] = cut_rows(tile, p.dw, rows, p.width, p.tokens, p.dtype, true);
+    const Cut &cut = p.stats_cut[last];
+    const int tiles = idiv(cut.main, kTiles[p.stats.shape].bm) + idiv(loss_rows - cut.main, kTiles[cut.rest.shape].bm);
+    p.stats_tiles += last ? tiles : (idiv(p.vocab, p.loss_piece) - 1) * tiles;
+  }
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -1368,8 +1377,8 @@ static VocabPlan vocab_plan(const cct_vocab_loss_args *a) {
     p.few_lds = kFewPanel;
   }
   p.few_blocks = 0;
-  if (!whole_chunks(p.ldw, p.width, p.el) && p.tokens <= kFewTokens && p.width * p.el >= 16 && !tuning().vocab_tile &&
-      tuning().vocab_keep != 1 && (f.panel == few_steps || few_tiles >= 1024))
+  if (!whole_chunks(p.ldw, p.width, p.el) && p.tokens <= kFewTokens && p.width * p.el >= 16 && !tile && keep != 1 &&
+      (f.panel == few_steps || few_tiles >= 1024))
     p.few_blocks = min(idiv(few_tiles, kFewWaves / f.split * f.rows),
                        p.few_lds <= 36 << 10 ? 1024 : p.few_lds <= 72 << 10 ? 512 : 256);
   // ranges of a token's kept scores: about 1024 workgroups, of 4096 scores or more, where a token would have four or more
@@ -1563,7 +1572,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     for (int v0 = 0; v0 < p.vocab; v0 += p.loss_piece) {
       const int rows = min(p.loss_piece, p.vocab - v0);
       if (int rc = rows_of_w(v0, rows, &w)) return rc;
-      const Cut cut = cut_rows(p.stats, rows, n, p.width, p.dtype, false);
+      const Cut &cut = p.stats_cut[v0 + rows == p.vocab];
       for (int r0 = 0; r0 < rows; r0 = r0 == 0 ? cut.main : rows) {
         ProductArgs a = score_args(w + r0 * ldw, v0 + r0, r0 == 0 ? cut.main : rows - r0);
         a.part = part;
@@ -1586,7 +1595,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
     const int rows = min(p.piece, p.vocab - v0), mpad = idiv(rows, chunk) * chunk;
     if (!keep) {
       if (int rc = rows_of_w(v0, rows, &w)) return rc;
-      const Cut cut = cut_rows(p.grad, rows, n, p.width, p.dtype, false);
+      const Cut &cut = p.grad_cut[v0 + rows == p.vocab];
       for (int r0 = 0; r0 < rows; r0 = r0 == 0 ? cut.main : rows) {
         const int some = r0 == 0 ? cut.main : rows - r0;
         ProductArgs a = score_args(w + r0 * ldw, v0 + r0, some);
@@ -1629,7 +1638,7 @@ static int vocab_run(const VocabPlan &p, const VocabCall &c) {
       }
     }
     if (c.dw) {
-      const Cut cut = cut_rows(p.dw, rows, p.width, n, p.dtype, true);
+      const Cut &cut = p.dw_cut[v0 + rows == p.vocab];
       for (int r0 = 0; r0 < rows; r0 = r0 == 0 ? cut.main : rows) {
         const int some = r0 == 0 ? cut.main : rows - r0;
         ProductArgs a{};

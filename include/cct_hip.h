@@ -113,7 +113,7 @@ int cct_hip_set_stream(void *hip_stream);
  * vocabulary loss's products: 1 = 256 x 256, 2 = 128 x 128, 3 = 64 x 64, 4 / 5 = 64 x 32 with two / four stages, 0 = automatic), "vocab_keep"
  * (1 = its scores are kept where they fit the limit, 2 = never, 0 = automatic; both also change what its workspace must hold).  The
  * environment variables CCT_HIP_<NAME IN CAPITALS> give the initial values; they are read once,
- * when the library initialises, never on a launch path.  No counterpart in the reference. */
+ * before the first use of any of them, never on a launch path.  No counterpart in the reference. */
 int cct_hip_set_tuning(const char *name, int value);
 /* DeviceDriver::device_sync, src/sched/DeviceDriver.h:267. */
 int cct_hip_device_sync(void);

@@ -1,10 +1,12 @@
 """The vocabulary operators where values are not finite, near the type's limits or cancel, against their definitions in 64
 bits with the bounds of test_gpu_vocab_ops."""
+import threading
+
 import numpy as np
 import pytest
 
-from gpu_util import tuning
-from test_gpu_vocab_ops import BOTH, Vocab, near, values
+from gpu_util import driver, host, tuning
+from test_gpu_vocab_ops import BOTH, Vocab, blank, near, space, values
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,61 @@ def test_vocab_loss_weights_that_are_not_finite(dtype, keep, kind):
             near(dx[~bad], sound.dx[~bad], sound.edx[~bad])
             assert not np.isfinite(dx[bad]).any() and bad[5] and not bad[7]
             assert not np.isfinite(dw).any() and not np.isfinite(db).any()
+
+
+# ---- knobs that change while calls run ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("training", [False, True])
+def test_vocab_loss_while_another_thread_changes_its_tile(training):
+    """A call keeps to the tile that it began with: every result is that of one setting or of the other, and the workspace,
+    which has room for either, ends where it says."""
+    import torch
+    from caffecontroll_amd.driver import BF16, vocab_loss_args
+    drv, tokens, width, vocab = driver(), 1023, 64, 50021
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, w = (torch.randn(n, width, generator=gen, device="cuda").to(torch.bfloat16) for n in (tokens, vocab))
+    labels = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda", dtype=torch.int32)
+    a, need = vocab_loss_args(tokens, width, vocab, BF16), 0
+    for tile in (0, 3):
+        with tuning("vocab_tile", tile):
+            need = max(need, drv.vocab_loss_workspace_bytes(a, training))
+    ws = space(need)
+
+    def outputs():
+        o = [blank((tokens,)), blank((tokens,))]
+        return o + [blank(x.shape, "bf16"), blank(w.shape, "bf16")] if training else o
+
+    def call(o):
+        if training:
+            drv.vocab_loss_forward_backward(o[0], o[1], o[2], o[3], None, x, w, None, labels, None, a, ws.ptr, need)
+        else:
+            drv.vocab_loss_forward(o[0], o[1], x, w, None, labels, a, ws.ptr, need)
+
+    want = []
+    for tile in (0, 3):
+        with tuning("vocab_tile", tile):
+            o = outputs()
+            call(o)
+            want.append([host(t.float()) for t in o])
+    stop = threading.Event()
+
+    def change():
+        n = 0
+        while not stop.is_set():
+            n += 1
+            drv.set_tuning("vocab_tile", 3 * (n % 2))
+
+    other = threading.Thread(target=change)
+    other.start()
+    try:
+        got = []
+        for _ in range(60):
+            o = outputs()
+            call(o)
+            got.append([host(t.float()) for t in o])
+    finally:
+        stop.set()
+        other.join()
+        drv.set_tuning("vocab_tile", 0)
+    assert ws.intact()
+    for g in got:
+        assert any(all(np.array_equal(a, b) for a, b in zip(g, w)) for w in want)
