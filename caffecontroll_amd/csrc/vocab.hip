@@ -399,8 +399,9 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
   const int mrow = m0 + wm * MI * 16 + fgroup * 4, ncol = n0 + wn * NI * 16 + frow;
 
   // The epilogues' exponents are score * log2 e - base * log2 e in one instruction, whose second product is rounded once for
-  // all rows, where the base is far enough from the type's limits for it.
-  constexpr float kScaledMax = 2e38f;
+  // all rows.  That rounding moves every exponent by up to 2^-24 of the product, 0.09 at this bound; scores past it are
+  // subtracted first.  (Without a bound the largest score's own power leaves the type's range from 2e9 on.)
+  constexpr float kScaledMax = 1 << 20;
   // bf16 rows leave through LDS, so that a store has up to 256 bytes of one, 16 a lane, instead of 32 with 8 straight from
   // the accumulators (dw of 64 tokens of 2048, 32000 rows: 51 -> 38 us; G of the largest step: 26.8 -> 26.65 ms in all).  A
   // wavefront takes its own part of the stages, as many rows at a time as it holds; the 16-byte chunks lie swizzled by the

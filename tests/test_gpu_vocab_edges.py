@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from gpu_util import driver, host, tuning
-from test_gpu_vocab_ops import BOTH, Vocab, blank, near, space, values
+from test_gpu_vocab_ops import BOTH, HALF, U, Vocab, blank, near, space, values
 
 pytestmark = pytest.mark.gpu
 
@@ -37,6 +37,41 @@ def test_vocab_loss_weights_that_are_not_finite(dtype, keep, kind):
             near(dx[~bad], sound.dx[~bad], sound.edx[~bad])
             assert not np.isfinite(dx[bad]).any() and bad[5] and not bad[7]
             assert not np.isfinite(dw).any() and not np.isfinite(db).any()
+
+
+# ---- scores far from zero ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("keep", [1, 2])
+def test_vocab_loss_scores_of_any_size(dtype, keep):
+    """Tokens whose largest scores are 1e6 to 1e32 and whose next ones are far below: lse is the largest score, the gradient
+    that of one entry against the label, and the other tokens' are as they were."""
+    v = Vocab(dtype, 80, 40, 900, bias=True)
+    big = {3: 1e6, 9: 3e9, 10: 3e10, 11: -7e11, 40: 2e15, 70: -1e20, 79: 1e32}
+    best, worst = 500, 20                                          # the rows with the largest and the smallest first column
+    v.w[:, 0] *= 0.5
+    v.w[best, 0], v.w[worst, 0] = 8.0, -8.0
+    for t, x in big.items():
+        v.x[t] = 0.0
+        v.x[t, 0] = x
+        v.labels[t] = 7
+    v.x64, v.w64 = values(v.x), values(v.w)
+    v.gs[:] = 0.5
+    v.reference()
+    rows, rest = list(big), [t for t in range(80) if t not in big]
+    with tuning("vocab_keep", keep):
+        for run in (v.both, lambda: (v.forward(), v.backward())):
+            v.outputs()
+            run()
+            near(values(v.o_lse)[rest], v.lse[rest], v.else_[rest])
+            near(values(v.o_dx)[rest], v.dx[rest], v.edx[rest])
+            # one product, the bias, a sum of one: four roundings at most
+            near(values(v.o_lse)[rows], v.lse[rows], 4 * U * np.abs(v.lse[rows]))
+            near(values(v.o_loss)[rows], v.loss[rows], 8 * U * np.abs(v.lse[rows]))
+            # G is 1 and -1 (times the weight, which the largest of them divides: all are alike), exactly
+            top = [best if x > 0 else worst for x in big.values()]
+            want = 0.5 * (v.w64[top] - v.w64[7])
+            near(values(v.o_dx)[rows], want, (2 * U + HALF[dtype]) * 0.5 * (np.abs(v.w64[top]) + np.abs(v.w64[7])))
+            assert np.isfinite(values(v.o_dw)).all() and np.isfinite(values(v.o_db)).all()
 
 
 # ---- knobs that change while calls run ---------------------------------------------------------------------------------
