@@ -1,7 +1,7 @@
 // Distillation loss from a teacher's top logits, on stored scores.
 //
 //   q = softmax(top_logits / T) over a token's list,  p = softmax(logits / T) over the vocabulary
-//   lse = log sum exp(logits / T),  loss = T^2 sum_k q_k (log q_k - logits[id_k] / T + lse)
+//   lse = log sum exp(logits / T),  loss = T^2 sum_k q_k (log q_k - logits[id_k] / T + lse), from the statistics behind lse
 //   dlogits_v = loss_grad * T * (p_v - sum of q_k over id_k == v)
 //
 // Exponentials are v_exp_f32 of (difference * log2 e / T).  Bound by HBM: the scores are read once for the loss (2051 tokens,
@@ -117,10 +117,7 @@ __device__ __forceinline__ void distill_loss_wave(float *__restrict__ loss, floa
   for (int k = lane; k < s.top; k += 64) {
     const int id = ids[k];
     const float q = teacher_weight(te, id, top[k], s.scale2);
-    if (q != 0.0f && id < s.vocab) {
-      const float logp = __builtin_fmaf((float)row[id], s.inv_t, -l);
-      sum += q * (((top[k] - te.m) * s.inv_t - logs) - logp);
-    }
+    if (q != 0.0f && id < s.vocab) sum += q * (((top[k] - te.m) * s.inv_t - logs) + label_loss(st, (float)row[id], s.inv_t));
   }
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
@@ -319,7 +316,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
     const float q = teacher_weight(teacher, id, weight, s.scale2);
     float term = 0.0f;
     if (inside && q != 0.0f)
-      term = q * (((weight - te.m) * s.inv_t - __builtin_log2f(te.s) * kLn2) - __builtin_fmaf(z, s.inv_t, -l));
+      term = q * (((weight - te.m) * s.inv_t - __builtin_log2f(te.s) * kLn2) + label_loss(st, z, s.inv_t));
     const bool mine = inside && q != 0.0f;
     sh_id[tid] = mine ? id : -1;
     sh_q[tid] = q;

@@ -100,5 +100,9 @@ __device__ __forceinline__ SoftStat shfl_xor_join(SoftStat a, int mask, float sc
 __device__ __forceinline__ float log_sum(SoftStat a, float inv_t) {
   return __builtin_fmaf(a.m, inv_t, __builtin_log2f(a.s) * kLn2);
 }
+// log_sum less v / T, without the rounding of log_sum
+__device__ __forceinline__ float label_loss(SoftStat a, float v, float inv_t) {
+  return __builtin_fmaf(a.m - v, inv_t, __builtin_log2f(a.s) * kLn2);
+}
 
 }  // namespace cct

@@ -508,6 +508,7 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
         for (int i = 0; i < MI; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) st.s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -scaled));
+        st.s *= exp2_fast(-__builtin_fmaf(base, kLog2e, -scaled));  // the rounding of `scaled`, the same in every term
       }
       st = shfl_xor_join(st, 16, kLog2e);
       st = shfl_xor_join(st, 32, kLog2e);
@@ -718,10 +719,14 @@ __global__ __launch_bounds__(256) void vocab_xt_kernel(T *__restrict__ xt, const
 }
 
 // ---- joining -----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void store_loss(float *__restrict__ loss, float *__restrict__ lse, int t, float l, int label,
-                                           float score, int vocab, int ignore) {
+// lse is one float, off by 2^-24 of the largest score; the loss is formed from the statistics, so that the loss of a confident
+// token, or of one whose every score is near the type's lowest value, is not lost in that.
+__device__ __forceinline__ float store_loss(float *__restrict__ loss, float *__restrict__ lse, int t, SoftStat st, int label,
+                                            float score, int vocab, int ignore) {
+  const float l = log_sum(st, 1.0f);
   lse[t] = l;
-  loss[t] = label == ignore ? 0.0f : (unsigned)label < (unsigned)vocab ? l - score : __builtin_nanf("");
+  loss[t] = label == ignore ? 0.0f : (unsigned)label < (unsigned)vocab ? label_loss(st, score, 1.0f) : __builtin_nanf("");
+  return l;
 }
 
 // The tiles' statistics of each token: 16 tokens per workgroup, 16 lanes each taking every 16th tile (many tokens), or one
@@ -755,7 +760,7 @@ __global__ __launch_bounds__(256) void vocab_loss_kernel(float *__restrict__ los
     __syncthreads();
   }
   if (y == 0 && t < tokens)
-    store_loss(loss, lse, t, log_sum(sh[0][x], 1.0f), labels[t], label_score[t], vocab, ignore);
+    store_loss(loss, lse, t, sh[0][x], labels[t], label_score[t], vocab, ignore);
 }
 
 // The loss of at most 64 tokens where w's rows would have to be packed first: one walk over w, its rows as they lie, bound by
@@ -1044,9 +1049,8 @@ __global__ __launch_bounds__(kRowThreads) void vocab_row_kernel(float *__restric
     const SoftStat st = row_stats<T>(row, p, 0, p.vocab, loss != nullptr);
     if (loss && threadIdx.x == 0) {
       const int label = p.labels[t];
-      lse_sh = log_sum(st, 1.0f);
-      store_loss(loss, lse_out, t, lse_sh, label, (unsigned)label < (unsigned)p.vocab ? row_score<T>(row, p, label) : 0.0f,
-                 p.vocab, p.ignore);
+      lse_sh = store_loss(loss, lse_out, t, st, label,
+                          (unsigned)label < (unsigned)p.vocab ? row_score<T>(row, p, label) : 0.0f, p.vocab, p.ignore);
     }
   }
   if (!loss && threadIdx.x == 0) lse_sh = lse_in[t];
@@ -1084,7 +1088,7 @@ __global__ __launch_bounds__(kRowThreads) void vocab_range_grad_kernel(float *__
       for (int m = 32; m > 0; m >>= 1) st = shfl_xor_join(st, m, kLog2e);
       if (threadIdx.x == 0) {
         lse_sh = log_sum(st, 1.0f);
-        if (blockIdx.x == 0) store_loss(loss, lse_out, t, lse_sh, p.labels[t], label_score[t], p.vocab, p.ignore);
+        if (blockIdx.x == 0) store_loss(loss, lse_out, t, st, p.labels[t], label_score[t], p.vocab, p.ignore);
       }
     }
   } else if (threadIdx.x == 0) {

@@ -6,9 +6,10 @@ import numpy as np
 import pytest
 
 from gpu_util import driver, host, tuning
-from test_gpu_vocab_ops import BOTH, HALF, U, Vocab, blank, near, space, values
+from test_gpu_vocab_ops import BOTH, HALF, U, Distill, Vocab, blank, near, space, values
 
 pytestmark = pytest.mark.gpu
+LOWEST = 255 * 2.0 ** 120                                      # the largest magnitude of a bf16, in both types
 
 
 # ---- vocabulary loss: weights of the tokens --------------------------------------------------------------------------
@@ -72,6 +73,53 @@ def test_vocab_loss_scores_of_any_size(dtype, keep):
             want = 0.5 * (v.w64[top] - v.w64[7])
             near(values(v.o_dx)[rows], want, (2 * U + HALF[dtype]) * 0.5 * (np.abs(v.w64[top]) + np.abs(v.w64[7])))
             assert np.isfinite(values(v.o_dw)).all() and np.isfinite(values(v.o_db)).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("keep", [1, 2])
+@pytest.mark.parametrize("tokens, width", [(70, 8), (5, 33)])
+@pytest.mark.parametrize("top, rest", [(4000.0, 3984.0), (-LOWEST, -LOWEST), (-1e30, -1e30), (2.0 ** 70, 2.0 ** 70)])
+def test_vocab_loss_is_not_lost_in_the_size_of_the_scores(dtype, keep, tokens, width, top, rest):
+    """Scores that are the bias alone: one entry ahead of the others by 16, or all alike.  The loss is of the size of the
+    scores' differences, whatever their own."""
+    v = Vocab(dtype, tokens, width, 900, bias=True)
+    v.x[:] = 0.0
+    v.b[:] = rest
+    v.b[123] = top
+    v.labels[:] = np.where(np.arange(tokens) % 3 == 0, 123, 7)
+    b = values(v.b)
+    ahead = float(b[123] - b[7])
+    assert ahead in (0.0, 16.0)
+    log_sum = np.log1p(899 * np.exp(-ahead))
+    want = np.where(v.labels == 123, log_sum, log_sum + ahead)
+    with tuning("vocab_keep", keep):
+        for run in (v.forward, v.both):
+            v.outputs()
+            run()
+            # exponentials and their sum: at most 100 additions in a row onto it; the logarithm and the difference in the result
+            near(values(v.o_loss), want, 100 * U + 2.0 ** -21 + 2 * U * want)
+            near(values(v.o_lse), np.full(tokens, b[123] + log_sum), 4 * U * abs(top))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("vocab", [300, 9001, 140000])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 0.25])
+@pytest.mark.parametrize("level", [-LOWEST, 4000.0, -1e30])
+def test_distill_loss_is_not_lost_in_the_size_of_the_scores(dtype, vocab, temperature, level):
+    """Scores that are all alike, at any level: the student's distribution is uniform."""
+    d = Distill(dtype, 3, vocab, 4, temperature=temperature)
+    d.z[:] = level
+    d.ids[:] = [0, 5, vocab - 1, -1]
+    d.tl[:] = np.array([1.0, 2.0, 0.0, 9.0]) * temperature
+    d.upload()
+    q = np.exp([1.0, 2.0, 0.0])
+    q /= q.sum()
+    want = temperature ** 2 * (q * (np.log(q) + np.log(vocab))).sum()
+    for both in (False, True):
+        d.run(both)
+        # additions as in Distill.reference, and the roundings of a sum of terms of log(vocab)
+        bound = temperature ** 2 * ((vocab / 256 + 200) * U * 2 + 20 * U * np.log(vocab) + 2.0 ** -20)
+        near(values(d.o_loss), np.full(3, want), bound)
 
 
 # ---- knobs that change while calls run ---------------------------------------------------------------------------------
