@@ -73,9 +73,19 @@ __global__ __launch_bounds__(DST_THREADS) void distill_stats_kernel(SoftStat *__
   if (threadIdx.x == 0) part[blockIdx.x] = st;
 }
 
-// softmax(logits / T) of one score; the difference is formed before log2 e is applied
-__device__ __forceinline__ float probability(float score, float lse, const DistillShape &s) {
-  return exp2_fast(__builtin_fmaf(score, s.inv_t, -lse) * kLog2e);
+// softmax(logits / T) of one score: 2^((score - m) log2 e / T - log2 of the sum).  The difference comes first, so that scores of
+// any size keep theirs, and none is above m.  A backward pass that has nothing but the lse takes T lse as m and a
+// sum of one: off by the rounding of both, 2^-23 |lse| in the exponent, and cut at one, which that may pass.
+struct Student {
+  float m, log2_sum;
+};
+__device__ __forceinline__ Student student(SoftStat st) { return Student{st.m, __builtin_log2f(st.s)}; }
+__device__ __forceinline__ float probability(float score, const Student &p, const DistillShape &s) {
+  return exp2_fast(__builtin_fmaf(score - p.m, s.scale2, -p.log2_sum));
+}
+__device__ __forceinline__ float probability_cut(float score, const Student &p, const DistillShape &s) {
+  const float e = __builtin_fmaf(score - p.m, s.scale2, -p.log2_sum);
+  return exp2_fast(e > 0.0f ? 0.0f : e);  // (NaN stays)
 }
 
 // The teacher's distribution of one token, by one wavefront: lane l holds entries l, l + 64, ...
@@ -199,17 +209,19 @@ __device__ __forceinline__ bool gather_entries(const EntryLists &e, const T *row
 
 // The entries of a list on top of what the row's lanes wrote.
 template <class T>
-__device__ __forceinline__ void store_entries(T *dst, const EntryLists &e, float g, float lse, const DistillShape &s) {
+__device__ __forceinline__ void store_entries(T *dst, const EntryLists &e, float g, const Student &p, const DistillShape &s) {
   for (int k = threadIdx.x; k < s.top; k += blockDim.x)
-    if (e.id[k] >= 0) dst[e.id[k]] = (T)(g * (probability(e.z[k], lse, s) - e.sum[k]));
+    if (e.id[k] >= 0) dst[e.id[k]] = (T)(g * (probability_cut(e.z[k], p, s) - e.sum[k]));
 }
 
-// The gradient of one range of one token's scores.
+// The gradient of one range of one token's scores; part: its ranges' statistics (at most 64, joined by every wavefront for
+// itself), or null where there is only the lse.
 template <class T>
 __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, const T *logits,
                                                                    const int *__restrict__ ids,
                                                                    const float *__restrict__ top,
                                                                    const float *__restrict__ lse,
+                                                                   const SoftStat *__restrict__ part,
                                                                    const float *__restrict__ loss_grad, DistillShape s) {
   constexpr int V = Num<T>::V;
   extern __shared__ float lists[];
@@ -220,17 +232,24 @@ __global__ __launch_bounds__(DST_THREADS) void distill_grad_kernel(T *dlogits, c
   T *dst = dlogits + (size_t)t * s.logits_stride;
   const bool weight =
       gather_entries<T>(e, row, ids + (size_t)t * s.top_stride, top + (size_t)t * s.top_stride, begin, end, s);
-  const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f), l = lse[t];
+  const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f);
+  Student p{0.0f, 0.0f};
+  if (part) {
+    const int lane = threadIdx.x & 63;
+    p = student(wave_join(lane < s.splits ? part[(size_t)t * s.splits + lane] : SoftStat{neg_inf(), 0.0f}, s.scale2));
+  } else {
+    p.m = lse[t] * s.temperature;
+  }
   for (int col = begin + threadIdx.x * V; col < end; col += DST_THREADS * V) {
     float f[V];
     load_vec<T>(f, row, col, end);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = weight ? g * probability(f[i], l, s) : 0.0f;
+    for (int i = 0; i < V; ++i) f[i] = weight ? g * probability_cut(f[i], p, s) : 0.0f;
     store_vec<T>(dst, f, col, end);
   }
   if (!weight) return;
   __syncthreads();
-  store_entries<T>(dst, e, g, l, s);
+  store_entries<T>(dst, e, g, p, s);
 }
 
 // Loss and gradient of whole rows, each read once: a workgroup keeps its row in registers from the statistics to the
@@ -310,6 +329,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
     te.m = __shfl(te.m, 0, 64);
     te.s = __shfl(te.s, 0, 64);
     const float l = log_sum(st, s.inv_t);
+    const Student p = student(st);
     const Teacher teacher{te.m, te.s, false};
     const bool some = teacher.some();
     // this lane's entry
@@ -334,7 +354,7 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
       }
     const float g = s.temperature * (loss_grad ? loss_grad[t] : 1.0f);
     T *dst = dlogits + (size_t)t * s.logits_stride;
-    const float entry_grad = g * (probability(z, l, s) - sum);
+    const float entry_grad = g * (probability(z, p, s) - sum);
     const int entry_id = id;
     const int next = t + (int)gridDim.x;
     const bool more = next < s.tokens;
@@ -349,13 +369,13 @@ __global__ __launch_bounds__(THREADS) void distill_row_kernel(float *__restrict_
       if (col < whole) {
         vec out;
 #pragma unroll
-        for (int k = 0; k < V; ++k) out[k] = (T)(some ? g * probability((float)v[i][k], l, s) : 0.0f);
+        for (int k = 0; k < V; ++k) out[k] = (T)(some ? g * probability((float)v[i][k], p, s) : 0.0f);
         __builtin_nontemporal_store(out, reinterpret_cast<vec *>(dst + col));
       }
       if (more) fetch(i, next_row);
     }
     if (tail >= 0) {
-      dst[tail] = (T)(some ? g * probability((float)rest, l, s) : 0.0f);
+      dst[tail] = (T)(some ? g * probability((float)rest, p, s) : 0.0f);
       if (more) rest = next_row[tail];
     }
     if (more && id >= 0 && id < s.vocab) z = (float)next_row[id];
@@ -416,9 +436,9 @@ static size_t distill_bytes(const cct_distill_loss_args *a) {
 
 template <class T>
 static int distill_forward(float *loss, float *lse, const void *logits, const int *ids, const float *top,
-                           const DistillShape &s, void *ws) {
+                           const DistillShape &s, void *ws, bool keep_stats) {
   hipStream_t st = ctx().stream;
-  if (s.splits == 1) {
+  if (s.splits == 1 && !keep_stats) {
     distill_token_kernel<T><<<s.tokens, DST_THREADS, 0, st>>>(loss, lse, (const T *)logits, ids, top, s);
     CCT_LAUNCH_CHECK();
     note_kernel("distill_token_kernel<%s>", Num<T>::NAME);
@@ -436,9 +456,9 @@ static int distill_forward(float *loss, float *lse, const void *logits, const in
 
 template <class T>
 static int distill_backward(void *dlogits, const void *logits, const int *ids, const float *top, const float *lse,
-                            const float *loss_grad, const DistillShape &s) {
+                            const SoftStat *part, const float *loss_grad, const DistillShape &s) {
   distill_grad_kernel<T><<<(unsigned)s.tokens * s.splits, DST_THREADS, 5 * s.top * sizeof(float), ctx().stream>>>(
-      (T *)dlogits, (const T *)logits, ids, top, lse, loss_grad, s);
+      (T *)dlogits, (const T *)logits, ids, top, lse, part, loss_grad, s);
   CCT_LAUNCH_CHECK();
   note_kernel("distill_grad_kernel<%s> splits=%d", Num<T>::NAME, s.splits);
   return 0;
@@ -464,8 +484,8 @@ static int distill_both(float *loss, float *lse, void *dlogits, const void *logi
   CCT_DISTILL_ROW(1024, 8, 1)
   CCT_DISTILL_ROW(1024, 16, 1)
 #undef CCT_DISTILL_ROW
-  if (int rc = distill_forward<T>(loss, lse, logits, ids, top, s, ws)) return rc;
-  return distill_backward<T>(dlogits, logits, ids, top, lse, loss_grad, s);
+  if (int rc = distill_forward<T>(loss, lse, logits, ids, top, s, ws, true)) return rc;
+  return distill_backward<T>(dlogits, logits, ids, top, lse, (const SoftStat *)ws, loss_grad, s);
 }
 
 static int check_distill_workspace(const cct_distill_loss_args *a, const void *ws, size_t bytes, const char *who) {
@@ -492,8 +512,8 @@ extern "C" int cct_hip_distill_loss_forward(float *loss, float *lse, const void 
   if (int rc = check_distill_workspace(args, workspace, workspace_bytes, "distill_loss_forward")) return rc;
   CCT_ENSURE_INIT();
   const DistillShape s = distill_shape(args);
-  return args->dtype == CCT_BF16 ? distill_forward<bf16>(loss, lse, logits, top_ids, top_logits, s, workspace)
-                                 : distill_forward<float>(loss, lse, logits, top_ids, top_logits, s, workspace);
+  return args->dtype == CCT_BF16 ? distill_forward<bf16>(loss, lse, logits, top_ids, top_logits, s, workspace, false)
+                                 : distill_forward<float>(loss, lse, logits, top_ids, top_logits, s, workspace, false);
 }
 
 extern "C" int cct_hip_distill_loss_backward(void *dlogits, const void *logits, const int *top_ids, const float *top_logits,
@@ -505,8 +525,8 @@ extern "C" int cct_hip_distill_loss_backward(void *dlogits, const void *logits, 
   if (int rc = check_distill_workspace(args, workspace, workspace_bytes, "distill_loss_backward")) return rc;
   CCT_ENSURE_INIT();
   const DistillShape s = distill_shape(args);
-  return args->dtype == CCT_BF16 ? distill_backward<bf16>(dlogits, logits, top_ids, top_logits, lse, loss_grad, s)
-                                 : distill_backward<float>(dlogits, logits, top_ids, top_logits, lse, loss_grad, s);
+  return args->dtype == CCT_BF16 ? distill_backward<bf16>(dlogits, logits, top_ids, top_logits, lse, nullptr, loss_grad, s)
+                                 : distill_backward<float>(dlogits, logits, top_ids, top_logits, lse, nullptr, loss_grad, s);
 }
 
 extern "C" int cct_hip_distill_loss_forward_backward(float *loss, float *lse, void *dlogits, const void *logits,

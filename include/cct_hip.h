@@ -592,7 +592,9 @@ int cct_hip_vocab_loss_forward_backward(float *loss, float *lse, void *dx, void 
  * An entry with a negative id is absent (lists of different lengths); one with a top logit of -inf has no weight.
  * A token without any entry of weight has loss 0 and gradient 0.  An id of vocab or above is never used as an index: that
  * token's loss is NaN, and the gradient subtracts nothing for it.  An id may appear more than once.  dlogits may be
- * logits itself. */
+ * logits itself.
+ * backward knows a token's scores by its lse, one float: its p has a relative error of 2^-23 |lse| (and is never above 1), which is
+ * everything for a token whose every score is near the type's lowest value.  forward_backward has p from the scores. */
 typedef struct cct_distill_loss_args {
   int tokens, vocab, top; /* top <= 1024 */
   int dtype;              /* of logits and dlogits; top_logits are fp32 */

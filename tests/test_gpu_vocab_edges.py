@@ -122,6 +122,41 @@ def test_distill_loss_is_not_lost_in_the_size_of_the_scores(dtype, vocab, temper
         near(values(d.o_loss), np.full(3, want), bound)
 
 
+@pytest.mark.parametrize("dtype, tokens, vocab", [(d, 3, v) for d in BOTH for v in (300, 9001, 140000)] + [("bf16", 8200, 140000)])
+@pytest.mark.parametrize("temperature, level", [(1.5, 1e10), (1.5, -LOWEST), (0.3, -1e30), (3.0, 4000.0)])
+def test_distill_gradient_of_scores_of_any_size(dtype, tokens, vocab, temperature, level):
+    """Scores that are all alike, at any level: p is 1 / vocab.  From the lse alone it is known to 2^-23 |lse|, and at most 1."""
+    import torch
+    d = Distill(dtype, 3, vocab, 4, temperature=temperature)
+    if tokens > 3:                                                 # more tokens than rows are cut into ranges for
+        d.z = torch.empty((tokens, vocab), dtype=torch.bfloat16, device="cuda")
+    d.z[:] = level
+    d.tokens = tokens
+    d.ids = np.tile([0, 5, vocab - 1, -1], (tokens, 1))
+    d.tl = np.tile(np.array([1.0, 2.0, 0.0, 9.0]) * temperature, (tokens, 1)).astype(np.float32)
+    d.gs = np.full(tokens, 0.5, np.float32)
+    d.upload()
+    q = np.exp([1.0, 2.0, 0.0])
+    want = np.full(vocab, 1.0 / vocab)
+    want[[0, 5, vocab - 1]] -= q / q.sum()
+    want *= 0.5 * temperature
+    d.run(True)
+    # p: the sum's additions (as in Distill.reference), its logarithm, the exponential; q: four entries; the products
+    e = ((vocab / 256 + 200) * U * 2 + 8 * U * np.log(vocab) + 2.0 ** -20) / vocab
+    bound = 0.5 * temperature * (e + (want < 0) * (16 * U + 2.0 ** -20)) + 4 * U * np.abs(want)
+    bound += HALF[dtype] * (np.abs(want) + bound)
+    some = d.o_d if tokens == 3 else d.o_d[[0, 1, tokens // 2, tokens - 1]]
+    near(values(some), np.tile(want, (some.shape[0], 1)), np.tile(bound, (some.shape[0], 1)))
+    d.run(False)
+    some = values(d.o_d if tokens == 3 else d.o_d[[0, 1, tokens // 2, tokens - 1]])
+    most = 0.5 * temperature * (1 + 2.0 ** -20) * (1 + HALF[dtype])
+    assert (np.abs(some) <= most).all()
+    lse = abs(level) / temperature + np.log(vocab)
+    if lse * 2.0 ** -23 < 0.01:
+        worse = 0.5 * temperature / vocab * 2.1 * lse * 2.0 ** -23
+        near(some, np.tile(want, (some.shape[0], 1)), np.tile(bound + worse * (1 + HALF[dtype]), (some.shape[0], 1)))
+
+
 # ---- knobs that change while calls run ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("training", [False, True])
 def test_vocab_loss_while_another_thread_changes_its_tile(training):
