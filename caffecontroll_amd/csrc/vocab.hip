@@ -221,8 +221,14 @@ __device__ __forceinline__ TokenGrad token_grad(int t, int tokens, const int *__
   }
   return g;
 }
+// A large score that was computed in another order than the lse's may lie above it by its own rounding: p is cut at one (NaN
+// stays).
+__device__ __forceinline__ float probability_cut(float score, float lse) {
+  const float e = (score - lse) * kLog2e;
+  return exp2_fast(e > 0.0f ? 0.0f : e);
+}
 __device__ __forceinline__ float grad_entry(float score, const TokenGrad &tg, bool is_label) {
-  const float p = exp2_fast((score - tg.lse) * kLog2e);
+  const float p = probability_cut(score, tg.lse);
   return tg.live ? tg.weight * (p - (is_label ? 1.0f : 0.0f)) : 0.0f;
 }
 
@@ -535,7 +541,7 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = exp2_fast((acc[i][j][r] - tg.lse) * kLog2e);
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = probability_cut(acc[i][j][r], tg.lse);
       } else {
         const float scaled = tg.lse * kLog2e;
 #pragma unroll

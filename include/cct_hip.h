@@ -560,7 +560,8 @@ int cct_hip_embedding_backward(void *dtable, const void *dout, const int *ids, c
  * of 16 bytes and are read as they are, other rows are copied into the workspace first (but for the loss of a few
  * tokens).  Outputs do not overlap inputs.
  * The gradients know a token's scores by its lse, one float: entries of G have a relative error of 2^-23 |lse|, which
- * is nothing for scores of a model, and everything for a token whose every score is near the type's lowest value.
+ * is nothing for scores of a model, and everything for a token whose every score is near the type's lowest value; with scores
+ * past 2^20 the exponential is cut at 1.
  * In bf16, G is rounded to bf16 as an operand of the two products (as an inner-product layer's output gradient
  * is); everything else stays in fp32 up to the final store.
  * forward_backward gives what forward and then backward give, to rounding.  Where that is cheaper, and the fp32 scores
