@@ -55,8 +55,8 @@ typedef __attribute__((address_space(3))) char lds_char;
 // 16 bytes a lane from global memory into LDS: lane l's land at dst + 16 l; an offset past the descriptor's 2^31 bytes fetches
 // nothing and writes zeros.  The instruction itself instead of its builtin: the compiler would wait for all copies
 // in flight before every ds_read_b64_tr_b16, whose address it cannot tell from theirs (a product with such an operand: 1.43
-// instead of 0.83 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 (the
-// LDS address) is used by nothing else in these kernels.
+// instead of 0.83 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 holds
+// the LDS address.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, uint32_t offset, lds_char *dst) {
   const uint64_t at = (uint64_t)base;
@@ -64,7 +64,7 @@ __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, u
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"((uint32_t)(uintptr_t)dst),
       "v"(lane_offset), "s"(rsrc), "s"(offset)
-      : "memory");
+      : "memory", "m0");
 }
 // all but the last N copies of this wavefront have landed
 template <int N>
