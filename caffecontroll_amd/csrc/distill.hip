@@ -401,6 +401,9 @@ static int check_distill(const cct_distill_loss_args *a, const char *who) {
               a->tokens, a->vocab);
   CCT_REQUIRE(a->temperature > 0.0f && a->temperature < __builtin_inff(), "%s: temperature %g is not a positive number", who,
               (double)a->temperature);
+  // T^2, 1 / T and log2 e / T are normal numbers
+  CCT_REQUIRE(a->temperature >= 0x1p-60f && a->temperature <= 0x1p60f, "%s: temperature %g is not within 2^-60 to 2^60", who,
+              (double)a->temperature);
   CCT_REQUIRE((a->logits_stride == 0 || a->logits_stride >= (size_t)a->vocab) &&
                   (a->top_stride == 0 || a->top_stride >= (size_t)a->top),
               "%s: a row stride is smaller than its row", who);

@@ -599,7 +599,7 @@ int cct_hip_vocab_loss_forward_backward(float *loss, float *lse, void *dx, void 
 typedef struct cct_distill_loss_args {
   int tokens, vocab, top; /* top <= 1024 */
   int dtype;              /* of logits and dlogits; top_logits are fp32 */
-  float temperature;
+  float temperature;      /* 2^-60 to 2^60 */
   size_t logits_stride, top_stride; /* elements between rows of logits / dlogits and of both top lists; 0 = dense */
 } cct_distill_loss_args;
 size_t cct_hip_distill_loss_workspace_bytes(const cct_distill_loss_args *args);

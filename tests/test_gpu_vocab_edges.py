@@ -179,6 +179,30 @@ def test_distill_gradient_of_scores_of_any_size(dtype, tokens, vocab, temperatur
         near(some, np.tile(want, (some.shape[0], 1)), np.tile(bound + worse * (1 + HALF[dtype]), (some.shape[0], 1)))
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("vocab", [300, 9001])
+@pytest.mark.parametrize("temperature", [2.0 ** -60, 2.0 ** 60])
+def test_distill_loss_at_the_ends_of_the_temperatures(dtype, vocab, temperature):
+    """Cold: all of p on the largest score and of q on the teacher's largest.  Hot: both uniform."""
+    d = Distill(dtype, 2, vocab, 3, temperature=temperature)
+    d.z[:] = 0.0
+    d.z[:, 8] = 1.0
+    d.ids = np.tile([8, 20, -1], (2, 1))
+    d.tl = np.tile([0.5, 0.25, 9.0], (2, 1)).astype(np.float32)
+    d.gs = np.full(2, 1.0, np.float32)
+    d.upload()
+    cold = temperature < 1
+    want = np.zeros(vocab) if cold else np.full(vocab, 1.0 / vocab)
+    if not cold:
+        want[[8, 20]] -= 0.5
+    for both in (False, True):
+        d.run(both)
+        loss = 0.0 if cold else temperature ** 2 * np.log(vocab / 2)
+        near(values(d.o_loss), np.full(2, loss), abs(loss) * ((vocab / 256 + 200) * U * 2 + 2.0 ** -20))
+        near(values(d.o_d) / temperature, np.tile(want, (2, 1)),
+             ((vocab / 256 + 200) * U * 2 + 40 * U * np.log(vocab) + 2.0 ** -20 + 1.1 * HALF[dtype]) * np.tile(np.abs(want), (2, 1)))
+
+
 # ---- knobs that change while calls run ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("training", [False, True])
 def test_vocab_loss_while_another_thread_changes_its_tile(training):

@@ -147,3 +147,14 @@ def test_distill_loss_refuses_arrays_and_workspaces(drv):
         extra = [] if call == drv.distill_loss_forward else [None]
         refused(call, *[A] * n, *extra, a, A, need - 1, match="workspace")
         refused(call, *[A] * n, *extra, a, A + 2, need, match="workspace")
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-39, 2.0 ** -61, 2.0 ** 61, 3e38])
+def test_distill_loss_refuses_temperatures_whose_square_or_inverse_is_no_normal_number(drv, temperature):
+    a = distill_loss_args(tokens=4, vocab=10, top=3, temperature=temperature)
+    refused(drv.distill_loss_forward, A, A, A, A, A, a, A, 1 << 30, match="temperature")
+    refused(drv.distill_loss_backward, A, A, A, A, A, None, a, A, 1 << 30, match="temperature")
+    refused(drv.distill_loss_forward_backward, A, A, A, A, A, A, None, a, A, 1 << 30, match="temperature")
+    assert drv.distill_loss_workspace_bytes(a) == 0
+    for least in (2.0 ** -60, 2.0 ** 60):
+        assert drv.distill_loss_workspace_bytes(distill_loss_args(4, 10, 3, temperature=least)) > 0
