@@ -521,7 +521,8 @@ int cct_hip_softmax_loss_backward(float *in_grad, const float *prob, const float
  * reference; they stand beside the inner-product layer (cct_hip_sgemm_new_bias) and the softmax loss
  * (cct_hip_softmax_loss_forward), take matrices of fp32 or bf16 elements (every sum, softmax statistic and exponential in
  * fp32, one rounding where a result is stored), 32-bit ids and labels, rows `stride` elements apart (0 = dense; what
- * lies between the rows is neither read nor written), and a workspace of the caller's: it may hold anything before the
+ * lies between the rows is not written and counts for nothing; at most the other half of a dword that a bf16 row begins or
+ * ends in is read with it), and a workspace of the caller's: it may hold anything before the
  * call, must not be shared by calls that run at the same time, and nothing in it is needed after the call, so a captured graph
  * and an eager call, or two graphs, are independent as soon as their workspaces are.  Workspaces start at a multiple
  * of 16 bytes.  Results do not depend on timing: no floating-point atomics, fixed orders of summation.  Arguments
@@ -552,7 +553,8 @@ int cct_hip_embedding_backward(void *dtable, const void *dout, const int *ids, c
  *   lse[t] = log sum_v exp l[t][v],  loss[t] = lse[t] - l[t][labels[t]].
  * A token whose label is ignore_label has loss 0 and takes no part in any gradient (its row of x may hold anything);
  * its lse is still computed.  Any other label outside [0, vocab) is never used as an index: that token's loss is NaN, and its
- * gradient is that of the lse alone, as in cct_hip_softmax_loss_backward.  A bias of -inf masks its row of the vocabulary.
+ * gradient is that of the lse alone, as in cct_hip_softmax_loss_backward.  A bias of -inf masks its row of the vocabulary,
+ * whose w has to be finite all the same: dx takes it 0 times.
  * Gradients for G[t][v] = loss_grad[t] * (exp(l[t][v] - lse[t]) - [v == labels[t]]), loss_grad NULL = all ones:
  *   dx = G w,  dw = G^T x,  db = column sums of G;  any of the three may be NULL.
  * A loss_grad that is NaN or infinite reaches its own token's row of dx, and dw and db.
