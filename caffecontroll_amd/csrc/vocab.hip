@@ -56,8 +56,10 @@ typedef __attribute__((address_space(3))) char lds_char;
 // nothing and writes zeros.  The instruction itself instead of its builtin: the compiler would wait for all copies
 // in flight before every ds_read_b64_tr_b16, whose address it cannot tell from theirs (a product with such an operand: 1.43
 // instead of 0.83 ms).  It has no result register; copy_wait() and a barrier stand before the reads that need it.  M0 holds
-// the LDS address.
+// the LDS address; the compiler's warning that it keeps M0 for itself is why the asm says that it writes it.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, uint32_t offset, lds_char *dst) {
   const uint64_t at = (uint64_t)base;
   const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, kOutOfRange, 0x00020000u};
@@ -66,6 +68,7 @@ __device__ __forceinline__ void copy16(const char *base, uint32_t lane_offset, u
       "v"(lane_offset), "s"(rsrc), "s"(offset)
       : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // all but the last N copies of this wavefront have landed
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -1431,8 +1434,8 @@ static int launch_product(ProductArgs &p) {
   p.blocks = (uint32_t)blocks;
   kern<<<p.blocks, S::THREADS, bytes, ctx().stream>>>(p);
   CCT_LAUNCH_CHECK();
-  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d, %d>, %d, %s, %s> splits=%d", Num<T>::NAME, S::BM, S::BN, S::WM,
-              S::WN, S::STAGES, USE, KA ? "true" : "false", KB ? "true" : "false", p.splits);
+  note_kernel("vocab_product_kernel<%s, Shape<%d, %d, %d, %d, %d>, %d, %s, %s> splits=%d m=%d n=%d", Num<T>::NAME, S::BM, S::BN,
+              S::WM, S::WN, S::STAGES, USE, KA ? "true" : "false", KB ? "true" : "false", p.splits, p.M, p.N);
   return 0;
 }
 
