@@ -2,11 +2,10 @@
 the definitions in 64 bits with the bounds of test_gpu_vocab_ops."""
 import re
 
-import numpy as np
 import pytest
 
 from gpu_util import driver, tuning
-from test_gpu_vocab_ops import BOTH, Distill, Vocab, blank, ints, near, space, up, values
+from test_gpu_vocab_ops import BOTH, Distill, Vocab, blank, code, near, space, up, values
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +85,128 @@ def test_vocab_loss_with_tiles_of_256_in_several_bands(dtype, keep, piece, token
         v.both(piece)
         v.check_loss()
         v.check_gradients()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("keep", [0, 1, 2])
+@pytest.mark.parametrize("x_gap, w_gap", [(0, 3), (3, 0), (8, 3), (3, 8)])
+def test_vocab_loss_with_one_operand_packed(dtype, keep, x_gap, w_gap):
+    """Rows of whole 16-byte chunks in one of x and w, read as they lie, beside rows that are copied first."""
+    v = Vocab(dtype, 130, 128, 1111, bias=True)
+    v.xs, v.ws = (128 + g if g else 0 for g in (x_gap, w_gap))
+    v.x, _ = up(v.x64, dtype, v.xs)
+    v.w, _ = up(v.w64, dtype, v.ws)
+    v.reference()
+    with tuning("vocab_keep", keep):
+        for piece in (0, 256):
+            v.outputs(fill=5.0)
+            v.forward(piece)
+            v.check_loss()
+            v.backward(piece)
+            v.check_gradients()
+            v.outputs(fill=5.0)
+            v.both(piece)
+            v.check_loss()
+            v.check_gradients()
+            assert (values(v.o_dx)[:, 128:] == 5.0).all() and (values(v.o_dw)[:, 128:] == 5.0).all()
+
+
+def test_vocab_loss_gradients_in_pieces_past_four_gib():
+    """A matrix of 2.3e9 elements in pieces of 65536 rows, one of which begins at 4 GiB: scores computed twice, dx added up
+    over the pieces, and dw on both sides of that boundary."""
+    import torch
+    from caffecontroll_amd.driver import BF16, vocab_loss_args
+    drv, vocab, width, tokens, piece = driver(), 565000, 4096, 24, 65536
+    edge = 8 * piece                                               # bf16: 4 GiB from the start
+    rows = torch.cat([torch.arange(edge - 32, edge + 32), torch.arange(vocab - 64, vocab)]).cuda()
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    w = torch.zeros((vocab, width), dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(tokens, width, generator=gen, device="cuda").to(torch.bfloat16)
+    some = (torch.randn(len(rows), width, generator=gen, device="cuda") / 16).to(torch.bfloat16)
+    w[rows] = some
+    at = torch.arange(tokens, device="cuda") * 5                   # places in `rows`: labels on both sides, and in the last rows
+    labels = rows[at].to(torch.int32)
+    a = vocab_loss_args(tokens, width, vocab, BF16, piece=piece)
+    n = drv.vocab_loss_workspace_bytes(a)
+    ws = space(n)
+    loss, lse, db = blank((tokens,)), blank((tokens,)), blank((vocab,), "bf16")
+    dx, dw = blank((tokens, width), "bf16"), blank((vocab, width), "bf16")
+    bias = torch.zeros(vocab, dtype=torch.bfloat16, device="cuda")
+    drv.vocab_loss_forward_backward(loss, lse, dx, None, db, x, w, bias, labels, None, a, ws.ptr, n)
+    _, use, _, _ = last_product()
+    assert use == 2 and ws.intact()                                # dx in parts that are added up
+    drv.vocab_loss_forward_backward(loss, lse, dx, dw, db, x, w, bias, labels, None, a, ws.ptr, n)
+    assert last_product()[3] <= vocab - 8 * piece and ws.intact()  # the last piece's rows
+    x64, w64 = x.double(), some.double()
+    s = x64 @ w64.T
+    total = torch.exp(s).sum(1) + (vocab - len(rows))
+    want = torch.log(total)
+    # scores of a few hundred: 4096 terms of a fp32 sum, 4096 * 2^-24 of the terms' size
+    size = 2.5e-4 * (x64.abs() @ w64.abs().T).amax(1)
+    near(values(lse), values(want), values(size))
+    near(values(loss), values(want - s[torch.arange(tokens), at]), 2 * values(size))
+    g = torch.exp(s - want[:, None])
+    g[torch.arange(tokens), at] -= 1.0
+    rest = 1.0 / total                                             # G of every row that is zero
+    # G: the scores' and lse's error, a rounding to bf16 of each entry and of the result
+    eg = g.abs() * (2 * size[:, None] + 2.0 ** -8) + (g + 1).abs() * 2 * size[:, None]
+    erest = rest * (2 * size + 2.0 ** -8)
+    wdx = g @ w64
+    edx = eg @ w64.abs()
+    near(values(dx), values(wdx), values(edx + 2.0 ** -8 * (wdx.abs() + edx)) + 1e-30)
+    wdw, edw = g.T @ x64, eg.T @ x64.abs()
+    near(values(dw[rows]), values(wdw), values(edw + 2.0 ** -8 * (wdw.abs() + edw)) + 1e-30)
+    wz, ez = rest @ x64, erest @ x64.abs()
+    ez = ez + 2.0 ** -8 * (wz.abs() + ez) + 1e-30
+    for r in (0, piece - 1, piece, edge - 33, edge + 32, edge + piece // 2, vocab - 65):
+        near(values(dw[r]), values(wz), values(ez))
+    for p in range(0, vocab, piece):                               # every row that is zero has the same gradient
+        part = dw[p:p + piece]
+        other = (part != dw[0]).any(1).nonzero()[:, 0] + p
+        assert set(other.tolist()) <= set(rows.tolist())
+    wdb, edb = g.sum(0), eg.sum(0)
+    near(values(db[rows]), values(wdb), values(edb + 2.0 ** -8 * (wdb.abs() + edb)))
+    assert float(db[7]) == float(db[edge + 100]) == float(db[vocab - 100])
+
+
+@pytest.mark.parametrize("tokens, width, vocab, top", [(347, 712, 45383, 5), (33, 1008, 49742, 3)])
+def test_calls_with_a_second_launch_in_a_replayed_graph(tokens, width, vocab, top):
+    from test_gpu_vocab_model import test_every_call_in_a_replayed_graph as replay
+    with tuning("vocab_keep", 2):
+        replay(tokens, width, vocab, top)
+
+
+# ---- distillation ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("tokens, vocab, top", [(5, 9, 2), (40, 300, 20), (3, 9001, 300), (2, 65536, 7), (3, 140000, 5)])
+def test_distill_loss_on_columns_of_wider_matrices(dtype, tokens, vocab, top):
+    """Rows that start at an element's alignment: the scores, their gradient and both lists are views from the second column on."""
+    import torch
+    from caffecontroll_amd.driver import distill_loss_args
+    drv, d = driver(), Distill(dtype, tokens, vocab, top).upload().reference()
+
+    def view(t, gap, fill):
+        whole = torch.full((t.shape[0], t.shape[1] + gap), fill, dtype=t.dtype, device="cuda")
+        whole[:, 1:1 + t.shape[1]] = t
+        return whole, whole[:, 1:1 + t.shape[1]]
+
+    _, z = view(d.z, 6, float("nan"))
+    _, ids = view(d.d_ids, 4, 2 ** 31 - 1)
+    _, tl = view(d.d_tl, 4, float("nan"))
+    a = distill_loss_args(tokens, vocab, top, code(dtype), d.T, vocab + 6, top + 4)
+    n = drv.distill_loss_workspace_bytes(a)
+    gs = up(d.gs)[0]
+    for both in (False, True):
+        for in_place in (False, True):
+            ws = space(n)
+            d.outputs()
+            dw, dz = view(z if in_place else torch.zeros_like(d.z), 6, 5.0)
+            source = dz if in_place else z
+            if both:
+                drv.distill_loss_forward_backward(d.o_loss, d.o_lse, dz, source, ids, tl, gs, a, ws.ptr, n)
+            else:
+                drv.distill_loss_forward(d.o_loss, d.o_lse, source, ids, tl, a, ws.ptr, n)
+                drv.distill_loss_backward(dz, source, ids, tl, d.o_lse, gs, a, ws.ptr, n)
+            d.o_d = dz
+            d.check()
+            assert (dw[:, 0] == 5.0).all() and (dw[:, vocab + 1:] == 5.0).all() and ws.intact()
