@@ -750,10 +750,14 @@ static int embedding_backward(void *dtable, const void *dout, const int *ids, Em
   float *parts = (float *)(ws + w.parts);
   EmbRun *runs = (EmbRun *)(ws + w.runs);
   const bool ranked = s.tokens <= EMB_RANK_MAX;
-  // Visiting only the rows with tokens writes those twice; looking every row's tokens up costs those that have none.
-  // 131072 rows of 4096 bf16, 65536 tokens as text has them (a fifth of the rows): 367 and 421 us; all of them different (half
-  // of the rows): 394 and 369 us.  With more tokens than half the rows the second way is taken.
-  const bool visit = ranked || s.tokens <= s.vocab / 2;
+  // Visiting only the rows with tokens writes those twice; looking every row's tokens up costs a search a row.  Rows of less
+  // than 4 KB: the search is the larger (131072 rows of 1024 bf16, 16384 to 524288 tokens as text has them: 81 to 525 us visited,
+  // 121 to 687 looked up; all different or uniform 74 to 452, 114 to 565; rows of 512 bytes to 2 KB alike, by up to 1.8; one of 34
+  // sizes 4 % the other way).  Longer rows: by how many have tokens, which only the ids say.  131072 rows of 4096 bf16,
+  // tokens as text has them: 225, 273, 373 (0.15 of the rows), 546 us (0.25) visited for 16384, 32768, 65536, 131072 tokens, 250,
+  // 311, 420, 589 looked up; all different: 225, 268, 402, 604 and 237, 228, 368, 493.  fp32, 16384 rows of 4096, as many
+  // tokens: 128 and 138, all different 145 and 113.  From more tokens than half the rows they are looked up.
+  const bool visit = ranked || s.width * sizeof(T) < 4096 || s.tokens <= s.vocab / 2;
   const unsigned clear_blocks = accumulate || !visit ? 0u : clear_blocks_of(s, Num<T>::V);
   uint32_t *keys = (uint32_t *)(ws + w.keys[0]);
   int *order = (int *)(ws + w.order[0]);

@@ -2,10 +2,11 @@
 the definitions in 64 bits with the bounds of test_gpu_vocab_ops."""
 import re
 
+import numpy as np
 import pytest
 
 from gpu_util import driver, tuning
-from test_gpu_vocab_ops import BOTH, Distill, Vocab, blank, code, near, space, up, values
+from test_gpu_vocab_ops import BOTH, HALF, U, Distill, Vocab, blank, code, ints, near, space, up, values
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +211,44 @@ def test_distill_loss_on_columns_of_wider_matrices(dtype, tokens, vocab, top):
             d.o_d = dz
             d.check()
             assert (dw[:, 0] == 5.0).all() and (dw[:, vocab + 1:] == 5.0).all() and ws.intact()
+
+
+# ---- embedding -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, width", [("f32", 1029), ("bf16", 2051), ("f32", 1023), ("bf16", 2047)])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("tokens, vocab, kind, gap", [(8200, 700, "skewed", 0), (9001, 16500, "uniform", 3), (8193, 33, "one", 0),
+                                                      (8300, 16700, "uniform", 0)])
+def test_embedding_gradient_by_rows_and_by_tokens(dtype, width, accumulate, tokens, vocab, kind, gap):
+    """Every row's tokens looked up (rows of 4 KB and more, more tokens than half the rows), or the rows with tokens visited."""
+    from caffecontroll_amd.driver import embedding_args
+    drv, rng = driver(), np.random.default_rng(tokens + width)
+    stride = width + gap if gap else 0
+    ids = {"skewed": np.minimum(rng.zipf(1.3, tokens) - 1, vocab - 1), "uniform": rng.integers(0, vocab, tokens),
+           "one": np.full(tokens, vocab - 1)}[kind]
+    if kind != "one":
+        ids[[5, 50, 60]] = -1, vocab, -7
+    dout, d64 = up(rng.standard_normal((tokens, width)), dtype, stride)
+    table, old = up(rng.standard_normal((vocab, width)), dtype, stride, 3.0)
+    args = embedding_args(tokens, width, vocab, code(dtype), 0.3, -1, stride, stride)
+    n = drv.embedding_workspace_bytes(args)
+    ws = space(n)
+    drv.embedding_backward(table, dout, ints(ids), args, ws.ptr, n, accumulate)
+    by_rows = width > 1024 + 1024 * (dtype == "bf16") and tokens > vocab // 2
+    assert drv.lib.cct_hip_last_kernel().decode().startswith("embedding_sum_kernel<" if by_rows else "embedding_runs_kernel<")
+    got = values(table)
+    assert ws.intact() and (got[:, width:] == 3.0).all()
+    ok = (ids >= 0) & (ids < vocab)
+    count = np.bincount(ids[ok], minlength=vocab)
+    order = np.argsort(ids[ok], kind="stable")
+    begin = np.concatenate([[0], np.cumsum(count)[:-1]])
+    some = count > 0
+    total, size = np.zeros((vocab, width)), np.zeros((vocab, width))
+    total[some] = np.add.reduceat(d64[ok][order], begin[some])
+    size[some] = np.add.reduceat(np.abs(d64[ok][order]), begin[some])
+    s32 = float(np.float32(0.3))
+    want = s32 * total + (old if accumulate else 0.0)
+    # count additions, the product with the scale, the addition to what was there, the rounding to the type
+    bound = s32 * (count[:, None] + 1) * U * size * (1 + 1e-3) + (U * np.abs(want) if accumulate else 0)
+    near(got[:, :width], want, bound + HALF[dtype] * (np.abs(want) + bound))
+    if accumulate:
+        assert (got[:, :width][~some] == old[~some]).all()
