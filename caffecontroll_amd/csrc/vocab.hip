@@ -678,7 +678,7 @@ __device__ __forceinline__ void largest_weight(float *__restrict__ wmax, float *
 // x as dw's operand, zero for ignored tokens, so that whatever their x holds stays out of the product.  bf16: transposed,
 // xt[c][t] = x[t][c] for t < tpad (zero past the end), since a transposed read of both operands from LDS is slower than
 // of one.  fp32: xl[t][c] for c < cpad.  With weights, one workgroup more takes the largest of them.  HBM, and a few
-// microseconds beside the products: 53 us for 8192 x 4096 bf16 transposed, 11 us for 2048 x 1024 fp32.
+// microseconds beside the products: 42 us for 8192 x 4096 bf16 transposed, 9 us for 2048 x 1024 fp32.
 template <class T>
 __global__ __launch_bounds__(256) void vocab_live_kernel(T *__restrict__ xl, const T *__restrict__ x, size_t ldx, int tokens,
                                                          int width, int cpad, const int *__restrict__ labels, int ignore,
