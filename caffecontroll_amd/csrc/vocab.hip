@@ -506,7 +506,7 @@ __global__ __launch_bounds__(S::THREADS) void vocab_product_kernel(ProductArgs p
         if (here) p.label_score[t] = score;
       }
       const float base = st.m == neg_inf() ? 0.0f : st.m;
-      if (__any(fabsf(base) > kScaledMax)) {
+      if (MI == 1 || __any(fabsf(base) > kScaledMax)) {  // (four scores: the correction below costs more than it saves)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
