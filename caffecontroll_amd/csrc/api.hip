@@ -18,6 +18,7 @@ static std::mutex g_mu;
 static thread_local char g_err[512] = "";
 
 Context &ctx() { return g_ctx; }
+
 static void read_tuning_from_env() {
   auto geti = [](const char *name, int dflt) {
     const char *e = getenv(name);
